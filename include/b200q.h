@@ -297,6 +297,50 @@ int32_t b200q_decode_attention_static(const void* q, const void* cache_k, const 
  * device-side assertion there). */
 int32_t b200q_decoder_status(void);
 
+/* ---- sampling many answers to one prompt ------------------------------------------
+ * No reference counterpart: the reference lowers rotary embedding, attention and
+ * log-softmax to PyTorch calls (examples/01-llama/src/attention.linnet). */
+
+/* Rotary positions of q [tokens, nq, head_dim] and k [tokens, nkv, head_dim] (nkv = 0: none),
+ * bf16 or f16: the first 2 * pairs numbers of a head, as pairs of the two halves (layout 0:
+ * numbers i and i + pairs) or of neighbours (layout 1: 2i and 2i + 1), are turned by
+ * positions[token] * frequencies[pair] (radians, f64) and multiplied by `factor`; the others
+ * are copied.  Angles are formed in f64.  Strides of tokens and heads are in numbers; an
+ * output may be its input, and otherwise must not overlap any tensor of the call.  head_dim
+ * up to 1024. */
+int32_t b200q_rotary(const void* q, const void* k, const int64_t* positions,
+                     const double* frequencies, void* q_out, void* k_out, int64_t tokens,
+                     int64_t nq, int64_t nkv, int64_t head_dim, int64_t pairs, int64_t q_token,
+                     int64_t q_head, int64_t k_token, int64_t k_head, int64_t q_out_token,
+                     int64_t q_out_head, int64_t k_out_token, int64_t k_out_head, float factor,
+                     int32_t layout, int32_t dtype, void* stream);
+
+/* b200q_rope_cache with the positions of b200q_rotary: qkv [batch, (nq + 2 nkv) * head_dim] of
+ * one token a row; keys and values go to slot positions[b] of cache_{k,v}[batch, nkv, max_seq,
+ * head_dim], queries to q_out [batch, nq, head_dim]; the angle is that of positions[b] plus
+ * `offset`, or plus *offset_at (a device word) where that is given.  A position outside the
+ * cache stores nothing and is recorded for b200q_decoder_status(). */
+int32_t b200q_rotary_cache(const void* qkv, const int64_t* positions, const double* frequencies,
+                           const int64_t* offset_at, int64_t offset, void* q_out, void* cache_k,
+                           void* cache_v, int64_t batch, int64_t nq, int64_t nkv,
+                           int64_t head_dim, int64_t pairs, int64_t max_seq, float factor,
+                           int32_t layout, int32_t dtype, void* stream);
+
+/* A table for b200q_rope_attention: [max_seq, pairs] of factor * (cos, sin) f32. */
+int32_t b200q_rotary_table(void* table, const double* frequencies, int64_t max_seq,
+                           int64_t pairs, float factor, void* stream);
+
+/* Of every row of logits [rows, vocab] (f32, bf16 or f16; rows `stride` elements apart, vocab
+ * up to 2^20): the log probability of tokens[row] (a negative token: none was given, 0; one
+ * past the vocabulary: NaN, and recorded for b200q_decoder_status()), the entropy in nats, and
+ * the `top` (0 to 32) largest logits as log probabilities with their tokens [rows, top], larger
+ * ones first and the lower index first among equals; f32 and int64 out.  Logits of -inf have
+ * probability 0; a row that holds NaN or +inf, or nothing else than -inf, gives NaN. */
+int32_t b200q_token_logprobs(const void* logits, const int64_t* tokens, float* logprob,
+                             float* entropy, float* top_logprob, int64_t* top_token, int64_t rows,
+                             int64_t vocab, int64_t stride, int64_t top, int32_t dtype,
+                             void* stream);
+
 /* out[rows, inner] = silu(gate_up[:, :inner]) * gate_up[:, inner:], silu rounded to
  * bf16 before the product as the two PyTorch ops round. */
 int32_t b200q_silu_mul(const void* gate_up, void* out, int64_t rows, int64_t inner,

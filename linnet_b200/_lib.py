@@ -63,6 +63,14 @@ PROTOTYPES: dict[str, list] = {
     "b200q_decoder_status": [],
     "b200q_set_wait_limit_ns": [c_int64],
     "b200q_silu_mul": [c_void_p, c_void_p, c_int64, c_int64, c_void_p],
+    "b200q_rotary": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64,
+                     c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_float, c_int32,
+                     c_int32, c_void_p],
+    "b200q_rotary_cache": [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64,
+                           c_int64, c_int64, c_int64, c_int64, c_int64, c_float, c_int32, c_int32, c_void_p],
+    "b200q_rotary_table": [c_void_p, c_void_p, c_int64, c_int64, c_float, c_void_p],
+    "b200q_token_logprobs": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64,
+                             c_int64, c_int32, c_void_p],
     "b200q_tp_allreduce_add_rmsnorm_flags": [c_void_p, c_void_p, c_int64, c_int64, c_int32, c_int32, c_void_p,
                                              c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
                                              c_float, c_void_p],

@@ -1,13 +1,23 @@
 """PyTorch-facing wrappers of the decode-step glue kernels (`csrc/decoder_glue.cu`):
 residual add + RMSNorm, rotary embedding + KV-cache write, single-query attention over
 the cache, and SwiGLU's `silu(gate) * up`.  bf16 CUDA tensors only; launches go to the
-current stream and record into CUDA graphs."""
+current stream and record into CUDA graphs.
+
+For many answers to one prompt, bf16 or f16: rotary positions of any frequencies, layout and part
+of a head (`csrc/rotary.cu`: `rotary`, `rotary_cache`, `rotary_table`; `rope_frequencies` makes the
+frequencies), attention over one shared prefix and each row's own cache
+(`csrc/prefix_attention.cu`: `prefix_attention`), and log probabilities of given tokens with entropy
+and alternatives (`csrc/token_logprobs.cu`: `token_logprobs`).  These have no derivative and refuse
+tensors that ask for one."""
 
 from __future__ import annotations
 
+from typing import NamedTuple
+
 import torch
 
-from . import _lib
+from . import _lib, rope
+from .kernels import _CODES, _Device, _raw_stream
 
 
 def _stream(t: torch.Tensor) -> int:
@@ -131,3 +141,174 @@ def silu_mul(gate_up: torch.Tensor) -> torch.Tensor:
     out = torch.empty(rows, width // 2, device=gate_up.device, dtype=gate_up.dtype)
     _lib.check(_lib.load().b200q_silu_mul(gate_up.data_ptr(), out.data_ptr(), rows, width // 2, _stream(gate_up)))
     return out
+
+
+# ---- many answers to one prompt --------------------------------------------------------------
+
+_LAYOUTS = {"half": 0, "interleaved": 1}
+
+
+def _same(who: str, kinds: tuple[torch.dtype, ...], *tensors: torch.Tensor) -> torch.device:
+    """One CUDA device, one of `kinds`, last dimension contiguous, no derivative asked for."""
+    first = tensors[0]
+    for t in tensors:
+        if not t.is_cuda or t.get_device() != first.get_device() or t.dtype != first.dtype or t.dtype not in kinds:
+            names = ", ".join(str(k).removeprefix("torch.") for k in kinds)
+            raise RuntimeError(f"{who} takes CUDA tensors of one device and one of the types {names}; got "
+                               f"{[f'{t.dtype} on {t.device}' for t in tensors]}")
+        if t.stride(-1) != 1 and t.numel() > 0 and t.shape[-1] > 1:
+            raise RuntimeError(f"{who}: the last dimension has to be contiguous")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{who} has no derivative: detach its inputs or call it under torch.no_grad()")
+    return first.device
+
+
+_HALF = (torch.bfloat16, torch.float16)
+_LOGITS = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def _contiguous(who: str, *tensors: torch.Tensor) -> None:
+    for t in tensors:
+        if not t.is_contiguous():
+            raise RuntimeError(f"{who} takes contiguous caches and projections")
+
+
+def _frequencies(who: str, frequencies: torch.Tensor, head_dim: int, device: torch.device) -> int:
+    """Read on the device as f64: anything else would be misread."""
+    if (frequencies.device != device or frequencies.dtype != torch.float64 or not frequencies.is_contiguous()
+            or frequencies.dim() != 1 or not 1 <= frequencies.numel() <= head_dim // 2):
+        raise ValueError(f"{who}: frequencies must be a contiguous float64 tensor of 1 to {head_dim // 2} entries on "
+                         f"{device}, not {frequencies.dtype}{list(frequencies.shape)} on {frequencies.device}")
+    return frequencies.numel()
+
+
+def _layout(who: str, layout: str) -> int:
+    if layout not in _LAYOUTS:
+        raise ValueError(f"{who}: layout is 'half' or 'interleaved', not {layout!r}")
+    return _LAYOUTS[layout]
+
+
+def _word(who: str, name: str, value: "int | torch.Tensor", device: torch.device) -> tuple[int | None, int]:
+    """A number known on the host, or one int64 word on the device: (address or None, number)."""
+    if not isinstance(value, torch.Tensor):
+        return None, int(value)
+    if value.device != device or value.dtype != torch.int64 or value.numel() != 1:
+        raise ValueError(f"{who}: {name} must be a number or one int64 on {device}, not "
+                         f"{value.dtype}{list(value.shape)} on {value.device}")
+    return value.data_ptr(), 0
+
+
+def rope_frequencies(rotary_dim: int, theta: float, *, scaling: "rope.RopeScaling | None" = None,
+                     device: "torch.device | str" = "cuda") -> tuple[torch.Tensor, float]:
+    """Frequencies f64 [rotary_dim / 2] on `device` and the factor on cosine and sine, for `rotary`,
+    `rotary_cache` and `rotary_table` (`rope.RopeScaling` says which scalings there are)."""
+    numbers, factor = rope.frequencies(rotary_dim, theta, scaling)
+    return torch.tensor(numbers, dtype=torch.float64, device=device), factor
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, frequencies: torch.Tensor, *,
+           layout: str = "half", factor: float = 1.0,
+           out: "tuple[torch.Tensor, torch.Tensor | None] | None" = None) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """Rotary positions of a prompt: q [T, nq, D] and k [T, nkv, D] (or None), bf16 or f16, rows and
+    heads at any stride (views of a fused projection).  The first `2 * len(frequencies)` numbers of
+    every head, as pairs of the two halves ("half") or of neighbours ("interleaved"), are turned by
+    positions[t] * frequencies[pair] and multiplied by `factor`; the others are copied.  `out`: where
+    the results go, (q, k) themselves to turn in place; other overlaps are not allowed."""
+    tensors = (q,) if k is None else (q, k)
+    device = _same("rotary", _HALF, *tensors)
+    if q.dim() != 3 or (k is not None and (k.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2])):
+        raise ValueError(f"rotary: q is [tokens, heads, D] and k the same, not {[list(t.shape) for t in tensors]}")
+    tokens, nq, hd = q.shape
+    _positions(positions, tokens, device)
+    pairs = _frequencies("rotary", frequencies, hd, device)
+    code = _layout("rotary", layout)
+    if out is None:
+        q_out, k_out = torch.empty(q.shape, dtype=q.dtype, device=device), None
+        if k is not None:
+            k_out = torch.empty(k.shape, dtype=k.dtype, device=device)
+    else:
+        q_out, k_out = out
+        if q_out.shape != q.shape or (k is None) != (k_out is None) or (k is not None and k_out.shape != k.shape):
+            raise ValueError("rotary: out has to have the shapes of q and k")
+        _same("rotary", _HALF, q, q_out, *(() if k is None else (k_out,)))
+    given, made = (q, q if k is None else k), (q_out, q_out if k is None else k_out)
+    strides = [t.stride(d) for t in (*given, *made) for d in (0, 1)]
+    with _Device(device):
+        _lib.check(_lib.load().b200q_rotary(
+            q.data_ptr(), None if k is None else k.data_ptr(), positions.data_ptr(), frequencies.data_ptr(),
+            q_out.data_ptr(), None if k is None else k_out.data_ptr(), tokens, nq, 0 if k is None else k.shape[1], hd,
+            pairs, *strides, factor, code, _CODES[q.dtype], _raw_stream(device.index)))
+    return q_out, k_out
+
+
+def rotary_cache(qkv: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, cache_k: torch.Tensor,
+                 cache_v: torch.Tensor, nq: int, nkv: int, *, layout: str = "half", factor: float = 1.0,
+                 offset: "int | torch.Tensor" = 0) -> torch.Tensor:
+    """`rope_cache` with the positions of `rotary`, bf16 or f16: turns q and k of qkv
+    [B, (nq + 2 nkv) * D] by (positions[b] + offset) * frequencies, writes k and v into the caches
+    [B, nkv, S, D] at slot positions[b] and returns q [B, nq, D].  `offset` (a number, or one int64 on
+    the device) is where a row's own cache begins: the length of the prefix it shares.  A position
+    outside the cache stores nothing and is reported by `decoder_status`."""
+    device = _same("rotary_cache", _HALF, qkv, cache_k, cache_v)
+    _contiguous("rotary_cache", qkv, cache_k, cache_v)
+    batch = qkv.shape[0]
+    if (cache_k.dim() != 4 or cache_k.shape != cache_v.shape or cache_k.shape[:2] != (batch, nkv)
+            or qkv.shape != (batch, (nq + 2 * nkv) * cache_k.shape[3])):
+        raise ValueError(f"rotary_cache: qkv {list(qkv.shape)} of {nq} and {nkv} heads and caches "
+                         f"{list(cache_k.shape)}, {list(cache_v.shape)} do not go together")
+    _positions(positions, batch, device)
+    _, _, max_seq, hd = cache_k.shape
+    pairs = _frequencies("rotary_cache", frequencies, hd, device)
+    code = _layout("rotary_cache", layout)
+    at, number = _word("rotary_cache", "offset", offset, device)
+    q = torch.empty(batch, nq, hd, device=device, dtype=qkv.dtype)
+    with _Device(device):
+        _lib.check(_lib.load().b200q_rotary_cache(
+            qkv.data_ptr(), positions.data_ptr(), frequencies.data_ptr(), at, number, q.data_ptr(), cache_k.data_ptr(),
+            cache_v.data_ptr(), batch, nq, nkv, hd, pairs, max_seq, factor, code, _CODES[qkv.dtype],
+            _raw_stream(device.index)))
+    return q
+
+
+def rotary_table(max_seq: int, frequencies: torch.Tensor, factor: float = 1.0) -> torch.Tensor:
+    """(cos, sin) * factor of positions 0 .. max_seq - 1, f32 [max_seq, len(frequencies), 2]: what
+    `rope_attention` takes, for frequencies of any scaling (of whole heads, halves turned)."""
+    device = frequencies.device
+    if device.type != "cuda" or max_seq < 1:
+        raise ValueError(f"rotary_table: {max_seq} positions, frequencies on {device}")
+    pairs = _frequencies("rotary_table", frequencies, 1024, device)
+    table = torch.empty(max_seq, pairs, 2, dtype=torch.float32, device=device)
+    with _Device(device):
+        _lib.check(_lib.load().b200q_rotary_table(table.data_ptr(), frequencies.data_ptr(), max_seq, pairs, factor,
+                                                  _raw_stream(device.index)))
+    return table
+
+
+class TokenLogprobs(NamedTuple):
+    logprob: torch.Tensor       # f32 [rows]: of the tokens given
+    entropy: torch.Tensor       # f32 [rows], in nats
+    top_logprobs: torch.Tensor  # f32 [rows, top], the most probable first
+    top_tokens: torch.Tensor    # int64 [rows, top]
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> TokenLogprobs:
+    """Log probabilities of tokens [rows] under softmax(logits [rows, vocab]), the entropy of every row
+    and its `top` (up to 32) most probable tokens with theirs, the lower index first among equals.
+    Logits are f32, bf16 or f16, rows at any stride; -inf is a forbidden token.  A negative token
+    stands for none (log probability 0: padded rows drop out of sums); one past the vocabulary gives
+    NaN and is reported by `decoder_status`."""
+    device = _same("token_logprobs", _LOGITS, logits)
+    if logits.dim() != 2 or not 0 < logits.shape[1]:
+        raise ValueError(f"token_logprobs: logits are [rows, vocab], not {list(logits.shape)}")
+    rows, vocab = logits.shape
+    if (tokens.device != device or tokens.dtype != torch.int64 or tokens.shape != (rows,) or not tokens.is_contiguous()):
+        raise ValueError(f"token_logprobs: tokens must be a contiguous int64 tensor of {rows} entries on {device}, not "
+                         f"{tokens.dtype}{list(tokens.shape)} on {tokens.device}")
+    numbers = torch.empty(rows * (2 + max(top, 0)), dtype=torch.float32, device=device)
+    index = torch.empty(rows, max(top, 0), dtype=torch.int64, device=device)
+    logprob, entropy, best = numbers[:rows], numbers[rows:2 * rows], numbers[2 * rows:].view(rows, max(top, 0))
+    with _Device(device):
+        _lib.check(_lib.load().b200q_token_logprobs(
+            logits.data_ptr(), tokens.data_ptr(), logprob.data_ptr(), entropy.data_ptr(), best.data_ptr(),
+            index.data_ptr(), rows, vocab, logits.stride(0), top, _CODES[logits.dtype], _raw_stream(device.index)))
+    return TokenLogprobs(logprob, entropy, best, index)
