@@ -330,6 +330,29 @@ int32_t b200q_rotary_cache(const void* qkv, const int64_t* positions, const doub
 int32_t b200q_rotary_table(void* table, const double* frequencies, int64_t max_seq,
                            int64_t pairs, float factor, void* stream);
 
+/* Single-query attention of a batch whose rows share a prefix: q [batch, nq, head_dim] over the
+ * first `prefix` (or *prefix_at, a device word) keys of prefix_{k,v}[nkv, prefix, head_dim] and
+ * then positions 0 .. positions[b] of cache_{k,v}[batch, nkv, max_seq, head_dim]; out
+ * [batch, nq * head_dim], bf16 or f16, head_dim 64 or 128, nq / nkv any whole number up to 128.
+ *   positions: -1 where a row has no keys of its own; a row without any key gives zeros.  A
+ *     position outside -1 .. max_seq-1 counts as -1 and is recorded for b200q_decoder_status(); a
+ *     prefix length outside 0 .. prefix counts as the nearer end and is recorded as row 0.
+ *   strides: HOST array of 12, in numbers, multiples of 8: q's rows and heads; keys and heads of
+ *     prefix_k, of prefix_v; keys, heads and rows of cache_k, of cache_v.
+ *   scratch: device memory of b200q_prefix_attention_scratch_bytes(...) bytes (-1: a shape that is
+ *     not taken), 16-byte aligned, of this call until it is done; nothing in it needs clearing.
+ *   scale: positive.
+ *   What lies behind the last key of a prefix or cache may hold anything, NaN too.
+ * Two launches.  A bounded wait that expires is reported by b200q_int4_gemm_status(). */
+int64_t b200q_prefix_attention_scratch_bytes(int64_t batch, int64_t nq, int64_t nkv,
+                                             int64_t head_dim, int64_t prefix, int64_t max_seq);
+int32_t b200q_prefix_attention(const void* q, const void* prefix_k, const void* prefix_v,
+                               const void* cache_k, const void* cache_v, const int64_t* positions,
+                               const int64_t* prefix_at, void* out, void* scratch, int64_t batch,
+                               int64_t nq, int64_t nkv, int64_t head_dim, int64_t prefix,
+                               int64_t max_seq, const int64_t* strides, float scale, int32_t dtype,
+                               void* stream);
+
 /* Of every row of logits [rows, vocab] (f32, bf16 or f16; rows `stride` elements apart, vocab
  * up to 2^20): the log probability of tokens[row] (a negative token: none was given, 0; one
  * past the vocabulary: NaN, and recorded for b200q_decoder_status()), the entropy in nats, and

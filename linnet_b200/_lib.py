@@ -69,6 +69,9 @@ PROTOTYPES: dict[str, list] = {
     "b200q_rotary_cache": [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64,
                            c_int64, c_int64, c_int64, c_int64, c_int64, c_float, c_int32, c_int32, c_void_p],
     "b200q_rotary_table": [c_void_p, c_void_p, c_int64, c_int64, c_float, c_void_p],
+    "b200q_prefix_attention_scratch_bytes": [c_int64, c_int64, c_int64, c_int64, c_int64, c_int64],
+    "b200q_prefix_attention": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                               c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_float, c_int32, c_void_p],
     "b200q_token_logprobs": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64,
                              c_int64, c_int32, c_void_p],
     "b200q_tp_allreduce_add_rmsnorm_flags": [c_void_p, c_void_p, c_int64, c_int64, c_int32, c_int32, c_void_p,

@@ -12,6 +12,7 @@ tensors that ask for one."""
 
 from __future__ import annotations
 
+import ctypes
 from typing import NamedTuple
 
 import torch
@@ -282,6 +283,52 @@ def rotary_table(max_seq: int, frequencies: torch.Tensor, factor: float = 1.0) -
         _lib.check(_lib.load().b200q_rotary_table(table.data_ptr(), frequencies.data_ptr(), max_seq, pairs, factor,
                                                   _raw_stream(device.index)))
     return table
+
+
+def prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor, cache_k: torch.Tensor,
+                     cache_v: torch.Tensor, positions: torch.Tensor, *, prefix_length: "torch.Tensor | None" = None,
+                     scale: float | None = None) -> torch.Tensor:
+    """Attention of one query per row, q [B, nq, D], over a prefix that all rows share, keys and values
+    [nkv, P, D] (read once for the batch), and then over positions 0..positions[b] of each row's own
+    cache [B, nkv, S, D]; returns [B, nq * D].  bf16 or f16, D 64 or 128, nq / nkv up to 128; `scale`, a
+    positive number, is D**-0.5 unless given.  A position of -1 is a row without keys of its own; one outside the cache
+    counts as that and is reported by `decoder_status`.  `prefix_length`: one int64 on the device, how
+    many of the P positions there are (a captured step can be replayed on another prompt).  The last
+    dimension is contiguous, other strides are multiples of 8 numbers (parts of longer caches)."""
+    device = _same("prefix_attention", _HALF, q, prefix_k, prefix_v, cache_k, cache_v)
+    if (q.dim() != 3 or prefix_k.dim() != 3 or cache_k.dim() != 4 or prefix_k.shape != prefix_v.shape
+            or cache_k.shape != cache_v.shape or cache_k.shape[:2] != (q.shape[0], prefix_k.shape[0])
+            or not q.shape[2] == prefix_k.shape[2] == cache_k.shape[3]):
+        raise ValueError(f"prefix_attention: q {list(q.shape)}, a prefix {list(prefix_k.shape)}, {list(prefix_v.shape)} and "
+                         f"caches {list(cache_k.shape)}, {list(cache_v.shape)} do not go together")
+    batch, nq, hd = q.shape
+    nkv, prefix = prefix_k.shape[:2]
+    _positions(positions, batch, device)
+    at = None
+    if prefix_length is not None:
+        at, _ = _word("prefix_attention", "prefix_length", prefix_length, device)
+        if at is None:
+            raise ValueError("prefix_attention: prefix_length is one int64 on the device (or cut the prefix to its length)")
+    strides = (*_steps(q, 0, 1), *_steps(prefix_k, 1, 0), *_steps(prefix_v, 1, 0), *_steps(cache_k, 2, 1, 0),
+               *_steps(cache_v, 2, 1, 0))
+    lib = _lib.load()
+    with _Device(device):
+        size = lib.b200q_prefix_attention_scratch_bytes(batch, nq, nkv, hd, prefix, cache_k.shape[2])
+        if size < 0:
+            raise ValueError(_lib.last_error())
+        scratch = torch.empty(size, dtype=torch.uint8, device=device)
+        out = torch.empty(batch, nq * hd, dtype=q.dtype, device=device)
+        _lib.check(lib.b200q_prefix_attention(
+            q.data_ptr(), prefix_k.data_ptr(), prefix_v.data_ptr(), cache_k.data_ptr(), cache_v.data_ptr(),
+            positions.data_ptr(), at, out.data_ptr(), scratch.data_ptr(), batch, nq, nkv, hd, prefix, cache_k.shape[2],
+            (ctypes.c_int64 * 12)(*strides), hd ** -0.5 if scale is None else scale, _CODES[q.dtype],
+            _raw_stream(device.index)))
+    return out
+
+
+def _steps(t: torch.Tensor, *dims: int) -> tuple[int, ...]:
+    """Strides of dims; that of a dimension of one means nothing."""
+    return tuple(t.stride(d) if t.shape[d] > 1 else 0 for d in dims)
 
 
 class TokenLogprobs(NamedTuple):
