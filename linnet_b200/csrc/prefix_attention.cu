@@ -38,8 +38,11 @@ using namespace umma;
 
 constexpr int kKeys = 128;                 // of a tile
 constexpr int kRows = 128;                 // of a group's products
-constexpr int kProducerWarp = 8, kIssuerWarp = 9, kQueryWarp = 10;
-constexpr int kThreads = 11 * 32;
+constexpr int kProducerWarp = 8, kIssuerWarp = 9, kQueryWarp = 11;  // 9 and 10: an issuer for each group
+constexpr int kThreads = 12 * 32;
+// Registers a thread of the softmax groups and of the others: 256 * 208 + 128 * 88 = 384 * 168, what the
+// block is launched with.
+constexpr int kSoftmaxRegisters = 208, kOtherRegisters = 88;
 constexpr uint32_t kTmemColumns = 512;     // S of both groups, O of both groups
 constexpr float kStale = 8.0f;             // how far (log2) a tile's maximum may exceed the row's before it moves
 
@@ -54,8 +57,6 @@ struct Shape {
 };
 
 struct PrefixArgs {
-    const uint16_t* q;
-    int64_t q_row, q_head;                 // strides, in numbers
     const int64_t* positions;
     const int64_t* prefix_at;              // its length on the device, or null: `prefix`
     uint16_t* out;
@@ -72,9 +73,11 @@ struct PrefixArgs {
 
 // ---- the sequence of tiles ---------------------------------------------------------------------
 
+__device__ __forceinline__ int own_keys(const PrefixArgs& a, int64_t position) {
+    return position < -1 || position >= a.slots ? 0 : int(position) + 1;  // outside the cache: none
+}
 __device__ __forceinline__ int own_tiles(const PrefixArgs& a, int64_t position) {
-    const int keys = position < -1 || position >= a.slots ? 0 : int(position) + 1;  // outside the cache: none
-    return (keys + kKeys - 1) / kKeys;
+    return (own_keys(a, position) + kKeys - 1) / kKeys;
 }
 __device__ __forceinline__ int prefix_length(const PrefixArgs& a) {
     if (a.prefix_at == nullptr) return a.prefix;
@@ -82,18 +85,26 @@ __device__ __forceinline__ int prefix_length(const PrefixArgs& a) {
     return int(given < 0 ? 0 : given > a.prefix ? a.prefix : given);
 }
 // The first tile of block c, and the block that takes tile t, of `total` over `blocks`: no more of
-// them than tiles, so that none between two has nothing.
+// them than tiles, so that none between two has nothing.  (total * c / blocks in 32 bits; its inverse
+// from an estimate that is a block off at most.)
 __device__ __forceinline__ int first_tile(int c, int total, int blocks) {
-    return total <= blocks ? min(c, total) : int(int64_t(total) * c / blocks);
+    if (total <= blocks) return min(c, total);
+    const int whole = total / blocks;
+    return whole * c + (total - whole * blocks) * c / blocks;
 }
 __device__ __forceinline__ int block_of(int t, int total, int blocks) {
-    return total <= blocks ? t : int(((int64_t(t) + 1) * blocks - 1) / total);
+    if (total <= blocks) return t;
+    int c = min(int(float(t) * (float(blocks) / float(total))), blocks - 1);
+    while (first_tile(c, total, blocks) > t) --c;
+    while (first_tile(c + 1, total, blocks) <= t) ++c;
+    return c;
 }
 
 struct Share {  // of a block; in shared memory
     int total, first, last;   // tiles
-    int prefix_keys, prefix_tiles;
-    int row, row_tile;        // the batch row whose own tiles hold the first own tile of the share, and where that row begins
+    int prefix_keys, prefix_tiles, own_first;
+    int head, row_tile, skipped;                     // where the share begins, if in the prefix
+    int own_row, own_head, own_skipped, own_keys;    // where its own tiles begin
 };
 
 struct Piece {
@@ -101,56 +112,94 @@ struct Piece {
     bool prefix, both;        // both: the groups take different rows (else alternate tiles)
     int head, row, rows;      // KV head, first batch row, batch rows
     int key, keys, tiles;     // first key, keys to the end of the item, tiles
+    int before;               // tiles of the share before it
+    bool both_next;           // of the piece after, if there is one
+    __device__ __forceinline__ int tasks() const { return both ? 2 * tiles : tiles; }
 };
 
 // The pieces of a block's share, in order.  Every role walks it for itself.
 struct Walk {
-    int t, row, at;           // next tile; the batch row that own tiles are looked up in, and its first tile
-    int64_t position, next;   // of that row and of the one after (read ahead)
-    __device__ __forceinline__ Walk(const PrefixArgs& a, const Share& s) {
-        t = s.first, row = s.row, at = s.row_tile;
-        position = row < a.batch ? ld_mutable(a.positions + row) : -1;
-        next = row + 1 < a.batch ? ld_mutable(a.positions + row + 1) : -1;
+    int t, head, row, skipped, keys;  // next tile; its head, its batch row (prefix: tile of rows), tiles of the item before it; own keys
+    bool own;
+    __device__ __forceinline__ explicit Walk(const Share& s) {
+        t = s.first, own = false, head = s.head, row = s.row_tile, skipped = s.skipped, keys = 0;
     }
-    __device__ __forceinline__ bool step(const PrefixArgs& a, const Share& s, Piece& p) {
+    // row_keys: own keys of the rows, where the block has them in shared memory
+    __device__ __forceinline__ bool step(const PrefixArgs& a, const Share& s, const int* row_keys, Piece& p) {
         if (t >= s.last) return false;
-        const int prefix_total = a.items * s.prefix_tiles;
-        if (t < prefix_total) {
-            const int item = t / s.prefix_tiles, skipped = t - item * s.prefix_tiles;
+        p.before = t - s.first;
+        if (t < s.own_first) {
             p.prefix = true;
-            p.head = item / a.row_tiles;
-            p.row = (item - p.head * a.row_tiles) * 2 * a.tile_rows;
+            p.head = head;
+            p.row = row * 2 * a.tile_rows;
             p.rows = min(2 * a.tile_rows, a.batch - p.row);
             p.both = p.rows > a.tile_rows;
             p.key = skipped * kKeys, p.keys = s.prefix_keys - p.key;
             p.tiles = min(s.prefix_tiles - skipped, s.last - t);
-            p.place = item + int(blockIdx.x);
+            p.place = head * a.row_tiles + row + int(blockIdx.x);
+            if (++row == a.row_tiles) row = 0, ++head;
+            p.both_next = t + p.tiles < min(s.own_first, s.last) && a.batch - row * 2 * a.tile_rows > a.tile_rows;
         } else {
-            int each = own_tiles(a, position);
-            while (t >= at + each * a.nkv) {  // (t is before the end of the sequence: some row has it)
-                at += each * a.nkv;
-                position = next, ++row;
-                next = row + 1 < a.batch ? ld_mutable(a.positions + row + 1) : -1;
-                each = own_tiles(a, position);
+            if (!own) {
+                own = true, head = s.own_head, row = s.own_row, skipped = s.own_skipped, keys = s.own_keys;
+            } else if (head == a.nkv) {
+                head = 0;
+                do {  // (t is before the end of the sequence: some row has it)
+                    ++row;
+                    keys = a.batch <= kThreads ? row_keys[row] : own_keys(a, ld_mutable(a.positions + row));
+                } while (keys == 0);
             }
-            p.prefix = false, p.both = false;
-            p.head = (t - at) / each;
-            const int skipped = t - at - p.head * each;
-            p.row = row, p.rows = 1;
-            p.key = skipped * kKeys, p.keys = int(position) + 1 - p.key;
-            p.tiles = min(each - skipped, s.last - t);
-            p.place = row * a.nkv + p.head + int(blockIdx.x);
+            p.prefix = false, p.both = false, p.both_next = false;
+            p.head = head, p.row = row, p.rows = 1;
+            p.key = skipped * kKeys, p.keys = keys - p.key;
+            p.tiles = min((p.keys + kKeys - 1) / kKeys, s.last - t);
+            p.place = row * a.nkv + head + int(blockIdx.x);
+            ++head;
         }
+        skipped = 0;
         t += p.tiles;
         return true;
     }
 };
 
-// Place of a tile's K and V among the loads of a piece: the order in which the products want them
-// (K of the task after next comes before V of the next one).
-__device__ __forceinline__ int place_of_k(const Piece& p, int tile) { return p.both ? 2 * tile : tile < 2 ? tile : 2 * tile - 1; }
-__device__ __forceinline__ int place_of_v(const Piece& p, int tile) {
-    return p.both ? 2 * tile + 1 : tile == p.tiles - 1 ? 2 * tile + 1 : 2 * tile + 2;
+// The tasks of a share, one after the other through its pieces.  Number k is group k & 1's; in a piece of
+// both halves of the rows a tile is two tasks, in others one.
+struct Tasks {
+    Walk walk;
+    Piece p;
+    int t, tasks;             // number of the task in its piece, and how many that has
+    uint32_t query;           // query buffers filled before the piece
+    bool both_before;         // of the piece before
+    bool valid;
+    __device__ __forceinline__ Tasks(const PrefixArgs& a, const Share& s, const int* row_keys, int first) : walk(s) {
+        t = first, query = 0, both_before = false;
+        valid = walk.step(a, s, row_keys, p);
+        tasks = valid ? p.tasks() : 0;
+        advance(a, s, row_keys, 0);
+    }
+    __device__ __forceinline__ void advance(const PrefixArgs& a, const Share& s, const int* row_keys, int by) {
+        t += by;
+        while (valid && t >= tasks) {
+            t -= tasks;
+            query += p.both ? 2 : 1, both_before = p.both;
+            valid = walk.step(a, s, row_keys, p);
+            tasks = valid ? p.tasks() : 0;
+        }
+    }
+    __device__ __forceinline__ int tile() const { return p.both ? t >> 1 : t; }
+};
+// K and V of a tile are these loads of the share: each group's products want their tiles in this order.
+// While the groups alternate, S(0) S(1) O(0) S(2) O(1) S(3) ... K of the tile after next comes before V of
+// the next one; beside a tile that both take, it does not, since the other group is at that V first.
+__device__ __forceinline__ uint32_t load_of_k(const Tasks& k) {
+    const int n = k.p.before + k.tile();
+    const bool before = k.tile() > 0 ? k.p.both : k.both_before;
+    return n == 0 ? 0u : uint32_t(2 * n - (before || k.p.both ? 0 : 1));
+}
+__device__ __forceinline__ uint32_t load_of_v(const Piece& p, int tile, int share_tiles) {
+    const int n = p.before + tile;
+    const bool after = tile < p.tiles - 1 ? p.both : p.both_next;
+    return uint32_t(2 * n + (p.both || after || n == share_tiles - 1 ? 1 : 2));
 }
 
 // ---- scratch memory: of a piece, per group, O as [D / 4][rows] float4, then m [rows] and l [rows] ----
@@ -242,33 +291,52 @@ __device__ __forceinline__ uint64_t value_desc(uint32_t addr, uint32_t half) {
            (uint64_t(1) << 46) | (uint64_t(2) << 61);
 }
 
+__device__ __forceinline__ void tmem_put_16(uint32_t taddr, const uint32_t* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map)); }
+
 struct Barriers {
     uint64_t full[10], empty[10];          // tiles of K and V
     uint64_t query_full[2], query_empty[2];
-    uint64_t scores[2], weights[2], result[2];  // of the groups: S is there, P is there, O of a piece is complete
+    uint64_t scores[2], weights[2][2], result[2];  // of the groups: S is there, P's halves are there, O of a piece is complete
     uint32_t tmem_base;
+    Share share;
+    int warp_tiles[kThreads / 32];
+    int row_keys[kThreads];                // own keys of the rows, of batches that small
 };
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads, 1)
 prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __grid_constant__ CUtensorMap prefix_v,
                         const __grid_constant__ CUtensorMap cache_k, const __grid_constant__ CUtensorMap cache_v,
+                        const __grid_constant__ CUtensorMap prefix_q, const __grid_constant__ CUtensorMap own_q,
                         const __grid_constant__ PrefixArgs a) {
     using H = Half16<T>;
     using S = Shape<HD>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* slots = smem + 2 * S::kQuery;
-    __shared__ Barriers bars;
-    __shared__ Share share;
-    __shared__ int warp_tiles[kThreads / 32];
+    Barriers& bars = *reinterpret_cast<Barriers*>(smem + S::kBytes);
+    Share& share = bars.share;
+    const int* row_keys = bars.row_keys;
     const int warp = __shfl_sync(0xFFFFFFFFu, int(threadIdx.x) / 32, 0), lane = threadIdx.x % 32;
 
+    if (threadIdx.x == kProducerWarp * 32) {
+        if (a.prefix > 0) prefetch_map(&prefix_k), prefetch_map(&prefix_v), prefetch_map(&prefix_q);
+        if (a.slots > 0) prefetch_map(&cache_k), prefetch_map(&cache_v), prefetch_map(&own_q);
+    }
     if (threadIdx.x == 0) {
-        for (int s = 0; s < S::kSlots; ++s) mbar_init(&bars.full[s], 1), mbar_init(&bars.empty[s], 1);
+        // (empty: the two issuers)
+        for (int s = 0; s < S::kSlots; ++s) mbar_init(&bars.full[s], 1), mbar_init(&bars.empty[s], 2);
         for (int g = 0; g < 2; ++g) {
-            mbar_init(&bars.query_full[g], 1), mbar_init(&bars.query_empty[g], 1);
-            mbar_init(&bars.scores[g], 1), mbar_init(&bars.weights[g], 4), mbar_init(&bars.result[g], 1);
+            mbar_init(&bars.query_full[g], 1), mbar_init(&bars.query_empty[g], 2);
+            mbar_init(&bars.scores[g], 1), mbar_init(&bars.result[g], 1);
+            mbar_init(&bars.weights[g][0], 4), mbar_init(&bars.weights[g][1], 4);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -285,10 +353,12 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
     {
         const int per = (a.batch + kThreads - 1) / kThreads, from = min(int(threadIdx.x) * per, a.batch), to = min(from + per, a.batch);
         int mine = 0;
+        const int keys = prefix_length(a), tiles = (keys + kKeys - 1) / kKeys;
         for (int b = from; b < to; ++b) {
             const int64_t position = ld_mutable(a.positions + b);
             if (blockIdx.x == 0 && (position < -1 || position >= a.slots)) record_bad_position(a.status, b);
             mine += own_tiles(a, position);
+            if (per == 1) bars.row_keys[b] = own_keys(a, position);
         }
         int before = mine;
 #pragma unroll
@@ -296,16 +366,15 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
             const int other = __shfl_up_sync(0xFFFFFFFFu, before, d);
             if (lane >= d) before += other;
         }
-        if (lane == 31) warp_tiles[warp] = before;
+        if (lane == 31) bars.warp_tiles[warp] = before;
         before -= mine;
         __syncthreads();
         int all = 0;
 #pragma unroll
         for (int w = 0; w < kThreads / 32; ++w) {
-            if (w < warp) before += warp_tiles[w];
-            all += warp_tiles[w];
+            if (w < warp) before += bars.warp_tiles[w];
+            all += bars.warp_tiles[w];
         }
-        const int keys = prefix_length(a), tiles = (keys + kKeys - 1) / kKeys;
         if (a.prefix_at != nullptr && blockIdx.x == 0 && threadIdx.x == 0) {
             const int64_t given = ld_mutable(a.prefix_at);
             if (given < 0 || given > a.prefix) record_bad_position(a.status, 0);
@@ -315,24 +384,29 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
         const int look = max(first, own_first);  // the first own tile this block can have
         if (threadIdx.x == 0) {
             share.total = total, share.first = first, share.last = last;
-            share.prefix_keys = keys, share.prefix_tiles = tiles;
-            if (look >= total) share.row = a.batch, share.row_tile = total;
+            share.prefix_keys = keys, share.prefix_tiles = tiles, share.own_first = own_first;
+            if (first < own_first) {
+                const int item = first / tiles, head = item / a.row_tiles;
+                share.skipped = first - item * tiles, share.head = head, share.row_tile = item - head * a.row_tiles;
+            }
         }
         const int begin = own_first + before * a.nkv, end = begin + mine * a.nkv;
         if (look >= begin && look < end) {
-            int row = from, at = begin;
-            for (;;) {
-                const int each = own_tiles(a, ld_mutable(a.positions + row));
+            int row = from, at = begin, each = mine;  // (one row a thread: it is this one)
+            for (; per > 1; ++row) {
+                each = own_tiles(a, ld_mutable(a.positions + row));
                 if (look < at + each * a.nkv) break;
-                at += each * a.nkv, ++row;
+                at += each * a.nkv;
             }
-            share.row = row, share.row_tile = at;
+            const int head = (look - at) / each;
+            share.own_row = row, share.own_head = head, share.own_skipped = look - at - head * each;
+            share.own_keys = own_keys(a, ld_mutable(a.positions + row));
         }
         if (blockIdx.x == 0) {  // for the joining kernel
             int c = before;
             for (int b = from; b < to; ++b) {
                 a.cum[b] = c;
-                c += own_tiles(a, ld_mutable(a.positions + b));
+                if (b + 1 < to) c += own_tiles(a, ld_mutable(a.positions + b));
             }
             if (threadIdx.x == 0) a.cum[a.batch] = total, a.cum[a.batch + 1] = tiles;
         }
@@ -345,149 +419,160 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
     auto wait = [&](uint64_t* bar, uint32_t parity, int code) {  // of a whole warp; bounded
         return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, a.error, code));
     };
-    Walk walk(a, share);
-    Piece p;
     bool ok = true;
 
+    if (warp >= kProducerWarp) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
     if (warp == kProducerWarp) {
-        uint32_t n = 0;  // loads so far
-        while (ok && walk.step(a, share, p)) {
-            for (int i = 0; i < 2 * p.tiles && ok; ++i, ++n) {
-                // the i-th load of the piece
-                int tile, value;
-                if (p.both) tile = i >> 1, value = i & 1;
-                else if (i < 2) tile = p.tiles > 1 ? i : 0, value = p.tiles > 1 ? 0 : i;
-                else if (i == 2 * p.tiles - 1) tile = p.tiles - 1, value = 1;
-                else tile = (i & 1) ? (i + 1) / 2 : (i - 2) / 2, value = (i & 1) ^ 1;
-                const uint32_t slot = n % S::kSlots, lap = n / S::kSlots;
-                if (lap > 0) ok = wait(&bars.empty[slot], (lap - 1) & 1, 41);
-                if (!ok) break;
-                if (lane == 0) {
-                    mbar_expect_tx(&bars.full[slot], S::kSlot);
-                    const int key = p.key + tile * kKeys;
+        if (lane == 0) {
+            Tasks keys(a, share, row_keys, 0), values(a, share, row_keys, 0);
+            const uint32_t loads = uint32_t(2 * (share.last - share.first));
+            uint32_t n = 0, slot = 0, lap = 0;
+            auto load = [&](Tasks& task, const CUtensorMap* shared, const CUtensorMap* own) {
+                mbar_expect_tx(&bars.full[slot], S::kSlot);
+                const int key = task.p.key + task.tile() * kKeys;
 #pragma unroll
-                    for (int h = 0; h < S::kHalves; ++h) {
-                        const uint32_t dst = smem_u32(slots) + slot * S::kSlot + h * S::kHalf;
-                        if (p.prefix) tma_load_3d(dst, value ? &prefix_v : &prefix_k, h * 64, key, p.head, &bars.full[slot]);
-                        else tma_load_4d(dst, value ? &cache_v : &cache_k, h * 64, key, p.head, p.row, &bars.full[slot]);
-                    }
+                for (int h = 0; h < S::kHalves; ++h) {
+                    const uint32_t dst = smem_u32(slots) + slot * S::kSlot + h * S::kHalf;
+                    if (task.p.prefix) tma_load_3d(dst, shared, h * 64, key, task.p.head, &bars.full[slot]);
+                    else tma_load_4d(dst, own, h * 64, key, task.p.head, task.p.row, &bars.full[slot]);
                 }
-                __syncwarp();
+                task.advance(a, share, row_keys, task.p.both ? 2 : 1);  // to the next tile
+            };
+            for (; n < loads; ++n) {
+                ok = lap == 0 || mbar_wait(&bars.empty[slot], (lap - 1) & 1, a.error, 41);
+                if (!ok) break;
+                if (keys.valid && load_of_k(keys) == n) load(keys, &prefix_k, &cache_k);
+                else load(values, &prefix_v, &cache_v);
+                if (++slot == S::kSlots) slot = 0, ++lap;
             }
+            if (!ok)  // what is in flight lands before the block leaves
+                for (uint32_t i = n > S::kSlots ? n - S::kSlots : 0; i < n; ++i) mbar_wait(&bars.full[i % S::kSlots], (i / S::kSlots) & 1, a.error, 42);
         }
-        if (!ok)  // what is in flight lands before the block leaves
-            for (uint32_t i = n > S::kSlots ? n - S::kSlots : 0; i < n; ++i) mbar_wait(&bars.full[i % S::kSlots], (i / S::kSlots) & 1, a.error, 42);
-    } else if (warp == kIssuerWarp) {
-        constexpr uint32_t kType = H::kDtype == B200Q_BF16 ? 1u : 0u;
-        constexpr uint32_t kScores = (1u << 4) | (kType << 7) | (kType << 10) | (uint32_t(kKeys >> 3) << 17) | (uint32_t(kRows >> 4) << 24);
-        constexpr uint32_t kValues = (1u << 4) | (kType << 7) | (kType << 10) | (1u << 16) | (uint32_t(HD >> 3) << 17) | (uint32_t(kRows >> 4) << 24);
-        const bool leader = elect_one();
-        uint32_t n = 0, queries = 0, done[2] = {0, 0};  // loads, query buffers and tasks of the groups before this piece
-        while (ok && walk.step(a, share, p)) {
-            const int tasks = p.both ? 2 * p.tiles : p.tiles;
-            auto scores = [&](int t) {
-                const int g = t & 1, tile = p.both ? t >> 1 : t;
-                const uint32_t query = queries + (p.both ? uint32_t(g) : 0u), buffer = query & 1;
-                if (t < 2) ok = wait(&bars.query_full[buffer], (query >> 1) & 1, 43);
-                const uint32_t load = n + uint32_t(place_of_k(p, tile)), slot = load % S::kSlots;
-                ok = ok && wait(&bars.full[slot], (load / S::kSlots) & 1, 44);
+        __syncwarp();
+    } else if (warp == kIssuerWarp || warp == kIssuerWarp + 1) {
+        // ---- the products of group g, from one thread ----
+        if (elect_one()) {
+            constexpr uint32_t kType = H::kDtype == B200Q_BF16 ? 1u : 0u;
+            constexpr uint32_t kScores = (1u << 4) | (kType << 7) | (kType << 10) | (uint32_t(kKeys >> 3) << 17) | (uint32_t(kRows >> 4) << 24);
+            constexpr uint32_t kValues = (1u << 4) | (kType << 7) | (kType << 10) | (1u << 16) | (uint32_t(HD >> 3) << 17) | (uint32_t(kRows >> 4) << 24);
+            const int g = warp - kIssuerWarp, share_tiles = share.last - share.first;
+            const uint32_t s_at = tmem + uint32_t(g) * kKeys, o_at = tmem + 2 * kKeys + uint32_t(g) * HD;
+            Tasks scores(a, share, row_keys, g), values(a, share, row_keys, g);
+            // Both issuers see every load and every buffer of queries, in order, and hand it back: a waiter
+            // that left one out could not tell a barrier's phase from the one after next.
+            uint32_t loads = 0, queries = 0;  // those handed back
+            auto take_load = [&](uint32_t load) {  // waits for it, hands back those before it; its slot
+                for (; ok && loads < load; ++loads) {
+                    ok = mbar_wait(&bars.full[loads % S::kSlots], (loads / S::kSlots) & 1, a.error, 44);
+                    if (ok) mbar_arrive(&bars.empty[loads % S::kSlots]);
+                }
+                const uint32_t slot = load % S::kSlots;
+                ok = ok && mbar_wait(&bars.full[slot], (load / S::kSlots) & 1, a.error, 44);
+                loads = load + 1;
+                return slot;
+            };
+            auto pass_queries = [&](uint32_t before) {
+                for (; ok && queries < before; ++queries) {
+                    ok = mbar_wait(&bars.query_full[queries & 1], (queries >> 1) & 1, a.error, 43);
+                    if (ok) mbar_arrive(&bars.query_empty[queries & 1]);
+                }
+            };
+            auto issue_scores = [&]() {
+                const Piece& p = scores.p;
+                const uint32_t query = scores.query + (p.both ? uint32_t(scores.t & 1) : 0u), buffer = query & 1;
+                if (scores.t < 2) {
+                    pass_queries(query);
+                    ok = ok && mbar_wait(&bars.query_full[buffer], (query >> 1) & 1, a.error, 43);
+                    queries = query + 1;
+                }
+                const uint32_t slot = take_load(load_of_k(scores));
                 if (!ok) return;
                 tc_fence_after();
-                if (leader) {
-                    const uint64_t qd = smem_desc(smem_u32(smem) + buffer * S::kQuery), kd = smem_desc(smem_u32(slots) + slot * S::kSlot);
+                const uint64_t qd = smem_desc(smem_u32(smem) + buffer * S::kQuery), kd = smem_desc(smem_u32(slots) + slot * S::kSlot);
 #pragma unroll
-                    for (int k = 0; k < HD / 16; ++k) {
-                        const uint32_t step = uint32_t(k / 4) * (S::kHalf >> 4) + uint32_t(k % 4) * 2;
-                        umma_f16_ss(tmem + uint32_t(g) * kKeys, qd + step, kd + step, kScores, k > 0);
-                    }
-                    umma_commit(&bars.scores[g]);
-                    if (!p.both || g == 1) umma_commit(&bars.empty[slot]);
-                    if (p.both ? t >= tasks - 2 : t == tasks - 1) umma_commit(&bars.query_empty[buffer]);
+                for (int k = 0; k < HD / 16; ++k) {
+                    const uint32_t step = uint32_t(k / 4) * (S::kHalf >> 4) + uint32_t(k % 4) * 2;
+                    umma_f16_ss(s_at, qd + step, kd + step, kScores, k > 0);
                 }
-                __syncwarp();
+                umma_commit(&bars.scores[g]);
+                umma_commit(&bars.empty[slot]);
+                if (scores.t >= scores.tasks - 2) umma_commit(&bars.query_empty[buffer]);
+                scores.advance(a, share, row_keys, 2);
             };
-            scores(0);
-            if (ok && tasks > 1) scores(1);
-            for (int t = 0; t < tasks && ok; ++t) {
-                const int g = t & 1, tile = p.both ? t >> 1 : t;
-                ok = wait(&bars.weights[g], done[g] & 1, 45);
-                const uint32_t load = n + uint32_t(place_of_v(p, tile)), slot = load % S::kSlots;
-                ok = ok && wait(&bars.full[slot], (load / S::kSlots) & 1, 46);
-                if (!ok) break;
-                ++done[g];
-                tc_fence_after();
-                if (leader) {
-                    const uint64_t vd = value_desc(smem_u32(slots) + slot * S::kSlot, S::kHalf);
+            if (scores.valid) issue_scores();
+            for (uint32_t n = 0; ok && values.valid; ++n) {
+                const int valid = values.p.keys - values.tile() * kKeys;
+                const uint32_t slot = take_load(load_of_v(values.p, values.tile(), share_tiles));
+                const uint64_t vd = value_desc(smem_u32(slots) + slot * S::kSlot, S::kHalf);
 #pragma unroll
-                    for (int k = 0; k < kKeys / 16; ++k)
-                        umma_f16_ts(tmem + 2 * kKeys + uint32_t(g) * HD, tmem + uint32_t(g) * kKeys + k * 8, vd + uint32_t(k) * (2048 >> 4),
-                                    kValues, k > 0 || t >= 2);
-                    if (!p.both || g == 1) umma_commit(&bars.empty[slot]);
-                    if (t >= tasks - 2) umma_commit(&bars.result[g]);
+                for (int h = 0; h < 2; ++h) {
+                    ok = ok && mbar_wait(&bars.weights[g][h], n & 1, a.error, 45);
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int k = 4 * h; k < 4 * h + 4; ++k)
+                        if (k == 0 || k * 16 < valid) umma_f16_ts(o_at, s_at + k * 8, vd + uint32_t(k) * (2048 >> 4), kValues, k > 0 || values.t >= 2);
                 }
-                __syncwarp();
-                if (t + 2 < tasks) scores(t + 2);
-            }
-            n += 2 * uint32_t(p.tiles);
-            queries += p.both ? 2 : 1;
-        }
-    } else if (warp == kQueryWarp) {
-        uint32_t query = 0;
-        while (ok && walk.step(a, share, p)) {
-            for (int g = 0; g < (p.both ? 2 : 1) && ok; ++g, ++query) {
-                const uint32_t buffer = query & 1;
-                if (query >= 2) ok = wait(&bars.query_empty[buffer], ((query >> 1) - 1) & 1, 47);
                 if (!ok) break;
-                const int row0 = p.row + g * a.tile_rows, rows = min(a.tile_rows, p.row + p.rows - row0) * a.rep;
-                const uint32_t to = smem_u32(smem) + buffer * S::kQuery;
-                constexpr int kPieces = HD / 8;  // of 16 bytes a row
-                for (int i = lane; i < rows * kPieces; i += 32) {
-                    const int r = i / kPieces, c = i % kPieces, b = r / a.rep;
-                    const uint16_t* src = a.q + (row0 + b) * a.q_row + (p.head * a.rep + r - b * a.rep) * a.q_head + c * 8;
-                    const uint32_t dst = to + uint32_t(c / 8) * (kRows * 128) + uint32_t(r) * 128 + uint32_t(((c % 8) ^ (r & 7)) << 4);
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-                }
-                asm volatile("cp.async.wait_all;" ::: "memory");
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bars.query_full[buffer]);
+                umma_commit(&bars.empty[slot]);
+                if (values.t >= values.tasks - 2) umma_commit(&bars.result[g]);
+                values.advance(a, share, row_keys, 2);
+                if (scores.valid) issue_scores();
+            }
+            pass_queries(scores.query);
+            if (share_tiles > 0 && ok) {
+                const uint32_t last = uint32_t(2 * share_tiles - 1);
+                if (loads <= last) mbar_arrive(&bars.empty[take_load(last)]);
             }
         }
-    } else {
+        __syncwarp();
+    } else if (warp == kQueryWarp) {
+        if (lane == 0) {
+            Walk walk(share);
+            Piece p;
+            uint32_t query = 0;
+            while (ok && walk.step(a, share, row_keys, p)) {
+                for (int half = 0; half < (p.both ? 2 : 1); ++half, ++query) {
+                    const uint32_t buffer = query & 1;
+                    ok = query < 2 || mbar_wait(&bars.query_empty[buffer], ((query >> 1) - 1) & 1, a.error, 47);
+                    if (!ok) break;
+                    // (batch rows past the last one read as zeros; rows of the buffer past the box are never looked at)
+                    mbar_expect_tx(&bars.query_full[buffer], uint32_t(S::kHalves * 128 * a.rep * (p.prefix ? a.tile_rows : 1)));
+#pragma unroll
+                    for (int h = 0; h < S::kHalves; ++h)
+                        tma_load_4d(smem_u32(smem) + buffer * S::kQuery + h * (kRows * 128), p.prefix ? &prefix_q : &own_q, h * 64, 0,
+                                    p.head, p.row + half * a.tile_rows, &bars.query_full[buffer]);
+                }
+            }
+            if (!ok)
+                for (uint32_t i = query > 2 ? query - 2 : 0; i < query; ++i) mbar_wait(&bars.query_full[i & 1], (i >> 1) & 1, a.error, 42);
+        }
+        __syncwarp();
+    } else if (warp < kProducerWarp) {
         // ---- softmax: group g, one query row a thread ----
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
         const int g = warp / 4, row = threadIdx.x % 128;
         const uint32_t lanes = tmem + (uint32_t(warp & 3) << 21);
         const uint32_t s_at = lanes + uint32_t(g) * kKeys, o_at = lanes + 2 * kKeys + uint32_t(g) * HD;
-        uint32_t n = 0, done = 0, pieces = 0;  // loads, tasks of this group and pieces with any before this one
-        while (ok && walk.step(a, share, p)) {
-            const int live = p.both ? min(a.tile_rows, p.rows - g * a.tile_rows) * a.rep : p.rows * a.rep;
+        Walk walk(share);
+        Piece p;
+        uint32_t first_task = 0, done = 0, pieces = 0;  // of the piece; tasks and pieces that this group has had
+        const int share_tiles = share.last - share.first;
+        while (ok && walk.step(a, share, row_keys, p)) {
+            // which of the piece's tasks are this group's: every other one, and of both halves of the rows always the same half
+            const int t0 = g ^ int(first_task & 1), live = p.both ? min(a.tile_rows, p.rows - t0 * a.tile_rows) * a.rep : p.rows * a.rep;
             const bool any = (warp & 3) * 32 < live;  // of this warp's rows
-            const int first = p.both ? 0 : g, stride = p.both ? 1 : 2;
+            first_task += uint32_t(p.tasks());
             float m = -INFINITY, l = 0.0f;
-            for (int tile = first; tile < p.tiles && ok; tile += stride) {
+            for (int tile = p.both ? 0 : t0; tile < p.tiles && ok; tile += p.both ? 1 : 2) {
                 ok = wait(&bars.scores[g], done & 1, 48);
                 if (!ok) break;
                 ++done;
                 tc_fence_after();
                 const int valid = p.keys - tile * kKeys;  // keys of the tile, and more
-                if (any) {
-                    uint32_t v[kKeys];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) tmem_ask_32(v + 32 * i, s_at + 32 * i);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) tmem_arrived(v + 32 * i);
-                    if (valid < kKeys) {
-#pragma unroll
-                        for (int i = 0; i < kKeys; ++i)
-                            if (i >= valid) v[i] = 0xFF800000u;
-                    }
-                    float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                    for (int i = 0; i < kKeys; i += 4)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) most[j] = fmaxf(most[j], __uint_as_float(v[i + j]));
-                    const float here = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * a.scale_log2;
-                    if (tile == first) {
+                // m of the row, `here` being the largest score of this tile
+                auto moved = [&](float here) {
+                    if (tile < (p.both ? 1 : 2)) {  // the group's first
                         m = here == -INFINITY ? 0.0f : here;
                     } else if (__any_sync(0xFFFFFFFFu, row < live && here > m + kStale)) {
                         const float next = here > m + kStale ? here : m, by = exp2_approx(m - next);
@@ -503,45 +588,99 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
                             tmem_put_32(o_at + c, o);
                         }
                     }
-                    const float2 scale = make_float2(a.scale_log2, a.scale_log2), minus = make_float2(-m, -m);
-                    float2 sum = make_float2(0.0f, 0.0f);
+                };
+                auto give = [&](int h) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bars.weights[g][h]);
+                };
+                const float2 scale = make_float2(a.scale_log2, a.scale_log2);
+                float2 sum = make_float2(0.0f, 0.0f);
+                // 2 weights of two scores, packed
+                auto weigh = [&](uint32_t x, uint32_t y, float2 minus) {
+                    const float2 t = fma2(make_float2(__uint_as_float(x), __uint_as_float(y)), scale, minus);
+                    const float2 e = make_float2(exp2_approx(t.x), exp2_approx(t.y));
+                    sum = add2(sum, e);
+                    return H::pack(e.x, e.y);
+                };
+                if (any && valid >= kKeys) {
+                    uint32_t v[kKeys];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) tmem_ask_32(v + 32 * i, s_at + 32 * i);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) tmem_arrived(v + 32 * i);
+                    float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int i = 0; i < kKeys; i += 4)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) most[j] = fmaxf(most[j], __uint_as_float(v[i + j]));
+                    moved(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * a.scale_log2);
+                    const float2 minus = make_float2(-m, -m);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         uint32_t w[32];
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const int at = 64 * h + 2 * i;
-                            const float2 t = fma2(make_float2(__uint_as_float(v[at]), __uint_as_float(v[at + 1])), scale, minus);
-                            const float2 e = make_float2(exp2_approx(t.x), exp2_approx(t.y));
-                            sum = add2(sum, e);
-                            w[i] = H::pack(e.x, e.y);
-                        }
+                        for (int i = 0; i < 32; ++i) w[i] = weigh(v[64 * h + 2 * i], v[64 * h + 2 * i + 1], minus);
                         tmem_put_32(s_at + 32 * h, w);
+                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                        if (h == 0) give(0);  // the first half's products begin
+                    }
+                    l += sum.x + sum.y;
+                } else if (any) {
+                    // the last tile of an item: 32 keys at a time, as far as there are keys
+                    const int chunks = (valid + 31) / 32;
+                    auto ask = [&](uint32_t* v, int c) {
+                        tmem_ask_32(v, s_at + 32 * c);
+                        tmem_arrived(v);
+                        const int rest = valid - 32 * c;
+                        if (rest < 32) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) v[i] = i < rest ? v[i] : 0xFF800000u;
+                        }
+                    };
+                    float most = -INFINITY;
+#pragma unroll 1
+                    for (int c = 0; c < chunks; ++c) {
+                        uint32_t v[32];
+                        ask(v, c);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) most = fmaxf(most, __uint_as_float(v[i]));
+                    }
+                    moved(most * a.scale_log2);
+                    const float2 minus = make_float2(-m, -m);
+#pragma unroll 1
+                    for (int c = 0; c < chunks; ++c) {  // (a chunk's weights go where scores of chunks before it were)
+                        uint32_t v[32], w[16];
+                        ask(v, c);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) w[i] = weigh(v[2 * i], v[2 * i + 1], minus);
+                        tmem_put_16(s_at + 16 * c, w);
                     }
                     l += sum.x + sum.y;
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 }
-                if (valid < kKeys && (!p.both || g == 0)) {
-                    // Rows of V past the last key may hold anything, and 0 * NaN is no 0.
-                    const uint32_t load = n + uint32_t(place_of_v(p, tile)), slot = load % S::kSlots;
+                if (valid < kKeys) {
+                    // Rows of V past the last key may hold anything, and 0 * NaN is no 0: those that the last
+                    // step of 16 keys takes in are cleared (by either group where both use the tile).
+                    const uint32_t load = load_of_v(p, tile, share_tiles), slot = load % S::kSlots;
                     ok = wait(&bars.full[slot], (load / S::kSlots) & 1, 49);
                     if (!ok) break;
                     uint8_t* tail = slots + slot * S::kSlot;
-                    for (int i = row; i < (kKeys - valid) * 8 * S::kHalves; i += 128) {
-                        const int h = i / ((kKeys - valid) * 8), rest = i - h * (kKeys - valid) * 8;
-                        *reinterpret_cast<uint4*>(tail + h * S::kHalf + valid * 128 + rest * 16) = make_uint4(0, 0, 0, 0);
+                    const int rows = (16 - valid % 16) % 16;
+                    for (int i = row; i < rows * 8 * S::kHalves; i += 128) {
+                        const int h = S::kHalves == 1 ? 0 : (i >> 3) & 1, r = valid + (i >> 3) / S::kHalves;
+                        *reinterpret_cast<uint4*>(tail + h * S::kHalf + r * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
                     }
                     fence_proxy_async();
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bars.weights[g]);
+                if (!any || valid < kKeys) give(0);
+                give(1);
             }
             if (!ok) break;
             // ---- the piece's result ----
             const int span = p.prefix ? kRows : a.rep;  // rows of a group in the scratch memory
-            float* to = a.scratch + (p.prefix ? 0 : a.own_at) + (2 * int64_t(p.place) + g) * group_floats(span, HD);
-            const bool worked = first < p.tiles;
+            float* to = a.scratch + (p.prefix ? 0 : a.own_at) + (2 * int64_t(p.place) + t0) * group_floats(span, HD);
+            const bool worked = p.both || t0 < p.tiles;
             if (worked) {
                 ok = wait(&bars.result[g], pieces & 1, 50);
                 if (!ok) break;
@@ -565,7 +704,6 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
                 to[int64_t(HD) * span + row] = worked ? m : -INFINITY;
                 to[int64_t(HD + 1) * span + row] = l;
             }
-            n += 2 * uint32_t(p.tiles);
         }
     }
 
@@ -579,72 +717,104 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
 }
 
 // ---- joining the pieces of a row ----------------------------------------------------------------
-// One query row a lane; the D / 4 columns of four numbers are dealt among warps and blocks, two a
-// thread.  out = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i in f32; a row without any key is 0.
-constexpr int kJoinWarps = 4, kJoinColumns = 2;
+// out = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i in f32 over a row's parts (a piece has one, or
+// one of each group); a row without any key is 0.  One query row a lane and two columns of four
+// numbers a block; the parts are dealt among its warps, four in flight each, since what the kernel
+// waits for is the way to the L2 cache: then the warps' sums meet in shared memory.
+constexpr int kJoinWarps = 8, kJoinColumns = 2, kJoinHeld = 4;
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(32 * kJoinWarps)
 prefix_join_kernel(const __grid_constant__ PrefixArgs a, int blocks) {
     using H = Half16<T>;
+    constexpr int kSums = 4 * kJoinColumns;
+    __shared__ float sums[kJoinWarps][kSums + 2][32];  // O, m and l
     pdl_launch_dependents();
     pdl_wait();
-    const int head = blockIdx.y, row = blockIdx.x * 32 + threadIdx.x % 32;  // batch row * rep + head of the group
-    const int column = (blockIdx.z * kJoinWarps + threadIdx.x / 32) * kJoinColumns;
-    if (row >= a.batch * a.rep) return;
-    const int b = row / a.rep, r = row - b * a.rep;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int head = blockIdx.y, row = blockIdx.x * 32 + lane;  // row: batch row * rep + head of the group
+    const int column = blockIdx.z * kJoinColumns;
+    const bool live = row < a.batch * a.rep;
+    const int b = live ? row / a.rep : 0, r = row - b * a.rep;
     auto word = [&](int i) { return int(ld_mutable(reinterpret_cast<const uint32_t*>(a.cum) + i)); };
-    const int total = word(a.batch), prefix_tiles = word(a.batch + 1);
+    const int total = word(a.batch), prefix_tiles = word(a.batch + 1), before = word(b);
+    const int each = own_tiles(a, ld_mutable(a.positions + b));
 
     struct Item {              // the prefix, and the row's own keys
         const float* base;     // of the first group that has the row, in the first piece
-        int parts, groups;     // groups that have the row: over all pieces, and of a piece
+        int parts, skip;       // groups that have the row: over all pieces; and the floats from one to the next
         int span, at;          // rows of a group in the scratch memory, and which one this is
-    } items[2] = {};
-    if (prefix_tiles > 0) {
+    } shared = {}, own = {};
+    if (live && prefix_tiles > 0) {
         const int pair = b / (2 * a.tile_rows), within = b - pair * 2 * a.tile_rows;
         const bool both = min(2 * a.tile_rows, a.batch - pair * 2 * a.tile_rows) > a.tile_rows;
         const int item = head * a.row_tiles + pair, first = item * prefix_tiles;
         const int from = block_of(first, total, blocks), to = block_of(first + prefix_tiles - 1, total, blocks);
-        const int g = both && within >= a.tile_rows;
-        items[0].base = a.scratch + (2 * int64_t(item + from) + g) * group_floats(kRows, HD);
-        items[0].groups = both ? 1 : 2, items[0].parts = (to - from + 1) * items[0].groups;
-        items[0].span = kRows, items[0].at = (within - g * a.tile_rows) * a.rep + r;
+        const int g = both && within >= a.tile_rows, groups = both ? 1 : 2;
+        shared.base = a.scratch + (2 * int64_t(item + from) + g) * group_floats(kRows, HD);
+        shared.parts = (to - from + 1) * groups, shared.skip = int(group_floats(kRows, HD)) * (2 / groups);
+        shared.span = kRows, shared.at = (within - g * a.tile_rows) * a.rep + r;
     }
-    const int each = own_tiles(a, ld_mutable(a.positions + b));
-    if (each > 0) {
-        const int first = a.items * prefix_tiles + word(b) * a.nkv + head * each;
+    if (live && each > 0) {
+        const int first = a.items * prefix_tiles + before * a.nkv + head * each;
         const int from = block_of(first, total, blocks), to = block_of(first + each - 1, total, blocks);
-        items[1].base = a.scratch + a.own_at + 2 * int64_t(b * a.nkv + head + from) * group_floats(a.rep, HD);
-        items[1].groups = 2, items[1].parts = (to - from + 1) * 2;
-        items[1].span = a.rep, items[1].at = r;
+        own.base = a.scratch + a.own_at + 2 * int64_t(b * a.nkv + head + from) * group_floats(a.rep, HD);
+        own.parts = (to - from + 1) * 2, own.skip = int(group_floats(a.rep, HD));
+        own.span = a.rep, own.at = r;
     }
-    auto part = [&](const Item& it, int k) {
-        return it.base + (it.groups == 2 ? k : 2 * k) * group_floats(it.span, HD);
-    };
-    float m = -INFINITY;
+    const int parts = shared.parts + own.parts;
+    float m = -INFINITY, l = 0.0f, o[kSums] = {};
+    for (int k0 = warp; k0 < parts; k0 += kJoinWarps * kJoinHeld) {
+        float ms[kJoinHeld], ls[kJoinHeld];
+        uint4 os[kJoinHeld][kJoinColumns];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll 8
-        for (int k = 0; k < items[i].parts; ++k) m = fmaxf(m, ld_mutable(part(items[i], k) + HD * items[i].span + items[i].at));
-    float l = 0.0f, o[4 * kJoinColumns] = {};
+        for (int u = 0; u < kJoinHeld; ++u) {
+            const int k = k0 + u * kJoinWarps;
+            ms[u] = -INFINITY;
+            if (k >= parts) continue;
+            const Item& it = k < shared.parts ? shared : own;
+            const float* from = it.base + int64_t(k < shared.parts ? k : k - shared.parts) * it.skip;
+            ms[u] = ld_mutable(from + HD * it.span + it.at);
+            ls[u] = ld_mutable(from + (HD + 1) * it.span + it.at);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const Item& it = items[i];
-#pragma unroll 4
-        for (int k = 0; k < it.parts; ++k) {
-            const float* from = part(it, k);
-            const float theirs = ld_mutable(from + HD * it.span + it.at);
-            if (theirs == -INFINITY) continue;  // a group that had no tile of the piece: nothing else is there
-            const float weight = exp2_approx(theirs - m);
-            l += weight * ld_mutable(from + (HD + 1) * it.span + it.at);
+            for (int c = 0; c < kJoinColumns; ++c) os[u][c] = ld_mutable(reinterpret_cast<const uint4*>(from) + (column + c) * it.span + it.at);
+        }
+        float most = m;
+#pragma unroll
+        for (int u = 0; u < kJoinHeld; ++u) most = fmaxf(most, ms[u]);
+        if (most == -INFINITY) continue;
+        const float by = exp2_approx(m - most);
+        m = most, l *= by;
+#pragma unroll
+        for (int i = 0; i < kSums; ++i) o[i] *= by;
+#pragma unroll
+        for (int u = 0; u < kJoinHeld; ++u) {
+            if (ms[u] == -INFINITY) continue;  // a group that had no tile of the piece: the rest of it was not stored
+            const float weight = exp2_approx(ms[u] - m);
+            l += weight * ls[u];
 #pragma unroll
             for (int c = 0; c < kJoinColumns; ++c) {
-                const uint4 v = ld_mutable(reinterpret_cast<const uint4*>(from) + (column + c) * it.span + it.at);
-                o[4 * c] += weight * __uint_as_float(v.x), o[4 * c + 1] += weight * __uint_as_float(v.y);
-                o[4 * c + 2] += weight * __uint_as_float(v.z), o[4 * c + 3] += weight * __uint_as_float(v.w);
+                o[4 * c] += weight * __uint_as_float(os[u][c].x), o[4 * c + 1] += weight * __uint_as_float(os[u][c].y);
+                o[4 * c + 2] += weight * __uint_as_float(os[u][c].z), o[4 * c + 3] += weight * __uint_as_float(os[u][c].w);
             }
         }
+    }
+#pragma unroll
+    for (int i = 0; i < kSums; ++i) sums[warp][i][lane] = o[i];
+    sums[warp][kSums][lane] = m, sums[warp][kSums + 1][lane] = l;
+    __syncthreads();
+    if (warp != 0 || !live) return;
+#pragma unroll
+    for (int w = 1; w < kJoinWarps; ++w) m = fmaxf(m, sums[w][kSums][lane]);
+    l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kSums; ++i) o[i] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) {
+        const float theirs = sums[w][kSums][lane], weight = theirs == -INFINITY ? 0.0f : exp2_approx(theirs - m);
+        l += weight * sums[w][kSums + 1][lane];
+#pragma unroll
+        for (int i = 0; i < kSums; ++i) o[i] += weight * sums[w][i][lane];
     }
     const float by = l == 0.0f ? 0.0f : 1.0f / l;
     uint16_t* to = a.out + (int64_t(b) * a.nq + head * a.rep + r) * HD + column * 4;
@@ -687,11 +857,11 @@ int32_t check_prefix(int64_t batch, int64_t nq, int64_t nkv, int64_t hd, int64_t
     return B200Q_OK;
 }
 
-// A map of keys or values [extents][hd], 64 numbers x 128 keys a box; strides in numbers.
+// A map of boxes of 64 numbers x `rows` x 1 x `last` (keys and values: 128 keys); strides in numbers.
 CUresult make_map(EncodeTiled encode, CUtensorMap* map, const void* base, int32_t dtype, int rank, const int64_t* extents,
-                  const int64_t* strides) {
+                  const int64_t* strides, int rows, int last) {
     cuuint64_t dims[4], bytes[3];
-    cuuint32_t box[4] = {64, cuuint32_t(kKeys), 1, 1}, elem[4] = {1, 1, 1, 1};
+    cuuint32_t box[4] = {64, cuuint32_t(rows), 1, cuuint32_t(last)}, elem[4] = {1, 1, 1, 1};
     int64_t dense = extents[0];
     for (int d = 0; d < rank; ++d) {
         dims[d] = cuuint64_t(extents[d]);
@@ -705,14 +875,15 @@ CUresult make_map(EncodeTiled encode, CUtensorMap* map, const void* base, int32_
 }
 
 template <typename T, int HD>
-cudaError_t launch_prefix(const CUtensorMap (&maps)[4], const PrefixArgs& a, int blocks, cudaStream_t stream) {
-    constexpr size_t kSmem = Shape<HD>::kBytes + 1024;
+cudaError_t launch_prefix(const CUtensorMap (&maps)[6], const PrefixArgs& a, int blocks, cudaStream_t stream) {
+    constexpr size_t kSmem = Shape<HD>::kBytes + sizeof(Barriers) + 1024;
+    static_assert(kSmem <= 227 * 1024, "shared memory of a block");
     cudaError_t err = ensure_dynamic_smem(reinterpret_cast<const void*>(prefix_attention_kernel<T, HD>), kSmem);
     if (err != cudaSuccess) return err;
     err = launch_overlapped(prefix_attention_kernel<T, HD>, dim3(unsigned(blocks)), dim3(kThreads), kSmem, stream, maps[0],
-                            maps[1], maps[2], maps[3], a);
+                            maps[1], maps[2], maps[3], maps[4], maps[5], a);
     if (err != cudaSuccess) return err;
-    const dim3 grid{unsigned((a.batch * a.rep + 31) / 32), unsigned(a.nkv), unsigned(HD / (4 * kJoinWarps * kJoinColumns))};
+    const dim3 grid{unsigned((a.batch * a.rep + 31) / 32), unsigned(a.nkv), unsigned(HD / (4 * kJoinColumns))};
     return launch_overlapped(prefix_join_kernel<T, HD>, grid, dim3(32 * kJoinWarps), 0, stream, a, blocks);
 }
 
@@ -748,18 +919,21 @@ extern "C" int32_t b200q_prefix_attention(const void* q, const void* prefix_k, c
     if (encode == nullptr) return unavailable("prefix_attention: the driver has no cuTensorMapEncodeTiled");
 
     const PrefixPlan p = plan_of(batch, nkv, nq / nkv, head_dim, prefix, max_seq);
-    CUtensorMap maps[4] = {};
+    CUtensorMap maps[6] = {};
     // strides: q (row, head), then (key, head) of the prefix's keys and values, (key, head, row) of the caches'
     for (int v = 0; v < 2; ++v) {
         const int64_t shared[3] = {head_dim, prefix, nkv}, alone[4] = {head_dim, max_seq, nkv, batch};
         CUresult made = CUDA_SUCCESS;
-        if (prefix > 0) made = make_map(encode, &maps[v], v ? prefix_v : prefix_k, dtype, 3, shared, strides + 2 + 2 * v);
+        if (prefix > 0) made = make_map(encode, &maps[v], v ? prefix_v : prefix_k, dtype, 3, shared, strides + 2 + 2 * v, kKeys, 1);
         if (made == CUDA_SUCCESS && max_seq > 0)
-            made = make_map(encode, &maps[2 + v], v ? cache_v : cache_k, dtype, 4, alone, strides + 6 + 3 * v);
+            made = make_map(encode, &maps[2 + v], v ? cache_v : cache_k, dtype, 4, alone, strides + 6 + 3 * v, kKeys, 1);
+        // queries of a KV head: of as many batch rows as a group takes, and of one
+        const int64_t rep = nq / nkv, queries[4] = {head_dim, rep, nkv, batch}, steps[3] = {strides[1], rep * strides[1], strides[0]};
+        if (made == CUDA_SUCCESS && (v ? max_seq : prefix) > 0)
+            made = make_map(encode, &maps[4 + v], q, dtype, 4, queries, steps, int(rep), v ? 1 : p.tile_rows);
         B200Q_REQUIRE(made == CUDA_SUCCESS, "prefix_attention: cuTensorMapEncodeTiled failed (%d)", int(made));
     }
     PrefixArgs a = {};
-    a.q = static_cast<const uint16_t*>(q), a.q_row = strides[0], a.q_head = strides[1];
     a.positions = positions, a.prefix_at = prefix_at, a.out = static_cast<uint16_t*>(out);
     a.scratch = static_cast<float*>(scratch), a.cum = static_cast<int*>(scratch) + p.cum_at;
     a.batch = int(batch), a.nq = int(nq), a.nkv = int(nkv), a.rep = int(nq / nkv);
