@@ -37,12 +37,10 @@ namespace {
 using namespace umma;
 
 constexpr int kKeys = 128;                 // of a tile
+constexpr int kPart = 64;                  // keys of one turn of scores, weights and sums: half a tile
 constexpr int kRows = 128;                 // of a group's products
 constexpr int kProducerWarp = 8, kIssuerWarp = 9, kQueryWarp = 11;  // 9 and 10: an issuer for each group
 constexpr int kThreads = 12 * 32;
-// Registers a thread of the softmax groups and of the others: 256 * 208 + 128 * 88 = 384 * 168, what the
-// block is launched with.
-constexpr int kSoftmaxRegisters = 208, kOtherRegisters = 88;
 constexpr uint32_t kTmemColumns = 512;     // S of both groups, O of both groups
 constexpr float kStale = 8.0f;             // how far (log2) a tile's maximum may exceed the row's before it moves
 
@@ -101,106 +99,24 @@ __device__ __forceinline__ int block_of(int t, int total, int blocks) {
 }
 
 struct Share {  // of a block; in shared memory
-    int total, first, last;   // tiles
+    int total, first, last;              // tiles
     int prefix_keys, prefix_tiles, own_first;
-    int head, row_tile, skipped;                     // where the share begins, if in the prefix
-    int own_row, own_head, own_skipped, own_keys;    // where its own tiles begin
+    int own_row, own_row_tile;           // the batch row that holds the first own tile of the share, and its first tile
 };
 
-struct Piece {
+// A piece, as the scheduling warp writes it down for the other roles.
+struct __align__(16) Piece {
     int place;                // item + block: of the scratch memory
-    bool prefix, both;        // both: the groups take different rows (else alternate tiles)
-    int head, row, rows;      // KV head, first batch row, batch rows
-    int key, keys, tiles;     // first key, keys to the end of the item, tiles
+    int head, row;            // KV head, first batch row
+    int key, keys, tiles;     // first key, keys to the end of the item, tiles (0: the share is at its end)
     int before;               // tiles of the share before it
-    bool both_next;           // of the piece after, if there is one
+    short rows;               // batch rows
+    bool both;                // the groups take different rows (else alternate tiles)
+    unsigned char kind;       // 1: of the prefix; 2: the piece after takes both halves of the rows
+    __device__ __forceinline__ bool prefix() const { return kind & 1; }
     __device__ __forceinline__ int tasks() const { return both ? 2 * tiles : tiles; }
 };
-
-// The pieces of a block's share, in order.  Every role walks it for itself.
-struct Walk {
-    int t, head, row, skipped, keys;  // next tile; its head, its batch row (prefix: tile of rows), tiles of the item before it; own keys
-    bool own;
-    __device__ __forceinline__ explicit Walk(const Share& s) {
-        t = s.first, own = false, head = s.head, row = s.row_tile, skipped = s.skipped, keys = 0;
-    }
-    // row_keys: own keys of the rows, where the block has them in shared memory
-    __device__ __forceinline__ bool step(const PrefixArgs& a, const Share& s, const int* row_keys, Piece& p) {
-        if (t >= s.last) return false;
-        p.before = t - s.first;
-        if (t < s.own_first) {
-            p.prefix = true;
-            p.head = head;
-            p.row = row * 2 * a.tile_rows;
-            p.rows = min(2 * a.tile_rows, a.batch - p.row);
-            p.both = p.rows > a.tile_rows;
-            p.key = skipped * kKeys, p.keys = s.prefix_keys - p.key;
-            p.tiles = min(s.prefix_tiles - skipped, s.last - t);
-            p.place = head * a.row_tiles + row + int(blockIdx.x);
-            if (++row == a.row_tiles) row = 0, ++head;
-            p.both_next = t + p.tiles < min(s.own_first, s.last) && a.batch - row * 2 * a.tile_rows > a.tile_rows;
-        } else {
-            if (!own) {
-                own = true, head = s.own_head, row = s.own_row, skipped = s.own_skipped, keys = s.own_keys;
-            } else if (head == a.nkv) {
-                head = 0;
-                do {  // (t is before the end of the sequence: some row has it)
-                    ++row;
-                    keys = a.batch <= kThreads ? row_keys[row] : own_keys(a, ld_mutable(a.positions + row));
-                } while (keys == 0);
-            }
-            p.prefix = false, p.both = false, p.both_next = false;
-            p.head = head, p.row = row, p.rows = 1;
-            p.key = skipped * kKeys, p.keys = keys - p.key;
-            p.tiles = min((p.keys + kKeys - 1) / kKeys, s.last - t);
-            p.place = row * a.nkv + head + int(blockIdx.x);
-            ++head;
-        }
-        skipped = 0;
-        t += p.tiles;
-        return true;
-    }
-};
-
-// The tasks of a share, one after the other through its pieces.  Number k is group k & 1's; in a piece of
-// both halves of the rows a tile is two tasks, in others one.
-struct Tasks {
-    Walk walk;
-    Piece p;
-    int t, tasks;             // number of the task in its piece, and how many that has
-    uint32_t query;           // query buffers filled before the piece
-    bool both_before;         // of the piece before
-    bool valid;
-    __device__ __forceinline__ Tasks(const PrefixArgs& a, const Share& s, const int* row_keys, int first) : walk(s) {
-        t = first, query = 0, both_before = false;
-        valid = walk.step(a, s, row_keys, p);
-        tasks = valid ? p.tasks() : 0;
-        advance(a, s, row_keys, 0);
-    }
-    __device__ __forceinline__ void advance(const PrefixArgs& a, const Share& s, const int* row_keys, int by) {
-        t += by;
-        while (valid && t >= tasks) {
-            t -= tasks;
-            query += p.both ? 2 : 1, both_before = p.both;
-            valid = walk.step(a, s, row_keys, p);
-            tasks = valid ? p.tasks() : 0;
-        }
-    }
-    __device__ __forceinline__ int tile() const { return p.both ? t >> 1 : t; }
-};
-// K and V of a tile are these loads of the share: each group's products want their tiles in this order.
-// While the groups alternate, S(0) S(1) O(0) S(2) O(1) S(3) ... K of the tile after next comes before V of
-// the next one; beside a tile that both take, it does not, since the other group is at that V first.
-__device__ __forceinline__ uint32_t load_of_k(const Tasks& k) {
-    const int n = k.p.before + k.tile();
-    const bool before = k.tile() > 0 ? k.p.both : k.both_before;
-    return n == 0 ? 0u : uint32_t(2 * n - (before || k.p.both ? 0 : 1));
-}
-__device__ __forceinline__ uint32_t load_of_v(const Piece& p, int tile, int share_tiles) {
-    const int n = p.before + tile;
-    const bool after = tile < p.tiles - 1 ? p.both : p.both_next;
-    return uint32_t(2 * n + (p.both || after || n == share_tiles - 1 ? 1 : 2));
-}
+constexpr int kBatch = 16;    // pieces that are written down at a time; there are two such batches
 
 // ---- scratch memory: of a piece, per group, O as [D / 4][rows] float4, then m [rows] and l [rows] ----
 
@@ -255,21 +171,15 @@ __device__ __forceinline__ void tmem_arrived(uint32_t* v) {  // (v passes throug
                  :
                  : "memory");
 }
-__device__ __forceinline__ void tmem_put_32(uint32_t taddr, const uint32_t* v) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
-        "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
-        "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
-        : "memory");
-}
 __device__ __forceinline__ float exp2_approx(float x) {  // relative error 2^-22
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
 }
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     float2 r;
@@ -291,24 +201,128 @@ __device__ __forceinline__ uint64_t value_desc(uint32_t addr, uint32_t half) {
            (uint64_t(1) << 46) | (uint64_t(2) << 61);
 }
 
-__device__ __forceinline__ void tmem_put_16(uint32_t taddr, const uint32_t* v) {
+__device__ __forceinline__ void tmem_put_32(uint32_t taddr, const uint32_t* v) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
         "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
+        "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
+        "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
         : "memory");
 }
+__device__ __forceinline__ void tmem_take_8(uint32_t (&v)[8], uint32_t taddr) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_put_8(uint32_t taddr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map)); }
+
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {  // does not suspend the thread
+    uint32_t ok;
+    asm volatile(
+        "{\n.reg .pred p;\n"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        "selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
 
 struct Barriers {
     uint64_t full[10], empty[10];          // tiles of K and V
     uint64_t query_full[2], query_empty[2];
-    uint64_t scores[2], weights[2][2], result[2];  // of the groups: S is there, P's halves are there, O of a piece is complete
-    uint32_t tmem_base;
+    uint64_t scores[2][2], weights[2][2];  // of the groups' halves of a tile: S is there, P is there
+    uint64_t summed[2], result[2];         // of the groups: P . V of a half is done; O of a piece is complete
+    uint64_t turn[2];                      // the exponential unit is this group's
+    uint64_t list_full[2], list_empty[2];  // batches of pieces
+    Piece list[2 * kBatch];
     Share share;
+    uint32_t tmem_base;
     int warp_tiles[kThreads / 32];
-    int row_keys[kThreads];                // own keys of the rows, of batches that small
 };
+constexpr int kListReaders = 3 + 8;        // producer, issuers, warps of the groups
+
+// One role's way through the pieces.  Every batch is waited for, and handed back by the roles that are
+// counted for it.
+struct Pieces {
+    Barriers* bars;
+    uint32_t i;               // pieces read
+    __device__ __forceinline__ explicit Pieces(Barriers* b) : bars(b), i(0) {}
+    // One thread's: the next piece; one without tiles at the end (or when a wait has expired).
+    __device__ __forceinline__ Piece next(bool hand_back, bool* ok, int* error) {
+        const uint32_t batch = i / kBatch;
+        if (i % kBatch == 0) {
+            if (hand_back && batch > 0) mbar_arrive(&bars->list_empty[(batch - 1) & 1]);
+            *ok = *ok && mbar_wait(&bars->list_full[batch & 1], (batch >> 1) & 1, error, 51);
+        }
+        Piece p = bars->list[i % (2 * kBatch)];
+        if (!*ok) p.tiles = 0;
+        ++i;
+        return p;
+    }
+    // A whole warp's.
+    __device__ __forceinline__ Piece next_of_warp(bool* ok, int* error) {
+        const uint32_t batch = i / kBatch;
+        if (i % kBatch == 0) {
+            __syncwarp();
+            if (batch > 0 && threadIdx.x % 32 == 0) mbar_arrive(&bars->list_empty[(batch - 1) & 1]);
+            *ok = *ok && __all_sync(0xFFFFFFFFu, mbar_wait(&bars->list_full[batch & 1], (batch >> 1) & 1, error, 51));
+        }
+        Piece p = bars->list[i % (2 * kBatch)];
+        if (!*ok) p.tiles = 0;
+        ++i;
+        return p;
+    }
+};
+
+// The tasks of a share, one after the other through its pieces.  Number k is group k & 1's; in a piece of
+// both halves of the rows a tile is two tasks, in others one.
+struct Tasks {
+    Pieces pieces;
+    Piece p;
+    int t;                    // number of the task in its piece
+    uint32_t query;           // query buffers filled before the piece
+    bool both_before;         // of the piece before
+    __device__ __forceinline__ Tasks(Barriers* bars, int first, bool hand_back, bool* ok, int* error) : pieces(bars) {
+        t = first, query = 0, both_before = false;
+        p = pieces.next(hand_back, ok, error);
+        advance(0, hand_back, ok, error);
+    }
+    __device__ __forceinline__ bool valid() const { return p.tiles > 0; }
+    __device__ __forceinline__ void advance(int by, bool hand_back, bool* ok, int* error) {
+        t += by;
+        while (p.tiles > 0 && t >= p.tasks()) {
+            t -= p.tasks();
+            query += p.both ? 2 : 1, both_before = p.both;
+            p = pieces.next(hand_back, ok, error);
+        }
+    }
+    __device__ __forceinline__ int tile() const { return p.both ? t >> 1 : t; }
+};
+// K and V of a tile are these loads of the share: each group's products want their tiles in this order.
+// While the groups alternate, S(0) S(1) O(0) S(2) O(1) S(3) ... K of the tile after next comes before V of
+// the next one; beside a tile that both take, it does not, since the other group is at that V first.
+__device__ __forceinline__ uint32_t load_of_k(const Tasks& k) {
+    const int n = k.p.before + k.tile();
+    const bool before = k.tile() > 0 ? k.p.both : k.both_before;
+    return n == 0 ? 0u : uint32_t(2 * n - (before || k.p.both ? 0 : 1));
+}
+__device__ __forceinline__ uint32_t load_of_v(const Piece& p, int tile, int share_tiles) {
+    const int n = p.before + tile;
+    const bool after = tile < p.tiles - 1 ? p.both : (p.kind & 2) != 0;
+    return uint32_t(2 * n + (p.both || after || n == share_tiles - 1 ? 1 : 2));
+}
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -323,7 +337,6 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
     uint8_t* slots = smem + 2 * S::kQuery;
     Barriers& bars = *reinterpret_cast<Barriers*>(smem + S::kBytes);
     Share& share = bars.share;
-    const int* row_keys = bars.row_keys;
     const int warp = __shfl_sync(0xFFFFFFFFu, int(threadIdx.x) / 32, 0), lane = threadIdx.x % 32;
 
     if (threadIdx.x == kProducerWarp * 32) {
@@ -335,8 +348,9 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
         for (int s = 0; s < S::kSlots; ++s) mbar_init(&bars.full[s], 1), mbar_init(&bars.empty[s], 2);
         for (int g = 0; g < 2; ++g) {
             mbar_init(&bars.query_full[g], 1), mbar_init(&bars.query_empty[g], 2);
-            mbar_init(&bars.scores[g], 1), mbar_init(&bars.result[g], 1);
-            mbar_init(&bars.weights[g][0], 4), mbar_init(&bars.weights[g][1], 4);
+            for (int h = 0; h < 2; ++h) mbar_init(&bars.scores[g][h], 1), mbar_init(&bars.weights[g][h], 4);
+            mbar_init(&bars.summed[g], 1), mbar_init(&bars.result[g], 1), mbar_init(&bars.turn[g], 4);
+            mbar_init(&bars.list_full[g], 1), mbar_init(&bars.list_empty[g], kListReaders);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -358,7 +372,6 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
             const int64_t position = ld_mutable(a.positions + b);
             if (blockIdx.x == 0 && (position < -1 || position >= a.slots)) record_bad_position(a.status, b);
             mine += own_tiles(a, position);
-            if (per == 1) bars.row_keys[b] = own_keys(a, position);
         }
         int before = mine;
 #pragma unroll
@@ -385,22 +398,16 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
         if (threadIdx.x == 0) {
             share.total = total, share.first = first, share.last = last;
             share.prefix_keys = keys, share.prefix_tiles = tiles, share.own_first = own_first;
-            if (first < own_first) {
-                const int item = first / tiles, head = item / a.row_tiles;
-                share.skipped = first - item * tiles, share.head = head, share.row_tile = item - head * a.row_tiles;
-            }
         }
         const int begin = own_first + before * a.nkv, end = begin + mine * a.nkv;
         if (look >= begin && look < end) {
-            int row = from, at = begin, each = mine;  // (one row a thread: it is this one)
-            for (; per > 1; ++row) {
-                each = own_tiles(a, ld_mutable(a.positions + row));
+            int row = from, at = begin;
+            for (; per > 1; ++row) {  // (one row a thread: it is this one)
+                const int each = own_tiles(a, ld_mutable(a.positions + row));
                 if (look < at + each * a.nkv) break;
                 at += each * a.nkv;
             }
-            const int head = (look - at) / each;
-            share.own_row = row, share.own_head = head, share.own_skipped = look - at - head * each;
-            share.own_keys = own_keys(a, ld_mutable(a.positions + row));
+            share.own_row = row, share.own_row_tile = at;
         }
         if (blockIdx.x == 0) {  // for the joining kernel
             int c = before;
@@ -421,28 +428,27 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
     };
     bool ok = true;
 
-    if (warp >= kProducerWarp) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
     if (warp == kProducerWarp) {
         if (lane == 0) {
-            Tasks keys(a, share, row_keys, 0), values(a, share, row_keys, 0);
+            Tasks keys(&bars, 0, false, &ok, a.error), values(&bars, 0, true, &ok, a.error);
             const uint32_t loads = uint32_t(2 * (share.last - share.first));
             uint32_t n = 0, slot = 0, lap = 0;
-            auto load = [&](Tasks& task, const CUtensorMap* shared, const CUtensorMap* own) {
+            auto load = [&](Tasks& task, bool hand_back, const CUtensorMap* shared, const CUtensorMap* own) {
                 mbar_expect_tx(&bars.full[slot], S::kSlot);
                 const int key = task.p.key + task.tile() * kKeys;
 #pragma unroll
                 for (int h = 0; h < S::kHalves; ++h) {
                     const uint32_t dst = smem_u32(slots) + slot * S::kSlot + h * S::kHalf;
-                    if (task.p.prefix) tma_load_3d(dst, shared, h * 64, key, task.p.head, &bars.full[slot]);
+                    if (task.p.prefix()) tma_load_3d(dst, shared, h * 64, key, task.p.head, &bars.full[slot]);
                     else tma_load_4d(dst, own, h * 64, key, task.p.head, task.p.row, &bars.full[slot]);
                 }
-                task.advance(a, share, row_keys, task.p.both ? 2 : 1);  // to the next tile
+                task.advance(task.p.both ? 2 : 1, hand_back, &ok, a.error);  // to the next tile
             };
             for (; n < loads; ++n) {
-                ok = lap == 0 || mbar_wait(&bars.empty[slot], (lap - 1) & 1, a.error, 41);
+                ok = ok && (lap == 0 || mbar_wait(&bars.empty[slot], (lap - 1) & 1, a.error, 41));
                 if (!ok) break;
-                if (keys.valid && load_of_k(keys) == n) load(keys, &prefix_k, &cache_k);
-                else load(values, &prefix_v, &cache_v);
+                if (keys.valid() && load_of_k(keys) == n) load(keys, false, &prefix_k, &cache_k);
+                else load(values, true, &prefix_v, &cache_v);
                 if (++slot == S::kSlots) slot = 0, ++lap;
             }
             if (!ok)  // what is in flight lands before the block leaves
@@ -453,11 +459,11 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
         // ---- the products of group g, from one thread ----
         if (elect_one()) {
             constexpr uint32_t kType = H::kDtype == B200Q_BF16 ? 1u : 0u;
-            constexpr uint32_t kScores = (1u << 4) | (kType << 7) | (kType << 10) | (uint32_t(kKeys >> 3) << 17) | (uint32_t(kRows >> 4) << 24);
+            constexpr uint32_t kScores = (1u << 4) | (kType << 7) | (kType << 10) | (uint32_t(kPart >> 3) << 17) | (uint32_t(kRows >> 4) << 24);
             constexpr uint32_t kValues = (1u << 4) | (kType << 7) | (kType << 10) | (1u << 16) | (uint32_t(HD >> 3) << 17) | (uint32_t(kRows >> 4) << 24);
             const int g = warp - kIssuerWarp, share_tiles = share.last - share.first;
             const uint32_t s_at = tmem + uint32_t(g) * kKeys, o_at = tmem + 2 * kKeys + uint32_t(g) * HD;
-            Tasks scores(a, share, row_keys, g), values(a, share, row_keys, g);
+            Tasks scores(&bars, g, false, &ok, a.error), values(&bars, g, true, &ok, a.error);
             // Both issuers see every load and every buffer of queries, in order, and hand it back: a waiter
             // that left one out could not tell a barrier's phase from the one after next.
             uint32_t loads = 0, queries = 0;  // those handed back
@@ -477,47 +483,72 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
                     if (ok) mbar_arrive(&bars.query_empty[queries & 1]);
                 }
             };
-            auto issue_scores = [&]() {
+            uint32_t k_slot = 0, k_query = 0;
+            auto parts = [](const Tasks& task) { return task.p.keys - task.tile() * kKeys > kPart ? 2 : 1; };  // halves with any key
+            auto issue_scores = [&](int h) {  // half h of the next tile
                 const Piece& p = scores.p;
-                const uint32_t query = scores.query + (p.both ? uint32_t(scores.t & 1) : 0u), buffer = query & 1;
-                if (scores.t < 2) {
-                    pass_queries(query);
-                    ok = ok && mbar_wait(&bars.query_full[buffer], (query >> 1) & 1, a.error, 43);
-                    queries = query + 1;
+                if (h == 0) {
+                    const uint32_t query = scores.query + (p.both ? uint32_t(scores.t & 1) : 0u);
+                    k_query = query & 1;
+                    if (scores.t < 2) {
+                        pass_queries(query);
+                        ok = ok && mbar_wait(&bars.query_full[k_query], (query >> 1) & 1, a.error, 43);
+                        queries = query + 1;
+                    }
+                    k_slot = take_load(load_of_k(scores));
                 }
-                const uint32_t slot = take_load(load_of_k(scores));
                 if (!ok) return;
                 tc_fence_after();
-                const uint64_t qd = smem_desc(smem_u32(smem) + buffer * S::kQuery), kd = smem_desc(smem_u32(slots) + slot * S::kSlot);
+                const uint64_t qd = smem_desc(smem_u32(smem) + k_query * S::kQuery);
+                const uint64_t kd = smem_desc(smem_u32(slots) + k_slot * S::kSlot + uint32_t(h) * (kPart * 128));
 #pragma unroll
                 for (int k = 0; k < HD / 16; ++k) {
                     const uint32_t step = uint32_t(k / 4) * (S::kHalf >> 4) + uint32_t(k % 4) * 2;
-                    umma_f16_ss(s_at, qd + step, kd + step, kScores, k > 0);
+                    umma_f16_ss(s_at + uint32_t(h) * kPart, qd + step, kd + step, kScores, k > 0);
                 }
-                umma_commit(&bars.scores[g]);
-                umma_commit(&bars.empty[slot]);
-                if (scores.t >= scores.tasks - 2) umma_commit(&bars.query_empty[buffer]);
-                scores.advance(a, share, row_keys, 2);
+                umma_commit(&bars.scores[g][h]);
+                if (h + 1 < parts(scores)) return;
+                umma_commit(&bars.empty[k_slot]);
+                if (scores.t >= p.tasks() - 2) umma_commit(&bars.query_empty[k_query]);
+                scores.advance(2, false, &ok, a.error);
             };
-            if (scores.valid) issue_scores();
-            for (uint32_t n = 0; ok && values.valid; ++n) {
+            auto issue_rest = [&](int h) {  // of the next tile, from half h on
+                const int n = parts(scores);
+                for (; h < n && ok; ++h) issue_scores(h);
+            };
+            if (scores.valid()) issue_rest(0);
+            uint32_t given[2] = {0, 0};
+            while (ok && values.valid()) {
                 const int valid = values.p.keys - values.tile() * kKeys;
                 const uint32_t slot = take_load(load_of_v(values.p, values.tile(), share_tiles));
                 const uint64_t vd = value_desc(smem_u32(slots) + slot * S::kSlot, S::kHalf);
+                int issued = 0;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    ok = ok && mbar_wait(&bars.weights[g][h], n & 1, a.error, 45);
+                    if (h * kPart >= valid) break;
+                    ok = ok && mbar_wait(&bars.weights[g][h], given[h]++ & 1, a.error, 45);
                     if (!ok) break;
                     tc_fence_after();
 #pragma unroll
                     for (int k = 4 * h; k < 4 * h + 4; ++k)
-                        if (k == 0 || k * 16 < valid) umma_f16_ts(o_at, s_at + k * 8, vd + uint32_t(k) * (2048 >> 4), kValues, k > 0 || values.t >= 2);
+                        if (k == 0 || k * 16 < valid)
+                            umma_f16_ts(o_at, s_at + h * kPart + (k - 4 * h) * 8, vd + uint32_t(k) * (2048 >> 4), kValues, k > 0 || values.t >= 2);
+                    umma_commit(&bars.summed[g]);
+                    // the next tile's first half, unless it would have to be waited for
+                    if (h == 0 && valid > kPart && scores.valid() && scores.t >= 2) {
+                        const uint32_t load = load_of_k(scores);
+                        if (loads == load && mbar_test(&bars.full[load % S::kSlots], (load / S::kSlots) & 1)) {
+                            const bool more = parts(scores) > 1;
+                            issue_scores(0);
+                            issued = more ? 1 : 2;
+                        }
+                    }
                 }
                 if (!ok) break;
                 umma_commit(&bars.empty[slot]);
-                if (values.t >= values.tasks - 2) umma_commit(&bars.result[g]);
-                values.advance(a, share, row_keys, 2);
-                if (scores.valid) issue_scores();
+                if (values.t >= values.p.tasks() - 2) umma_commit(&bars.result[g]);
+                values.advance(2, true, &ok, a.error);
+                if (issued < 2 && scores.valid()) issue_rest(issued);
             }
             pass_queries(scores.query);
             if (share_tiles > 0 && ok) {
@@ -527,159 +558,210 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
         }
         __syncwarp();
     } else if (warp == kQueryWarp) {
-        if (lane == 0) {
-            Walk walk(share);
-            Piece p;
-            uint32_t query = 0;
-            while (ok && walk.step(a, share, row_keys, p)) {
+        // ---- the pieces, a batch at a time, and their queries ----
+        int t = share.first, row = share.own_row, at = share.own_row_tile;
+        int keys_of = 0, held = -1;            // own keys of rows 32 * held + lane
+        const int prefix_end = min(share.own_first, share.last);
+        uint32_t query = 0;
+        for (uint32_t batch = 0; ok; ++batch) {
+            if (batch >= 2) ok = wait(&bars.list_empty[batch & 1], ((batch >> 1) - 1) & 1, 52);
+            if (!ok) break;
+            Piece* list = bars.list + (batch & 1) * kBatch;
+            int n = 0;
+            bool over = false;
+            while (n < kBatch && !over) {
+                Piece p;
+                int begin, end;                // tiles of this lane's piece
+                if (t < prefix_end) {          // an item a lane
+                    const int item = t / share.prefix_tiles + lane, head = item / a.row_tiles, tile = item - head * a.row_tiles;
+                    const int first = item * share.prefix_tiles;
+                    begin = max(t, first), end = min(first + share.prefix_tiles, prefix_end);
+                    p.head = head, p.row = tile * 2 * a.tile_rows;
+                    p.rows = short(min(2 * a.tile_rows, a.batch - p.row));
+                    p.both = p.rows > a.tile_rows;
+                    const int row_next = tile + 1 == a.row_tiles ? 0 : p.row + 2 * a.tile_rows;
+                    p.kind = 1 | (end < prefix_end && a.batch - row_next > a.tile_rows ? 2 : 0);
+                    p.key = (begin - first) * kKeys, p.keys = share.prefix_keys - p.key;
+                    p.place = item + int(blockIdx.x);
+                } else if (t < share.last) {   // a head of the row a lane
+                    int keys, each;
+                    for (;; ++row) {           // (t is before the end of the sequence: some row has it)
+                        if (row / 32 != held) {
+                            held = row / 32;
+                            const int r = held * 32 + lane;
+                            keys_of = r < a.batch ? own_keys(a, ld_mutable(a.positions + r)) : 0;
+                        }
+                        keys = __shfl_sync(0xFFFFFFFFu, keys_of, row % 32);
+                        each = (keys + kKeys - 1) / kKeys;
+                        if (t < at + each * a.nkv) break;
+                        at += each * a.nkv;
+                    }
+                    const int head = (t - at) / each + lane, first = at + head * each;
+                    begin = max(t, first), end = head < a.nkv ? min(first + each, share.last) : begin;
+                    p.head = head, p.row = row, p.rows = 1, p.both = false, p.kind = 0;
+                    p.key = (begin - first) * kKeys, p.keys = keys - p.key;
+                    p.place = row * a.nkv + head + int(blockIdx.x);
+                } else {
+                    over = true;
+                    begin = end = t;
+                    if (lane == 0) list[n].tiles = 0;
+                }
+                const bool there = begin < end && n + lane < kBatch;
+                const int count = __popc(__ballot_sync(0xFFFFFFFFu, there));
+                if (there) {
+                    p.tiles = end - begin, p.before = begin - share.first;
+                    list[n + lane] = p;
+                }
+                if (count > 0) t = __shfl_sync(0xFFFFFFFFu, end, count - 1);
+                n += count;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.list_full[batch & 1]);
+            for (int i = 0; i < n && ok; ++i) {
+                const Piece& p = list[i];
                 for (int half = 0; half < (p.both ? 2 : 1); ++half, ++query) {
                     const uint32_t buffer = query & 1;
-                    ok = query < 2 || mbar_wait(&bars.query_empty[buffer], ((query >> 1) - 1) & 1, a.error, 47);
+                    ok = query < 2 || wait(&bars.query_empty[buffer], ((query >> 1) - 1) & 1, 47);
                     if (!ok) break;
-                    // (batch rows past the last one read as zeros; rows of the buffer past the box are never looked at)
-                    mbar_expect_tx(&bars.query_full[buffer], uint32_t(S::kHalves * 128 * a.rep * (p.prefix ? a.tile_rows : 1)));
+                    if (lane == 0) {
+                        // (batch rows past the last one read as zeros; rows of the buffer past the box are never looked at)
+                        mbar_expect_tx(&bars.query_full[buffer], uint32_t(S::kHalves * 128 * a.rep * (p.prefix() ? a.tile_rows : 1)));
 #pragma unroll
-                    for (int h = 0; h < S::kHalves; ++h)
-                        tma_load_4d(smem_u32(smem) + buffer * S::kQuery + h * (kRows * 128), p.prefix ? &prefix_q : &own_q, h * 64, 0,
-                                    p.head, p.row + half * a.tile_rows, &bars.query_full[buffer]);
+                        for (int h = 0; h < S::kHalves; ++h)
+                            tma_load_4d(smem_u32(smem) + buffer * S::kQuery + h * (kRows * 128), p.prefix() ? &prefix_q : &own_q, h * 64, 0,
+                                        p.head, p.row + half * a.tile_rows, &bars.query_full[buffer]);
+                    }
+                    __syncwarp();
                 }
             }
-            if (!ok)
-                for (uint32_t i = query > 2 ? query - 2 : 0; i < query; ++i) mbar_wait(&bars.query_full[i & 1], (i >> 1) & 1, a.error, 42);
+            if (over) break;
         }
+        if (!ok && lane == 0)
+            for (uint32_t i = query > 2 ? query - 2 : 0; i < query; ++i) mbar_wait(&bars.query_full[i & 1], (i >> 1) & 1, a.error, 42);
         __syncwarp();
     } else if (warp < kProducerWarp) {
         // ---- softmax: group g, one query row a thread ----
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
         const int g = warp / 4, row = threadIdx.x % 128;
         const uint32_t lanes = tmem + (uint32_t(warp & 3) << 21);
         const uint32_t s_at = lanes + uint32_t(g) * kKeys, o_at = lanes + 2 * kKeys + uint32_t(g) * HD;
-        Walk walk(share);
-        Piece p;
-        uint32_t first_task = 0, done = 0, pieces = 0;  // of the piece; tasks and pieces that this group has had
+        Pieces list(&bars);
+        uint32_t first_task = 0, pieces = 0;      // of the piece; pieces that this group has had
+        uint32_t had = 0, had_first = 0;          // halves of tiles that this group has had, and first halves
         const int share_tiles = share.last - share.first;
-        while (ok && walk.step(a, share, row_keys, p)) {
+        const float2 scale = make_float2(a.scale_log2, a.scale_log2);
+        // Where both groups take every tile they would run in step, both at their exponentials and then
+        // both at none: they take the exponential unit in turn.
+        uint32_t turns = 0;
+        auto take_turn = [&]() {
+            const uint32_t before = g == 0 ? turns - 1 : turns;  // of the other group's
+            if (g == 1 || turns > 0) ok = ok && wait(&bars.turn[g], before & 1, 54);
+            ++turns;
+        };
+        auto give_turn = [&]() {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.turn[g ^ 1]);
+        };
+        for (;;) {
+            const Piece p = list.next_of_warp(&ok, a.error);
+            if (p.tiles == 0) break;
             // which of the piece's tasks are this group's: every other one, and of both halves of the rows always the same half
             const int t0 = g ^ int(first_task & 1), live = p.both ? min(a.tile_rows, p.rows - t0 * a.tile_rows) * a.rep : p.rows * a.rep;
             const bool any = (warp & 3) * 32 < live;  // of this warp's rows
             first_task += uint32_t(p.tasks());
-            float m = -INFINITY, l = 0.0f;
-            for (int tile = p.both ? 0 : t0; tile < p.tiles && ok; tile += p.both ? 1 : 2) {
-                ok = wait(&bars.scores[g], done & 1, 48);
-                if (!ok) break;
-                ++done;
-                tc_fence_after();
+            float m = 0.0f, l = 0.0f;
+            const int first = p.both ? 0 : t0, step = p.both ? 1 : 2;
+            for (int tile = first; tile < p.tiles && ok; tile += step) {
                 const int valid = p.keys - tile * kKeys;  // keys of the tile, and more
-                // m of the row, `here` being the largest score of this tile
-                auto moved = [&](float here) {
-                    if (tile < (p.both ? 1 : 2)) {  // the group's first
-                        m = here == -INFINITY ? 0.0f : here;
-                    } else if (__any_sync(0xFFFFFFFFu, row < live && here > m + kStale)) {
-                        const float next = here > m + kStale ? here : m, by = exp2_approx(m - next);
-                        m = next;
-                        l *= by;
+#pragma unroll 1
+                for (int h = 0; h * kPart < min(valid, kKeys); ++h) {
+                    const int keys = valid - h * kPart;   // of this half, and more
+                    const uint32_t at = s_at + uint32_t(h) * kPart;
+                    const uint32_t turn = h == 0 ? had_first++ : had - had_first;
+                    ok = wait(&bars.scores[g][h], turn & 1, 48);
+                    if (!ok) break;
+                    ++had;
+                    tc_fence_after();
+                    if (any) {
+                        // Few warps run here, so every step is written as independent instructions in a row.
+                        uint32_t v[kPart];
+                        tmem_ask_32(v, at), tmem_ask_32(v + 32, at + 32);
+                        tmem_arrived(v), tmem_arrived(v + 32);
+                        if (keys < kPart) {
 #pragma unroll
-                        for (int c = 0; c < HD; c += 32) {
-                            uint32_t o[32];
-                            tmem_ask_32(o, o_at + c);
-                            tmem_arrived(o);
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * by);
-                            tmem_put_32(o_at + c, o);
+                            for (int i = 0; i < kPart; ++i) v[i] = i < keys ? v[i] : 0xFF800000u;
                         }
+                        float most[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) most[i] = __uint_as_float(v[i]);
+#pragma unroll
+                        for (int i = 8; i < kPart - 8; i += 16)
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) most[k] = max3(most[k], __uint_as_float(v[i + k]), __uint_as_float(v[i + 8 + k]));
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) most[k] = fmaxf(most[k], __uint_as_float(v[kPart - 8 + k]));
+                        const float here = a.scale_log2 * fmaxf(max3(max3(most[0], most[1], most[2]), most[3], most[4]),
+                                                                max3(most[5], most[6], most[7]));
+                        if (tile == first && h == 0) {
+                            m = here == -INFINITY ? 0.0f : here;
+                        } else if (__any_sync(0xFFFFFFFFu, row < live && here > m + kStale)) {
+                            const float next = here > m + kStale ? here : m, by = exp2_approx(m - next);
+                            m = next;
+                            l *= by;
+                            // (these scores were asked for behind the sums before the last ones)
+                            ok = wait(&bars.summed[g], (had - 2) & 1, 53);
+                            tc_fence_after();
+#pragma unroll 1
+                            for (int c = 0; c < HD; c += 8) {
+                                uint32_t o[8];
+                                tmem_take_8(o, o_at + c);
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * by);
+                                tmem_put_8(o_at + c, o);
+                            }
+                        }
+                        const float2 minus = make_float2(-m, -m);
+                        float2 sum[4];
+                        float2 e[kPart / 2];
+                        if (p.both) take_turn();
+#pragma unroll
+                        for (int i = 0; i < kPart / 2; ++i) e[i] = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), scale, minus);
+#pragma unroll
+                        for (int i = 0; i < kPart / 2; ++i) e[i] = make_float2(exp2_approx(e[i].x), exp2_approx(e[i].y));
+#pragma unroll
+                        for (int i = 0; i < kPart / 2; ++i) sum[i & 3] = i < 4 ? e[i] : add2(sum[i & 3], e[i]);
+#pragma unroll
+                        for (int i = 0; i < kPart / 2; ++i) v[i] = H::pack(e[i].x, e[i].y);
+                        tmem_put_32(at, v);
+                        if (p.both) give_turn();
+                        const float2 pair = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+                        l += pair.x + pair.y;
+                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    } else if (p.both) {
+                        take_turn(), give_turn();
                     }
-                };
-                auto give = [&](int h) {
+                    if (keys < kPart) {
+                        // Rows of V past the last key may hold anything, and 0 * NaN is no 0: those that the last
+                        // step of 16 keys takes in are cleared (by either group where both use the tile).
+                        const uint32_t load = load_of_v(p, tile, share_tiles), slot = load % S::kSlots;
+                        ok = ok && wait(&bars.full[slot], (load / S::kSlots) & 1, 49);
+                        if (!ok) break;
+                        uint8_t* tail = slots + slot * S::kSlot;
+                        const int rows = (16 - valid % 16) % 16;
+                        for (int i = row; i < rows * 8 * S::kHalves; i += 128) {
+                            const int c = S::kHalves == 1 ? 0 : (i >> 3) & 1, r = valid + (i >> 3) / S::kHalves;
+                            *reinterpret_cast<uint4*>(tail + c * S::kHalf + r * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+                        }
+                        fence_proxy_async();
+                    }
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&bars.weights[g][h]);
-                };
-                const float2 scale = make_float2(a.scale_log2, a.scale_log2);
-                float2 sum = make_float2(0.0f, 0.0f);
-                // 2 weights of two scores, packed
-                auto weigh = [&](uint32_t x, uint32_t y, float2 minus) {
-                    const float2 t = fma2(make_float2(__uint_as_float(x), __uint_as_float(y)), scale, minus);
-                    const float2 e = make_float2(exp2_approx(t.x), exp2_approx(t.y));
-                    sum = add2(sum, e);
-                    return H::pack(e.x, e.y);
-                };
-                if (any && valid >= kKeys) {
-                    uint32_t v[kKeys];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) tmem_ask_32(v + 32 * i, s_at + 32 * i);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) tmem_arrived(v + 32 * i);
-                    float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                    for (int i = 0; i < kKeys; i += 4)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) most[j] = fmaxf(most[j], __uint_as_float(v[i + j]));
-                    moved(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * a.scale_log2);
-                    const float2 minus = make_float2(-m, -m);
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        uint32_t w[32];
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) w[i] = weigh(v[64 * h + 2 * i], v[64 * h + 2 * i + 1], minus);
-                        tmem_put_32(s_at + 32 * h, w);
-                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                        if (h == 0) give(0);  // the first half's products begin
-                    }
-                    l += sum.x + sum.y;
-                } else if (any) {
-                    // the last tile of an item: 32 keys at a time, as far as there are keys
-                    const int chunks = (valid + 31) / 32;
-                    auto ask = [&](uint32_t* v, int c) {
-                        tmem_ask_32(v, s_at + 32 * c);
-                        tmem_arrived(v);
-                        const int rest = valid - 32 * c;
-                        if (rest < 32) {
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) v[i] = i < rest ? v[i] : 0xFF800000u;
-                        }
-                    };
-                    float most = -INFINITY;
-#pragma unroll 1
-                    for (int c = 0; c < chunks; ++c) {
-                        uint32_t v[32];
-                        ask(v, c);
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) most = fmaxf(most, __uint_as_float(v[i]));
-                    }
-                    moved(most * a.scale_log2);
-                    const float2 minus = make_float2(-m, -m);
-#pragma unroll 1
-                    for (int c = 0; c < chunks; ++c) {  // (a chunk's weights go where scores of chunks before it were)
-                        uint32_t v[32], w[16];
-                        ask(v, c);
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) w[i] = weigh(v[2 * i], v[2 * i + 1], minus);
-                        tmem_put_16(s_at + 16 * c, w);
-                    }
-                    l += sum.x + sum.y;
-                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 }
-                if (valid < kKeys) {
-                    // Rows of V past the last key may hold anything, and 0 * NaN is no 0: those that the last
-                    // step of 16 keys takes in are cleared (by either group where both use the tile).
-                    const uint32_t load = load_of_v(p, tile, share_tiles), slot = load % S::kSlots;
-                    ok = wait(&bars.full[slot], (load / S::kSlots) & 1, 49);
-                    if (!ok) break;
-                    uint8_t* tail = slots + slot * S::kSlot;
-                    const int rows = (16 - valid % 16) % 16;
-                    for (int i = row; i < rows * 8 * S::kHalves; i += 128) {
-                        const int h = S::kHalves == 1 ? 0 : (i >> 3) & 1, r = valid + (i >> 3) / S::kHalves;
-                        *reinterpret_cast<uint4*>(tail + h * S::kHalf + r * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
-                    }
-                    fence_proxy_async();
-                }
-                if (!any || valid < kKeys) give(0);
-                give(1);
             }
             if (!ok) break;
             // ---- the piece's result ----
-            const int span = p.prefix ? kRows : a.rep;  // rows of a group in the scratch memory
-            float* to = a.scratch + (p.prefix ? 0 : a.own_at) + (2 * int64_t(p.place) + t0) * group_floats(span, HD);
+            const int span = p.prefix() ? kRows : a.rep;  // rows of a group in the scratch memory
+            float* to = a.scratch + (p.prefix() ? 0 : a.own_at) + (2 * int64_t(p.place) + t0) * group_floats(span, HD);
             const bool worked = p.both || t0 < p.tiles;
             if (worked) {
                 ok = wait(&bars.result[g], pieces & 1, 50);
@@ -687,15 +769,15 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
                 ++pieces;
                 tc_fence_after();
                 if (any) {
-#pragma unroll
+                    uint4* column = reinterpret_cast<uint4*>(to) + row;
+#pragma unroll 1
                     for (int c = 0; c < HD; c += 32) {
                         uint32_t o[32];
                         tmem_ask_32(o, o_at + c);
                         tmem_arrived(o);
                         if (row < live) {
 #pragma unroll
-                            for (int i = 0; i < 32; i += 4)
-                                reinterpret_cast<uint4*>(to)[((c + i) / 4) * span + row] = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                            for (int i = 0; i < 32; i += 4, column += span) *column = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
                         }
                     }
                 }
