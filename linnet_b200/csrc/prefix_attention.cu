@@ -105,16 +105,19 @@ struct Share {  // of a block; in shared memory
 };
 
 // A piece, as the scheduling warp writes it down for the other roles.
+enum Who : unsigned char { kGroup0, kGroup1, kAlternate, kBoth };  // whose the tiles are: one group's, each group's in turn, all both's
 struct __align__(16) Piece {
     int place;                // item + block: of the scratch memory
     int head, row;            // KV head, first batch row
     int key, keys, tiles;     // first key, keys to the end of the item, tiles (0: the share is at its end)
     int before;               // tiles of the share before it
     short rows;               // batch rows
-    bool both;                // the groups take different rows (else alternate tiles)
-    unsigned char kind;       // 1: of the prefix; 2: the piece after takes both halves of the rows
-    __device__ __forceinline__ bool prefix() const { return kind & 1; }
-    __device__ __forceinline__ int tasks() const { return both ? 2 * tiles : tiles; }
+    unsigned char who;
+    bool prefix;
+    // of a group: its first tile of the piece, and how far on the next one is
+    __device__ __forceinline__ int first(int g) const { return who == kAlternate ? g : who == kBoth || who == g ? 0 : tiles; }
+    __device__ __forceinline__ int step() const { return who == kAlternate ? 2 : 1; }
+    __device__ __forceinline__ int queries() const { return who == kBoth ? 2 : 1; }  // buffers
 };
 constexpr int kBatch = 16;    // pieces that are written down at a time; there are two such batches
 
@@ -244,7 +247,6 @@ struct Barriers {
     uint64_t query_full[2], query_empty[2];
     uint64_t scores[2][2], weights[2][2];  // of the groups' halves of a tile: S is there, P is there
     uint64_t summed[2], result[2];         // of the groups: P . V of a half is done; O of a piece is complete
-    uint64_t turn[2];                      // the exponential unit is this group's
     uint64_t list_full[2], list_empty[2];  // batches of pieces
     Piece list[2 * kBatch];
     Share share;
@@ -253,17 +255,16 @@ struct Barriers {
 };
 constexpr int kListReaders = 3 + 8;        // producer, issuers, warps of the groups
 
-// One role's way through the pieces.  Every batch is waited for, and handed back by the roles that are
-// counted for it.
+// One role's way through the pieces.  Every batch is waited for and handed back.
 struct Pieces {
     Barriers* bars;
     uint32_t i;               // pieces read
     __device__ __forceinline__ explicit Pieces(Barriers* b) : bars(b), i(0) {}
     // One thread's: the next piece; one without tiles at the end (or when a wait has expired).
-    __device__ __forceinline__ Piece next(bool hand_back, bool* ok, int* error) {
+    __device__ __forceinline__ Piece next(bool* ok, int* error) {
         const uint32_t batch = i / kBatch;
         if (i % kBatch == 0) {
-            if (hand_back && batch > 0) mbar_arrive(&bars->list_empty[(batch - 1) & 1]);
+            if (batch > 0) mbar_arrive(&bars->list_empty[(batch - 1) & 1]);
             *ok = *ok && mbar_wait(&bars->list_full[batch & 1], (batch >> 1) & 1, error, 51);
         }
         Piece p = bars->list[i % (2 * kBatch)];
@@ -286,42 +287,45 @@ struct Pieces {
     }
 };
 
-// The tasks of a share, one after the other through its pieces.  Number k is group k & 1's; in a piece of
-// both halves of the rows a tile is two tasks, in others one.
+// A group's tiles, one after the other through the pieces.
 struct Tasks {
     Pieces pieces;
     Piece p;
-    int t;                    // number of the task in its piece
+    int g, tile;
     uint32_t query;           // query buffers filled before the piece
-    bool both_before;         // of the piece before
-    __device__ __forceinline__ Tasks(Barriers* bars, int first, bool hand_back, bool* ok, int* error) : pieces(bars) {
-        t = first, query = 0, both_before = false;
-        p = pieces.next(hand_back, ok, error);
-        advance(0, hand_back, ok, error);
+    // `leave` is called for every piece that is left behind, the group's or not, with the buffers filled up to its end.
+    template <typename Leave>
+    __device__ __forceinline__ Tasks(Barriers* bars, int group, bool* ok, int* error, Leave leave) : pieces(bars) {
+        g = group, query = 0;
+        p = pieces.next(ok, error);
+        tile = p.first(g);
+        settle(ok, error, leave);
     }
     __device__ __forceinline__ bool valid() const { return p.tiles > 0; }
-    __device__ __forceinline__ void advance(int by, bool hand_back, bool* ok, int* error) {
-        t += by;
-        while (p.tiles > 0 && t >= p.tasks()) {
-            t -= p.tasks();
-            query += p.both ? 2 : 1, both_before = p.both;
-            p = pieces.next(hand_back, ok, error);
+    template <typename Leave>
+    __device__ __forceinline__ void settle(bool* ok, int* error, Leave leave) {
+        while (p.tiles > 0 && tile >= p.tiles) {
+            query += p.queries();
+            leave(p, query);
+            p = pieces.next(ok, error);
+            tile = p.first(g);
         }
     }
-    __device__ __forceinline__ int tile() const { return p.both ? t >> 1 : t; }
+    template <typename Leave>
+    __device__ __forceinline__ void advance(bool* ok, int* error, Leave leave) {
+        tile += p.step();
+        settle(ok, error, leave);
+    }
+    __device__ __forceinline__ bool starts() const { return tile == p.first(g); }
+    __device__ __forceinline__ bool ends() const { return tile + p.step() >= p.tiles; }
 };
-// K and V of a tile are these loads of the share: each group's products want their tiles in this order.
-// While the groups alternate, S(0) S(1) O(0) S(2) O(1) S(3) ... K of the tile after next comes before V of
-// the next one; beside a tile that both take, it does not, since the other group is at that V first.
-__device__ __forceinline__ uint32_t load_of_k(const Tasks& k) {
-    const int n = k.p.before + k.tile();
-    const bool before = k.tile() > 0 ? k.p.both : k.both_before;
-    return n == 0 ? 0u : uint32_t(2 * n - (before || k.p.both ? 0 : 1));
+// K and V of a tile are these loads of the share, in the order in which each group's products want them;
+// where the groups alternate, K of the tile after next comes before V of the next one.
+__device__ __forceinline__ uint32_t load_of_k(const Piece& p, int tile) {
+    return uint32_t(2 * (p.before + tile) - (p.who == kAlternate && tile > 0 ? 1 : 0));
 }
-__device__ __forceinline__ uint32_t load_of_v(const Piece& p, int tile, int share_tiles) {
-    const int n = p.before + tile;
-    const bool after = tile < p.tiles - 1 ? p.both : (p.kind & 2) != 0;
-    return uint32_t(2 * n + (p.both || after || n == share_tiles - 1 ? 1 : 2));
+__device__ __forceinline__ uint32_t load_of_v(const Piece& p, int tile) {
+    return uint32_t(2 * (p.before + tile) + (p.who == kAlternate && tile < p.tiles - 1 ? 2 : 1));
 }
 
 template <typename T, int HD>
@@ -349,7 +353,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
         for (int g = 0; g < 2; ++g) {
             mbar_init(&bars.query_full[g], 1), mbar_init(&bars.query_empty[g], 2);
             for (int h = 0; h < 2; ++h) mbar_init(&bars.scores[g][h], 1), mbar_init(&bars.weights[g][h], 4);
-            mbar_init(&bars.summed[g], 1), mbar_init(&bars.result[g], 1), mbar_init(&bars.turn[g], 4);
+            mbar_init(&bars.summed[g], 1), mbar_init(&bars.result[g], 1);
             mbar_init(&bars.list_full[g], 1), mbar_init(&bars.list_empty[g], kListReaders);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -430,26 +434,32 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
 
     if (warp == kProducerWarp) {
         if (lane == 0) {
-            Tasks keys(&bars, 0, false, &ok, a.error), values(&bars, 0, true, &ok, a.error);
-            const uint32_t loads = uint32_t(2 * (share.last - share.first));
+            Pieces pieces(&bars);
             uint32_t n = 0, slot = 0, lap = 0;
-            auto load = [&](Tasks& task, bool hand_back, const CUtensorMap* shared, const CUtensorMap* own) {
-                mbar_expect_tx(&bars.full[slot], S::kSlot);
-                const int key = task.p.key + task.tile() * kKeys;
-#pragma unroll
-                for (int h = 0; h < S::kHalves; ++h) {
-                    const uint32_t dst = smem_u32(slots) + slot * S::kSlot + h * S::kHalf;
-                    if (task.p.prefix()) tma_load_3d(dst, shared, h * 64, key, task.p.head, &bars.full[slot]);
-                    else tma_load_4d(dst, own, h * 64, key, task.p.head, task.p.row, &bars.full[slot]);
-                }
-                task.advance(task.p.both ? 2 : 1, hand_back, &ok, a.error);  // to the next tile
-            };
-            for (; n < loads; ++n) {
+            auto load = [&](const Piece& p, int tile, const CUtensorMap* shared, const CUtensorMap* own) {
                 ok = ok && (lap == 0 || mbar_wait(&bars.empty[slot], (lap - 1) & 1, a.error, 41));
-                if (!ok) break;
-                if (keys.valid() && load_of_k(keys) == n) load(keys, false, &prefix_k, &cache_k);
-                else load(values, true, &prefix_v, &cache_v);
+                if (!ok) return;
+                mbar_expect_tx(&bars.full[slot], S::kSlot);
+#pragma unroll
+                for (int c = 0; c < S::kHalves; ++c) {
+                    const uint32_t dst = smem_u32(slots) + slot * S::kSlot + c * S::kHalf;
+                    const int key = p.key + tile * kKeys;
+                    if (p.prefix) tma_load_3d(dst, shared, c * 64, key, p.head, &bars.full[slot]);
+                    else tma_load_4d(dst, own, c * 64, key, p.head, p.row, &bars.full[slot]);
+                }
+                ++n;
                 if (++slot == S::kSlots) slot = 0, ++lap;
+            };
+            for (;;) {
+                const Piece p = pieces.next(&ok, a.error);
+                if (p.tiles == 0) break;
+                load(p, 0, &prefix_k, &cache_k);
+                for (int tile = 0; tile < p.tiles && ok; ++tile) {
+                    const bool ahead = p.who == kAlternate && tile + 1 < p.tiles;
+                    if (ahead) load(p, tile + 1, &prefix_k, &cache_k);
+                    load(p, tile, &prefix_v, &cache_v);
+                    if (!ahead && tile + 1 < p.tiles) load(p, tile + 1, &prefix_k, &cache_k);
+                }
             }
             if (!ok)  // what is in flight lands before the block leaves
                 for (uint32_t i = n > S::kSlots ? n - S::kSlots : 0; i < n; ++i) mbar_wait(&bars.full[i % S::kSlots], (i / S::kSlots) & 1, a.error, 42);
@@ -461,11 +471,10 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
             constexpr uint32_t kType = H::kDtype == B200Q_BF16 ? 1u : 0u;
             constexpr uint32_t kScores = (1u << 4) | (kType << 7) | (kType << 10) | (uint32_t(kPart >> 3) << 17) | (uint32_t(kRows >> 4) << 24);
             constexpr uint32_t kValues = (1u << 4) | (kType << 7) | (kType << 10) | (1u << 16) | (uint32_t(HD >> 3) << 17) | (uint32_t(kRows >> 4) << 24);
-            const int g = warp - kIssuerWarp, share_tiles = share.last - share.first;
+            const int g = warp - kIssuerWarp;
             const uint32_t s_at = tmem + uint32_t(g) * kKeys, o_at = tmem + 2 * kKeys + uint32_t(g) * HD;
-            Tasks scores(&bars, g, false, &ok, a.error), values(&bars, g, true, &ok, a.error);
-            // Both issuers see every load and every buffer of queries, in order, and hand it back: a waiter
-            // that left one out could not tell a barrier's phase from the one after next.
+            // Both issuers see every load and every buffer of queries, piece by piece in order, and hand it back: a
+            // waiter that left one out could not tell a barrier's phase from the one after next.
             uint32_t loads = 0, queries = 0;  // those handed back
             auto take_load = [&](uint32_t load) {  // waits for it, hands back those before it; its slot
                 for (; ok && loads < load; ++loads) {
@@ -483,20 +492,17 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
                     if (ok) mbar_arrive(&bars.query_empty[queries & 1]);
                 }
             };
+            auto pass_piece = [&](const Piece& p, uint32_t filled) {
+                pass_queries(filled);
+                const uint32_t end = uint32_t(2 * (p.before + p.tiles));
+                if (ok && loads < end) mbar_arrive(&bars.empty[take_load(end - 1)]);
+            };
+            Tasks task(&bars, g, &ok, a.error, pass_piece);
+            const Piece& p = task.p;
+            int ahead = 0;            // the tile whose scores are issued next; one ahead of the tile that is summed
             uint32_t k_slot = 0, k_query = 0;
-            auto parts = [](const Tasks& task) { return task.p.keys - task.tile() * kKeys > kPart ? 2 : 1; };  // halves with any key
-            auto issue_scores = [&](int h) {  // half h of the next tile
-                const Piece& p = scores.p;
-                if (h == 0) {
-                    const uint32_t query = scores.query + (p.both ? uint32_t(scores.t & 1) : 0u);
-                    k_query = query & 1;
-                    if (scores.t < 2) {
-                        pass_queries(query);
-                        ok = ok && mbar_wait(&bars.query_full[k_query], (query >> 1) & 1, a.error, 43);
-                        queries = query + 1;
-                    }
-                    k_slot = take_load(load_of_k(scores));
-                }
+            auto issue_scores = [&](int h) {  // of half h; after its last half, on to the next tile
+                if (h == 0) k_slot = take_load(load_of_k(p, ahead));
                 if (!ok) return;
                 tc_fence_after();
                 const uint64_t qd = smem_desc(smem_u32(smem) + k_query * S::kQuery);
@@ -507,21 +513,30 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
                     umma_f16_ss(s_at + uint32_t(h) * kPart, qd + step, kd + step, kScores, k > 0);
                 }
                 umma_commit(&bars.scores[g][h]);
-                if (h + 1 < parts(scores)) return;
+                if (h == 0 && p.keys - ahead * kKeys > kPart) return;
                 umma_commit(&bars.empty[k_slot]);
-                if (scores.t >= p.tasks() - 2) umma_commit(&bars.query_empty[k_query]);
-                scores.advance(2, false, &ok, a.error);
+                ahead += p.step();
+                if (ahead >= p.tiles) umma_commit(&bars.query_empty[k_query]);
             };
             auto issue_rest = [&](int h) {  // of the next tile, from half h on
-                const int n = parts(scores);
-                for (; h < n && ok; ++h) issue_scores(h);
+                for (const int tile = ahead; ok && ahead == tile; ++h) issue_scores(h);
             };
-            if (scores.valid()) issue_rest(0);
             uint32_t given[2] = {0, 0};
-            while (ok && values.valid()) {
-                const int valid = values.p.keys - values.tile() * kKeys;
-                const uint32_t slot = take_load(load_of_v(values.p, values.tile(), share_tiles));
+            while (ok && task.valid()) {
+                const bool begun = !task.starts();
+                if (!begun) {
+                    const uint32_t query = task.query + (p.who == kBoth ? uint32_t(g) : 0u);
+                    k_query = query & 1;
+                    pass_queries(query);
+                    ok = ok && mbar_wait(&bars.query_full[k_query], (query >> 1) & 1, a.error, 43);
+                    queries = query + 1;
+                    ahead = task.tile;
+                    issue_rest(0);
+                }
+                const int valid = p.keys - task.tile * kKeys;
+                const uint32_t slot = take_load(load_of_v(p, task.tile));
                 const uint64_t vd = value_desc(smem_u32(slots) + slot * S::kSlot, S::kHalf);
+                const int next = task.tile + p.step();
                 int issued = 0;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -532,28 +547,19 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
 #pragma unroll
                     for (int k = 4 * h; k < 4 * h + 4; ++k)
                         if (k == 0 || k * 16 < valid)
-                            umma_f16_ts(o_at, s_at + h * kPart + (k - 4 * h) * 8, vd + uint32_t(k) * (2048 >> 4), kValues, k > 0 || values.t >= 2);
+                            umma_f16_ts(o_at, s_at + h * kPart + (k - 4 * h) * 8, vd + uint32_t(k) * (2048 >> 4), kValues, k > 0 || begun);
                     umma_commit(&bars.summed[g]);
                     // the next tile's first half, unless it would have to be waited for
-                    if (h == 0 && valid > kPart && scores.valid() && scores.t >= 2) {
-                        const uint32_t load = load_of_k(scores);
-                        if (loads == load && mbar_test(&bars.full[load % S::kSlots], (load / S::kSlots) & 1)) {
-                            const bool more = parts(scores) > 1;
-                            issue_scores(0);
-                            issued = more ? 1 : 2;
-                        }
+                    if (h == 0 && next < p.tiles) {
+                        const uint32_t load = load_of_k(p, next);
+                        if (loads == load && mbar_test(&bars.full[load % S::kSlots], (load / S::kSlots) & 1)) issue_scores(0), issued = 1;
                     }
                 }
                 if (!ok) break;
                 umma_commit(&bars.empty[slot]);
-                if (values.t >= values.p.tasks() - 2) umma_commit(&bars.result[g]);
-                values.advance(2, true, &ok, a.error);
-                if (issued < 2 && scores.valid()) issue_rest(issued);
-            }
-            pass_queries(scores.query);
-            if (share_tiles > 0 && ok) {
-                const uint32_t last = uint32_t(2 * share_tiles - 1);
-                if (loads <= last) mbar_arrive(&bars.empty[take_load(last)]);
+                if (task.ends()) umma_commit(&bars.result[g]);
+                if (ahead == next && next < p.tiles) issue_rest(issued);
+                task.advance(&ok, a.error, pass_piece);
             }
         }
         __syncwarp();
@@ -578,9 +584,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
                     begin = max(t, first), end = min(first + share.prefix_tiles, prefix_end);
                     p.head = head, p.row = tile * 2 * a.tile_rows;
                     p.rows = short(min(2 * a.tile_rows, a.batch - p.row));
-                    p.both = p.rows > a.tile_rows;
-                    const int row_next = tile + 1 == a.row_tiles ? 0 : p.row + 2 * a.tile_rows;
-                    p.kind = 1 | (end < prefix_end && a.batch - row_next > a.tile_rows ? 2 : 0);
+                    p.who = p.rows > a.tile_rows ? kBoth : kAlternate, p.prefix = true;
                     p.key = (begin - first) * kKeys, p.keys = share.prefix_keys - p.key;
                     p.place = item + int(blockIdx.x);
                 } else if (t < share.last) {   // a head of the row a lane
@@ -598,7 +602,8 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
                     }
                     const int head = (t - at) / each + lane, first = at + head * each;
                     begin = max(t, first), end = head < a.nkv ? min(first + each, share.last) : begin;
-                    p.head = head, p.row = row, p.rows = 1, p.both = false, p.kind = 0;
+                    // (one group's: the other is done with the piece before meanwhile, or begins the next)
+                    p.head = head, p.row = row, p.rows = 1, p.who = (n + lane) & 1 ? kGroup1 : kGroup0, p.prefix = false;
                     p.key = (begin - first) * kKeys, p.keys = keys - p.key;
                     p.place = row * a.nkv + head + int(blockIdx.x);
                 } else {
@@ -619,16 +624,16 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
             if (lane == 0) mbar_arrive(&bars.list_full[batch & 1]);
             for (int i = 0; i < n && ok; ++i) {
                 const Piece& p = list[i];
-                for (int half = 0; half < (p.both ? 2 : 1); ++half, ++query) {
+                for (int half = 0; half < p.queries(); ++half, ++query) {
                     const uint32_t buffer = query & 1;
                     ok = query < 2 || wait(&bars.query_empty[buffer], ((query >> 1) - 1) & 1, 47);
                     if (!ok) break;
                     if (lane == 0) {
                         // (batch rows past the last one read as zeros; rows of the buffer past the box are never looked at)
-                        mbar_expect_tx(&bars.query_full[buffer], uint32_t(S::kHalves * 128 * a.rep * (p.prefix() ? a.tile_rows : 1)));
+                        mbar_expect_tx(&bars.query_full[buffer], uint32_t(S::kHalves * 128 * a.rep * (p.prefix ? a.tile_rows : 1)));
 #pragma unroll
                         for (int h = 0; h < S::kHalves; ++h)
-                            tma_load_4d(smem_u32(smem) + buffer * S::kQuery + h * (kRows * 128), p.prefix() ? &prefix_q : &own_q, h * 64, 0,
+                            tma_load_4d(smem_u32(smem) + buffer * S::kQuery + h * (kRows * 128), p.prefix ? &prefix_q : &own_q, h * 64, 0,
                                         p.head, p.row + half * a.tile_rows, &bars.query_full[buffer]);
                     }
                     __syncwarp();
@@ -645,31 +650,17 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
         const uint32_t lanes = tmem + (uint32_t(warp & 3) << 21);
         const uint32_t s_at = lanes + uint32_t(g) * kKeys, o_at = lanes + 2 * kKeys + uint32_t(g) * HD;
         Pieces list(&bars);
-        uint32_t first_task = 0, pieces = 0;      // of the piece; pieces that this group has had
+        uint32_t pieces = 0;                      // that this group has had
         uint32_t had = 0, had_first = 0;          // halves of tiles that this group has had, and first halves
-        const int share_tiles = share.last - share.first;
         const float2 scale = make_float2(a.scale_log2, a.scale_log2);
-        // Where both groups take every tile they would run in step, both at their exponentials and then
-        // both at none: they take the exponential unit in turn.
-        uint32_t turns = 0;
-        auto take_turn = [&]() {
-            const uint32_t before = g == 0 ? turns - 1 : turns;  // of the other group's
-            if (g == 1 || turns > 0) ok = ok && wait(&bars.turn[g], before & 1, 54);
-            ++turns;
-        };
-        auto give_turn = [&]() {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bars.turn[g ^ 1]);
-        };
         for (;;) {
             const Piece p = list.next_of_warp(&ok, a.error);
             if (p.tiles == 0) break;
-            // which of the piece's tasks are this group's: every other one, and of both halves of the rows always the same half
-            const int t0 = g ^ int(first_task & 1), live = p.both ? min(a.tile_rows, p.rows - t0 * a.tile_rows) * a.rep : p.rows * a.rep;
+            const int first = p.first(g), step = p.step();
+            if (p.who <= kGroup1 && p.who != g) continue;
+            const int live = p.who == kBoth ? min(a.tile_rows, p.rows - g * a.tile_rows) * a.rep : p.rows * a.rep;
             const bool any = (warp & 3) * 32 < live;  // of this warp's rows
-            first_task += uint32_t(p.tasks());
             float m = 0.0f, l = 0.0f;
-            const int first = p.both ? 0 : t0, step = p.both ? 1 : 2;
             for (int tile = first; tile < p.tiles && ok; tile += step) {
                 const int valid = p.keys - tile * kKeys;  // keys of the tile, and more
 #pragma unroll 1
@@ -720,29 +711,34 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
                             }
                         }
                         const float2 minus = make_float2(-m, -m);
-                        float2 sum[4];
-                        float2 e[kPart / 2];
-                        if (p.both) take_turn();
+                        // Scaled scores run kAhead pairs ahead of the exponentials and the sums as far behind, so that
+                        // the exponential unit, which takes eight clocks an instruction, always has one to do.
+                        constexpr int kPairs = kPart / 2, kAhead = 4;
+                        float2 e[kPairs], sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+                        auto scaled = [&](int i) { e[i] = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), scale, minus); };
+                        auto added = [&](int i) {
+                            sum[i & 1] = add2(sum[i & 1], e[i]);
+                            v[i] = H::pack(e[i].x, e[i].y);
+                        };
 #pragma unroll
-                        for (int i = 0; i < kPart / 2; ++i) e[i] = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), scale, minus);
+                        for (int i = 0; i < kAhead; ++i) scaled(i);
 #pragma unroll
-                        for (int i = 0; i < kPart / 2; ++i) e[i] = make_float2(exp2_approx(e[i].x), exp2_approx(e[i].y));
+                        for (int i = 0; i < kPairs; ++i) {
+                            if (i + kAhead < kPairs) scaled(i + kAhead);
+                            e[i] = make_float2(exp2_approx(e[i].x), exp2_approx(e[i].y));
+                            if (i >= kAhead) added(i - kAhead);
+                        }
 #pragma unroll
-                        for (int i = 0; i < kPart / 2; ++i) sum[i & 3] = i < 4 ? e[i] : add2(sum[i & 3], e[i]);
-#pragma unroll
-                        for (int i = 0; i < kPart / 2; ++i) v[i] = H::pack(e[i].x, e[i].y);
+                        for (int i = kPairs - kAhead; i < kPairs; ++i) added(i);
                         tmem_put_32(at, v);
-                        if (p.both) give_turn();
-                        const float2 pair = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+                        const float2 pair = add2(sum[0], sum[1]);
                         l += pair.x + pair.y;
                         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                    } else if (p.both) {
-                        take_turn(), give_turn();
                     }
                     if (keys < kPart) {
                         // Rows of V past the last key may hold anything, and 0 * NaN is no 0: those that the last
                         // step of 16 keys takes in are cleared (by either group where both use the tile).
-                        const uint32_t load = load_of_v(p, tile, share_tiles), slot = load % S::kSlots;
+                        const uint32_t load = load_of_v(p, tile), slot = load % S::kSlots;
                         ok = ok && wait(&bars.full[slot], (load / S::kSlots) & 1, 49);
                         if (!ok) break;
                         uint8_t* tail = slots + slot * S::kSlot;
@@ -760,9 +756,9 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
             }
             if (!ok) break;
             // ---- the piece's result ----
-            const int span = p.prefix() ? kRows : a.rep;  // rows of a group in the scratch memory
-            float* to = a.scratch + (p.prefix() ? 0 : a.own_at) + (2 * int64_t(p.place) + t0) * group_floats(span, HD);
-            const bool worked = p.both || t0 < p.tiles;
+            const int span = p.prefix ? kRows : a.rep;  // rows of a group in the scratch memory
+            float* to = a.scratch + (p.prefix ? 0 : a.own_at) + (p.prefix ? 2 * int64_t(p.place) + g : int64_t(p.place)) * group_floats(span, HD);
+            const bool worked = first < p.tiles;
             if (worked) {
                 ok = wait(&bars.result[g], pieces & 1, 50);
                 if (!ok) break;
@@ -800,22 +796,25 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
 
 // ---- joining the pieces of a row ----------------------------------------------------------------
 // out = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i in f32 over a row's parts (a piece has one, or
-// one of each group); a row without any key is 0.  One query row a lane and two columns of four
-// numbers a block; the parts are dealt among its warps, four in flight each, since what the kernel
-// waits for is the way to the L2 cache: then the warps' sums meet in shared memory.
-constexpr int kJoinWarps = 8, kJoinColumns = 2, kJoinHeld = 4;
+// one of each group); a row without any key is 0.  One query row a lane.  What the kernel waits for is
+// the way to the L2 cache, so a thread has several parts in flight.  Few parts a row: a block has all
+// columns of its rows, four columns of four numbers a warp.  Many (a long prefix for few rows and heads):
+// the parts are dealt among the warps too, and their sums meet in shared memory.
+constexpr int kJoinWarps = 8, kJoinHeld = 4;
+constexpr int kManyParts = 12;  // more than this many parts of a row are dealt among the warps
 
-template <typename T, int HD>
+template <typename T, int HD, bool MANY>
 __global__ void __launch_bounds__(32 * kJoinWarps)
 prefix_join_kernel(const __grid_constant__ PrefixArgs a, int blocks) {
     using H = Half16<T>;
-    constexpr int kSums = 4 * kJoinColumns;
-    __shared__ float sums[kJoinWarps][kSums + 2][32];  // O, m and l
+    constexpr int kSlices = MANY ? kJoinWarps : 1;     // warps that share a row's parts
+    constexpr int kColumns = MANY ? 2 : HD / 4 / kJoinWarps, kSums = 4 * kColumns;
+    __shared__ float sums[MANY ? kJoinWarps : 1][kSums + 2][32];  // O, m and l
     pdl_launch_dependents();
     pdl_wait();
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int head = blockIdx.y, row = blockIdx.x * 32 + lane;  // row: batch row * rep + head of the group
-    const int column = blockIdx.z * kJoinColumns;
+    const int slice = MANY ? warp : 0, column = (MANY ? int(blockIdx.z) : warp) * kColumns;
     const bool live = row < a.batch * a.rep;
     const int b = live ? row / a.rep : 0, r = row - b * a.rep;
     auto word = [&](int i) { return int(ld_mutable(reinterpret_cast<const uint32_t*>(a.cum) + i)); };
@@ -840,18 +839,18 @@ prefix_join_kernel(const __grid_constant__ PrefixArgs a, int blocks) {
     if (live && each > 0) {
         const int first = a.items * prefix_tiles + before * a.nkv + head * each;
         const int from = block_of(first, total, blocks), to = block_of(first + each - 1, total, blocks);
-        own.base = a.scratch + a.own_at + 2 * int64_t(b * a.nkv + head + from) * group_floats(a.rep, HD);
-        own.parts = (to - from + 1) * 2, own.skip = int(group_floats(a.rep, HD));
+        own.base = a.scratch + a.own_at + int64_t(b * a.nkv + head + from) * group_floats(a.rep, HD);
+        own.parts = to - from + 1, own.skip = int(group_floats(a.rep, HD));
         own.span = a.rep, own.at = r;
     }
     const int parts = shared.parts + own.parts;
     float m = -INFINITY, l = 0.0f, o[kSums] = {};
-    for (int k0 = warp; k0 < parts; k0 += kJoinWarps * kJoinHeld) {
+    for (int k0 = slice; k0 < parts; k0 += kSlices * kJoinHeld) {
         float ms[kJoinHeld], ls[kJoinHeld];
-        uint4 os[kJoinHeld][kJoinColumns];
+        uint4 os[kJoinHeld][kColumns];
 #pragma unroll
         for (int u = 0; u < kJoinHeld; ++u) {
-            const int k = k0 + u * kJoinWarps;
+            const int k = k0 + u * kSlices;
             ms[u] = -INFINITY;
             if (k >= parts) continue;
             const Item& it = k < shared.parts ? shared : own;
@@ -859,7 +858,7 @@ prefix_join_kernel(const __grid_constant__ PrefixArgs a, int blocks) {
             ms[u] = ld_mutable(from + HD * it.span + it.at);
             ls[u] = ld_mutable(from + (HD + 1) * it.span + it.at);
 #pragma unroll
-            for (int c = 0; c < kJoinColumns; ++c) os[u][c] = ld_mutable(reinterpret_cast<const uint4*>(from) + (column + c) * it.span + it.at);
+            for (int c = 0; c < kColumns; ++c) os[u][c] = ld_mutable(reinterpret_cast<const uint4*>(from) + (column + c) * it.span + it.at);
         }
         float most = m;
 #pragma unroll
@@ -875,39 +874,45 @@ prefix_join_kernel(const __grid_constant__ PrefixArgs a, int blocks) {
             const float weight = exp2_approx(ms[u] - m);
             l += weight * ls[u];
 #pragma unroll
-            for (int c = 0; c < kJoinColumns; ++c) {
+            for (int c = 0; c < kColumns; ++c) {
                 o[4 * c] += weight * __uint_as_float(os[u][c].x), o[4 * c + 1] += weight * __uint_as_float(os[u][c].y);
                 o[4 * c + 2] += weight * __uint_as_float(os[u][c].z), o[4 * c + 3] += weight * __uint_as_float(os[u][c].w);
             }
         }
     }
+    if (MANY) {
 #pragma unroll
-    for (int i = 0; i < kSums; ++i) sums[warp][i][lane] = o[i];
-    sums[warp][kSums][lane] = m, sums[warp][kSums + 1][lane] = l;
-    __syncthreads();
-    if (warp != 0 || !live) return;
+        for (int i = 0; i < kSums; ++i) sums[slice][i][lane] = o[i];
+        sums[slice][kSums][lane] = m, sums[slice][kSums + 1][lane] = l;
+        __syncthreads();
+        if (warp != 0) return;
 #pragma unroll
-    for (int w = 1; w < kJoinWarps; ++w) m = fmaxf(m, sums[w][kSums][lane]);
-    l = 0.0f;
+        for (int w = 1; w < kSlices; ++w) m = fmaxf(m, sums[w][kSums][lane]);
+        l = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kSums; ++i) o[i] = 0.0f;
+        for (int i = 0; i < kSums; ++i) o[i] = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) {
-        const float theirs = sums[w][kSums][lane], weight = theirs == -INFINITY ? 0.0f : exp2_approx(theirs - m);
-        l += weight * sums[w][kSums + 1][lane];
+        for (int w = 0; w < kSlices; ++w) {
+            const float theirs = sums[w][kSums][lane], weight = theirs == -INFINITY ? 0.0f : exp2_approx(theirs - m);
+            l += weight * sums[w][kSums + 1][lane];
 #pragma unroll
-        for (int i = 0; i < kSums; ++i) o[i] += weight * sums[w][i][lane];
+            for (int i = 0; i < kSums; ++i) o[i] += weight * sums[w][i][lane];
+        }
     }
+    if (!live) return;
     const float by = l == 0.0f ? 0.0f : 1.0f / l;
-    uint16_t* to = a.out + (int64_t(b) * a.nq + head * a.rep + r) * HD + column * 4;
-    *reinterpret_cast<uint4*>(to) = make_uint4(H::pack(o[0] * by, o[1] * by), H::pack(o[2] * by, o[3] * by),
-                                               H::pack(o[4] * by, o[5] * by), H::pack(o[6] * by, o[7] * by));
+    uint4* to = reinterpret_cast<uint4*>(a.out + (int64_t(b) * a.nq + head * a.rep + r) * HD + column * 4);
+#pragma unroll
+    for (int i = 0; i < kSums; i += 8)
+        *to++ = make_uint4(H::pack(o[i] * by, o[i + 1] * by), H::pack(o[i + 2] * by, o[i + 3] * by),
+                           H::pack(o[i + 4] * by, o[i + 5] * by), H::pack(o[i + 6] * by, o[i + 7] * by));
 }
 
 // ---- host -----------------------------------------------------------------------------------------
 
 struct PrefixPlan {
     int tile_rows, row_tiles, items, blocks;
+    bool many;                             // parts of a row
     int64_t own_at, cum_at, floats;
 };
 
@@ -919,8 +924,12 @@ PrefixPlan plan_of(int64_t batch, int64_t nkv, int64_t rep, int64_t hd, int64_t 
     p.blocks = sm_count();
     const int64_t tiles = p.items * ((prefix + kKeys - 1) / kKeys) + batch * nkv * ((slots + kKeys - 1) / kKeys);
     if (tiles < p.blocks) p.blocks = tiles < 1 ? 1 : int(tiles);
+    // Parts of a row, were all rows' caches full: blocks an item's tiles are spread over, and a block at either end.
+    const int64_t share = tiles < 1 ? 1 : (tiles + p.blocks - 1) / p.blocks, of_prefix = ((prefix + kKeys - 1) / kKeys + share - 1) / share + 1;
+    const int64_t of_own = ((slots + kKeys - 1) / kKeys + share - 1) / share + 1;
+    p.many = (p.items > 0 ? of_prefix * (batch > p.tile_rows ? 1 : 2) : 0) + of_own > kManyParts;
     p.own_at = (p.items > 0 ? p.items + p.blocks : 0) * 2 * group_floats(kRows, int(hd));
-    p.cum_at = p.own_at + (batch * nkv + p.blocks) * 2 * group_floats(int(rep), int(hd));
+    p.cum_at = p.own_at + (batch * nkv + p.blocks) * group_floats(int(rep), int(hd));
     p.floats = p.cum_at + (batch + 2 + 3) / 4 * 4;
     return p;
 }
@@ -957,7 +966,7 @@ CUresult make_map(EncodeTiled encode, CUtensorMap* map, const void* base, int32_
 }
 
 template <typename T, int HD>
-cudaError_t launch_prefix(const CUtensorMap (&maps)[6], const PrefixArgs& a, int blocks, cudaStream_t stream) {
+cudaError_t launch_prefix(const CUtensorMap (&maps)[6], const PrefixArgs& a, int blocks, bool many, cudaStream_t stream) {
     constexpr size_t kSmem = Shape<HD>::kBytes + sizeof(Barriers) + 1024;
     static_assert(kSmem <= 227 * 1024, "shared memory of a block");
     cudaError_t err = ensure_dynamic_smem(reinterpret_cast<const void*>(prefix_attention_kernel<T, HD>), kSmem);
@@ -965,8 +974,9 @@ cudaError_t launch_prefix(const CUtensorMap (&maps)[6], const PrefixArgs& a, int
     err = launch_overlapped(prefix_attention_kernel<T, HD>, dim3(unsigned(blocks)), dim3(kThreads), kSmem, stream, maps[0],
                             maps[1], maps[2], maps[3], maps[4], maps[5], a);
     if (err != cudaSuccess) return err;
-    const dim3 grid{unsigned((a.batch * a.rep + 31) / 32), unsigned(a.nkv), unsigned(HD / (4 * kJoinColumns))};
-    return launch_overlapped(prefix_join_kernel<T, HD>, grid, dim3(32 * kJoinWarps), 0, stream, a, blocks);
+    const dim3 grid{unsigned((a.batch * a.rep + 31) / 32), unsigned(a.nkv), unsigned(many ? HD / 8 : 1)};
+    return many ? launch_overlapped(prefix_join_kernel<T, HD, true>, grid, dim3(32 * kJoinWarps), 0, stream, a, blocks)
+                : launch_overlapped(prefix_join_kernel<T, HD, false>, grid, dim3(32 * kJoinWarps), 0, stream, a, blocks);
 }
 
 }  // namespace
@@ -1026,8 +1036,8 @@ extern "C" int32_t b200q_prefix_attention(const void* q, const void* prefix_k, c
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t err;
     if (dtype == B200Q_BF16)
-        err = head_dim == 128 ? launch_prefix<__nv_bfloat16, 128>(maps, a, p.blocks, s) : launch_prefix<__nv_bfloat16, 64>(maps, a, p.blocks, s);
+        err = head_dim == 128 ? launch_prefix<__nv_bfloat16, 128>(maps, a, p.blocks, p.many, s) : launch_prefix<__nv_bfloat16, 64>(maps, a, p.blocks, p.many, s);
     else
-        err = head_dim == 128 ? launch_prefix<__half, 128>(maps, a, p.blocks, s) : launch_prefix<__half, 64>(maps, a, p.blocks, s);
+        err = head_dim == 128 ? launch_prefix<__half, 128>(maps, a, p.blocks, p.many, s) : launch_prefix<__half, 64>(maps, a, p.blocks, p.many, s);
     return launch_status("prefix_attention", err);
 }
