@@ -36,20 +36,20 @@ namespace {
 
 using namespace umma;
 
-constexpr int kKeys = 128;                 // of a tile
-constexpr int kPart = 64;                  // keys of one turn of scores, weights and sums: half a tile
+constexpr int kKeys = 64;                  // of a tile
 constexpr int kRows = 128;                 // of a group's products
-constexpr int kProducerWarp = 8, kIssuerWarp = 9, kQueryWarp = 11;  // 9 and 10: an issuer for each group
-constexpr int kThreads = 12 * 32;
+constexpr int kProducerWarp = 8, kIssuerWarp = 10, kListWarp = 12;  // a producer and an issuer for each group
+constexpr int kThreads = 13 * 32;
 constexpr uint32_t kTmemColumns = 512;     // S of both groups, O of both groups
 constexpr float kStale = 8.0f;             // how far (log2) a tile's maximum may exceed the row's before it moves
+constexpr int kOwnStart = 1;               // what an item of own keys costs beside its tiles, in tiles
 
 template <int HD>
 struct Shape {
     static constexpr int kHalves = HD / 64;                    // 128-byte columns of a tile
     static constexpr uint32_t kHalf = kKeys * 128;             // bytes of one
     static constexpr uint32_t kSlot = kHalves * kHalf;         // a tile of K or V
-    static constexpr int kSlots = HD == 128 ? 5 : 10;
+    static constexpr int kSlots = HD == 128 ? 10 : 20;
     static constexpr uint32_t kQuery = kHalves * kRows * 128;  // a group's queries; two of them
     static constexpr uint32_t kBytes = 2 * kQuery + kSlots * kSlot;
 };
@@ -59,10 +59,11 @@ struct PrefixArgs {
     const int64_t* prefix_at;              // its length on the device, or null: `prefix`
     uint16_t* out;
     float* scratch;
-    int* cum;                              // [batch + 1]: tiles of a KV head before row b; then the total, then tiles of an item's prefix
+    int* cum;                              // [batch]: units of a KV head before row b; then their total, then tiles of an item's prefix
     int batch, nq, nkv, rep, prefix, slots;  // slots: of a row's own cache
     int tile_rows;                         // batch rows of a group's products: 128 / rep
     int row_tiles, items;                  // of the prefix: ceil(batch / 2 tile_rows), that times nkv
+    int weight;                            // units of a tile of the prefix
     int64_t own_at;                        // where the scratch memory of own pieces begins, in floats
     float scale_log2;
     int* status;
@@ -74,52 +75,47 @@ struct PrefixArgs {
 __device__ __forceinline__ int own_keys(const PrefixArgs& a, int64_t position) {
     return position < -1 || position >= a.slots ? 0 : int(position) + 1;  // outside the cache: none
 }
-__device__ __forceinline__ int own_tiles(const PrefixArgs& a, int64_t position) {
-    return (own_keys(a, position) + kKeys - 1) / kKeys;
-}
+__device__ __forceinline__ int tiles_of(int keys) { return (keys + kKeys - 1) / kKeys; }
+// Units of one head of a row.
+__device__ __forceinline__ int own_units(int keys) { return keys > 0 ? tiles_of(keys) + kOwnStart : 0; }
 __device__ __forceinline__ int prefix_length(const PrefixArgs& a) {
     if (a.prefix_at == nullptr) return a.prefix;
     const int64_t given = ld_mutable(a.prefix_at);
     return int(given < 0 ? 0 : given > a.prefix ? a.prefix : given);
 }
-// The first tile of block c, and the block that takes tile t, of `total` over `blocks`: no more of
-// them than tiles, so that none between two has nothing.  (total * c / blocks in 32 bits; its inverse
-// from an estimate that is a block off at most.)
-__device__ __forceinline__ int first_tile(int c, int total, int blocks) {
-    if (total <= blocks) return min(c, total);
+// The first unit of block c, and the block that takes unit t, of `total` over `blocks`: no more of them
+// than half the units, so that every block between two of an item's has a tile of it.  (total * c / blocks
+// in 32 bits; its inverse from an estimate that is a block off at most.)
+__device__ __forceinline__ int used_blocks(int total, int blocks) { return max(1, min(total / 2, blocks)); }
+__device__ __forceinline__ int first_unit(int c, int total, int blocks) {
     const int whole = total / blocks;
-    return whole * c + (total - whole * blocks) * c / blocks;
+    return c >= blocks ? total : whole * c + (total - whole * blocks) * c / blocks;
 }
 __device__ __forceinline__ int block_of(int t, int total, int blocks) {
-    if (total <= blocks) return t;
     int c = min(int(float(t) * (float(blocks) / float(total))), blocks - 1);
-    while (first_tile(c, total, blocks) > t) --c;
-    while (first_tile(c + 1, total, blocks) <= t) ++c;
+    while (first_unit(c, total, blocks) > t) --c;
+    while (first_unit(c + 1, total, blocks) <= t) ++c;
     return c;
 }
 
 struct Share {  // of a block; in shared memory
-    int total, first, last;              // tiles
-    int prefix_keys, prefix_tiles, own_first;
-    int own_row, own_row_tile;           // the batch row that holds the first own tile of the share, and its first tile
+    int first, last, own_first;          // units; of the rows' own keys
+    int prefix_keys;
+    int own_row, own_row_unit;           // the batch row that holds the first own unit of the share, and its first unit
 };
 
-// A piece, as the scheduling warp writes it down for the other roles.
-enum Who : unsigned char { kGroup0, kGroup1, kAlternate, kBoth };  // whose the tiles are: one group's, each group's in turn, all both's
+// A piece, as the listing warp writes it down for the other roles.
+enum Who : unsigned char { kGroup0, kGroup1, kBoth, kNobody, kEnd };
+enum Kind : unsigned char { kRowsOfBoth, kHalves, kOwn };  // both groups its rows; its keys halved between them; own keys, one group's
 struct __align__(16) Piece {
     int place;                // item + block: of the scratch memory
     int head, row;            // KV head, first batch row
-    int key, keys, tiles;     // first key, keys to the end of the item, tiles (0: the share is at its end)
-    int before;               // tiles of the share before it
+    int key, keys, tiles;     // first key, keys to the end of the item, tiles
     short rows;               // batch rows
-    unsigned char who;
-    bool prefix;
-    // of a group: its first tile of the piece, and how far on the next one is
-    __device__ __forceinline__ int first(int g) const { return who == kAlternate ? g : who == kBoth || who == g ? 0 : tiles; }
-    __device__ __forceinline__ int step() const { return who == kAlternate ? 2 : 1; }
-    __device__ __forceinline__ int queries() const { return who == kBoth ? 2 : 1; }  // buffers
+    unsigned char who, kind;
+    __device__ __forceinline__ bool of(int g) const { return who == g || who == kBoth; }
 };
-constexpr int kBatch = 16;    // pieces that are written down at a time; there are two such batches
+constexpr int kBatch = 8;     // pieces that are written down at a time; there are two such batches (even: pairs stay together)
 
 // ---- scratch memory: of a piece, per group, O as [D / 4][rows] float4, then m [rows] and l [rows] ----
 
@@ -243,24 +239,26 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {  // 
 }
 
 struct Barriers {
-    uint64_t full[10], empty[10];          // tiles of K and V
-    uint64_t query_full[2], query_empty[2];
-    uint64_t scores[2][2], weights[2][2];  // of the groups' halves of a tile: S is there, P is there
-    uint64_t summed[2], result[2];         // of the groups: P . V of a half is done; O of a piece is complete
-    uint64_t list_full[2], list_empty[2];  // batches of pieces
+    uint64_t full[20], empty[20];              // tiles of K and V that both groups take
+    uint64_t own_full[2][10], own_empty[2][10];    // ... that one takes: half of the slots each
+    uint64_t query_full[2][2], query_empty[2][2];  // of the groups: two buffers
+    uint64_t scores[2][2], weights[2][2];      // of the groups' two buffers: S is there, P is there
+    uint64_t summed[2], result[2];             // of the groups: P . V of a tile is done; O of a piece is complete
+    uint64_t changed;                          // the pieces of one kind are done, those of another begin
+    uint64_t list_full[2], list_empty[2];      // batches of pieces
     Piece list[2 * kBatch];
     Share share;
     uint32_t tmem_base;
-    int warp_tiles[kThreads / 32];
+    int warp_units[kThreads / 32];
 };
-constexpr int kListReaders = 3 + 8;        // producer, issuers, warps of the groups
+constexpr int kListReaders = 4 + 8;            // producers, issuers, warps of the groups
 
 // One role's way through the pieces.  Every batch is waited for and handed back.
 struct Pieces {
     Barriers* bars;
     uint32_t i;               // pieces read
     __device__ __forceinline__ explicit Pieces(Barriers* b) : bars(b), i(0) {}
-    // One thread's: the next piece; one without tiles at the end (or when a wait has expired).
+    // One thread's: the next piece, or the end (also when a wait has expired), after which there is none.
     __device__ __forceinline__ Piece next(bool* ok, int* error) {
         const uint32_t batch = i / kBatch;
         if (i % kBatch == 0) {
@@ -268,7 +266,7 @@ struct Pieces {
             *ok = *ok && mbar_wait(&bars->list_full[batch & 1], (batch >> 1) & 1, error, 51);
         }
         Piece p = bars->list[i % (2 * kBatch)];
-        if (!*ok) p.tiles = 0;
+        if (!*ok) p.who = kEnd;
         ++i;
         return p;
     }
@@ -281,52 +279,30 @@ struct Pieces {
             *ok = *ok && __all_sync(0xFFFFFFFFu, mbar_wait(&bars->list_full[batch & 1], (batch >> 1) & 1, error, 51));
         }
         Piece p = bars->list[i % (2 * kBatch)];
-        if (!*ok) p.tiles = 0;
+        if (!*ok) p.who = kEnd;
         ++i;
         return p;
     }
 };
 
-// A group's tiles, one after the other through the pieces.
-struct Tasks {
-    Pieces pieces;
-    Piece p;
-    int g, tile;
-    uint32_t query;           // query buffers filled before the piece
-    // `leave` is called for every piece that is left behind, the group's or not, with the buffers filled up to its end.
-    template <typename Leave>
-    __device__ __forceinline__ Tasks(Barriers* bars, int group, bool* ok, int* error, Leave leave) : pieces(bars) {
-        g = group, query = 0;
-        p = pieces.next(ok, error);
-        tile = p.first(g);
-        settle(ok, error, leave);
+// What a group's roles count alike: the loads of the two rings, and the pieces of own keys, before the piece at hand.
+struct Counts {
+    uint32_t both, mine, own;
+    __device__ __forceinline__ Counts() : both(0), mine(0), own(0) {}
+    __device__ __forceinline__ uint32_t base(const Piece& p) const { return p.who == kBoth ? both : mine; }
+    __device__ __forceinline__ void pass(const Piece& p, int g) {
+        if (!p.of(g)) return;
+        (p.who == kBoth ? both : mine) += uint32_t(2 * p.tiles);
+        if (p.kind == kOwn && p.tiles > 0) ++own;
     }
-    __device__ __forceinline__ bool valid() const { return p.tiles > 0; }
-    template <typename Leave>
-    __device__ __forceinline__ void settle(bool* ok, int* error, Leave leave) {
-        while (p.tiles > 0 && tile >= p.tiles) {
-            query += p.queries();
-            leave(p, query);
-            p = pieces.next(ok, error);
-            tile = p.first(g);
-        }
-    }
-    template <typename Leave>
-    __device__ __forceinline__ void advance(bool* ok, int* error, Leave leave) {
-        tile += p.step();
-        settle(ok, error, leave);
-    }
-    __device__ __forceinline__ bool starts() const { return tile == p.first(g); }
-    __device__ __forceinline__ bool ends() const { return tile + p.step() >= p.tiles; }
+    // Which buffer the piece's queries are in, and how many times it has been filled before.  Those of up to 64 rows take
+    // half of the memory, so that the next piece's can be there early.
+    __device__ __forceinline__ uint32_t buffer(const Piece& p, int rep) const { return p.kind == kOwn && rep <= 64 ? own & 1 : 0; }
 };
-// K and V of a tile are these loads of the share, in the order in which each group's products want them;
-// where the groups alternate, K of the tile after next comes before V of the next one.
-__device__ __forceinline__ uint32_t load_of_k(const Piece& p, int tile) {
-    return uint32_t(2 * (p.before + tile) - (p.who == kAlternate && tile > 0 ? 1 : 0));
-}
-__device__ __forceinline__ uint32_t load_of_v(const Piece& p, int tile) {
-    return uint32_t(2 * (p.before + tile) + (p.who == kAlternate && tile < p.tiles - 1 ? 2 : 1));
-}
+// K and V of a tile are these loads of the piece, in the order in which the products want them: S of the tile
+// after next comes before P . V of the next one.
+__device__ __forceinline__ uint32_t load_of_k(int tile) { return tile == 0 ? 0u : uint32_t(2 * tile - 1); }
+__device__ __forceinline__ uint32_t load_of_v(int tile, int tiles) { return uint32_t(2 * tile + (tile == tiles - 1 ? 1 : 2)); }
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -347,15 +323,19 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
         if (a.prefix > 0) prefetch_map(&prefix_k), prefetch_map(&prefix_v), prefetch_map(&prefix_q);
         if (a.slots > 0) prefetch_map(&cache_k), prefetch_map(&cache_v), prefetch_map(&own_q);
     }
+    constexpr int kOwnSlots = S::kSlots / 2;
     if (threadIdx.x == 0) {
-        // (empty: the two issuers)
         for (int s = 0; s < S::kSlots; ++s) mbar_init(&bars.full[s], 1), mbar_init(&bars.empty[s], 2);
         for (int g = 0; g < 2; ++g) {
-            mbar_init(&bars.query_full[g], 1), mbar_init(&bars.query_empty[g], 2);
-            for (int h = 0; h < 2; ++h) mbar_init(&bars.scores[g][h], 1), mbar_init(&bars.weights[g][h], 4);
+            for (int s = 0; s < kOwnSlots; ++s) mbar_init(&bars.own_full[g][s], 1), mbar_init(&bars.own_empty[g][s], 1);
+            for (int b = 0; b < 2; ++b) {
+                mbar_init(&bars.query_full[g][b], 1), mbar_init(&bars.query_empty[g][b], 1);
+                mbar_init(&bars.scores[g][b], 1), mbar_init(&bars.weights[g][b], 4);
+            }
             mbar_init(&bars.summed[g], 1), mbar_init(&bars.result[g], 1);
             mbar_init(&bars.list_full[g], 1), mbar_init(&bars.list_empty[g], kListReaders);
         }
+        mbar_init(&bars.changed, 4);  // producers and issuers
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kIssuerWarp) {
@@ -367,15 +347,15 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
     pdl_launch_dependents();
     pdl_wait();
 
-    // ---- this block's share: every thread sums some rows' own tiles ----
+    // ---- this block's share: every thread sums some rows' own units ----
     {
         const int per = (a.batch + kThreads - 1) / kThreads, from = min(int(threadIdx.x) * per, a.batch), to = min(from + per, a.batch);
         int mine = 0;
-        const int keys = prefix_length(a), tiles = (keys + kKeys - 1) / kKeys;
+        const int keys = prefix_length(a);
         for (int b = from; b < to; ++b) {
             const int64_t position = ld_mutable(a.positions + b);
             if (blockIdx.x == 0 && (position < -1 || position >= a.slots)) record_bad_position(a.status, b);
-            mine += own_tiles(a, position);
+            mine += own_units(own_keys(a, position));
         }
         int before = mine;
 #pragma unroll
@@ -383,43 +363,41 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
             const int other = __shfl_up_sync(0xFFFFFFFFu, before, d);
             if (lane >= d) before += other;
         }
-        if (lane == 31) bars.warp_tiles[warp] = before;
+        if (lane == 31) bars.warp_units[warp] = before;
         before -= mine;
         __syncthreads();
         int all = 0;
 #pragma unroll
         for (int w = 0; w < kThreads / 32; ++w) {
-            if (w < warp) before += bars.warp_tiles[w];
-            all += bars.warp_tiles[w];
+            if (w < warp) before += bars.warp_units[w];
+            all += bars.warp_units[w];
         }
-        if (a.prefix_at != nullptr && blockIdx.x == 0 && threadIdx.x == 0) {
-            const int64_t given = ld_mutable(a.prefix_at);
-            if (given < 0 || given > a.prefix) record_bad_position(a.status, 0);
-        }
-        const int own_first = a.items * tiles, total = own_first + all * a.nkv;
-        const int first = first_tile(blockIdx.x, total, gridDim.x), last = first_tile(blockIdx.x + 1, total, gridDim.x);
-        const int look = max(first, own_first);  // the first own tile this block can have
-        if (threadIdx.x == 0) {
-            share.total = total, share.first = first, share.last = last;
-            share.prefix_keys = keys, share.prefix_tiles = tiles, share.own_first = own_first;
-        }
+        const int own_first = a.items * tiles_of(keys) * a.weight, total = own_first + all * a.nkv;
+        const int blocks = used_blocks(total, gridDim.x);
+        const int first = first_unit(blockIdx.x, total, blocks), last = first_unit(blockIdx.x + 1, total, blocks);
+        const int look = max(first, own_first);  // the first own unit this block can have
+        if (threadIdx.x == 0) share.first = first, share.last = last, share.own_first = own_first, share.prefix_keys = keys;
         const int begin = own_first + before * a.nkv, end = begin + mine * a.nkv;
         if (look >= begin && look < end) {
             int row = from, at = begin;
             for (; per > 1; ++row) {  // (one row a thread: it is this one)
-                const int each = own_tiles(a, ld_mutable(a.positions + row));
+                const int each = own_units(own_keys(a, ld_mutable(a.positions + row)));
                 if (look < at + each * a.nkv) break;
                 at += each * a.nkv;
             }
-            share.own_row = row, share.own_row_tile = at;
+            share.own_row = row, share.own_row_unit = at;
         }
         if (blockIdx.x == 0) {  // for the joining kernel
             int c = before;
             for (int b = from; b < to; ++b) {
                 a.cum[b] = c;
-                if (b + 1 < to) c += own_tiles(a, ld_mutable(a.positions + b));
+                if (b + 1 < to) c += own_units(own_keys(a, ld_mutable(a.positions + b)));
             }
-            if (threadIdx.x == 0) a.cum[a.batch] = total, a.cum[a.batch + 1] = tiles;
+            if (threadIdx.x == 0) {
+                a.cum[a.batch] = total, a.cum[a.batch + 1] = tiles_of(keys);
+                const int64_t given = a.prefix_at != nullptr ? ld_mutable(a.prefix_at) : 0;
+                if (given < 0 || given > a.prefix) record_bad_position(a.status, 0);
+            }
         }
     }
     tc_fence_before();
@@ -432,334 +410,384 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
     };
     bool ok = true;
 
-    if (warp == kProducerWarp) {
+    if (warp == kProducerWarp || warp == kProducerWarp + 1) {
+        // ---- group g's queries, and its tiles of K and V (producer 0: those of both, too) ----
         if (lane == 0) {
+            const int g = warp - kProducerWarp;
             Pieces pieces(&bars);
-            uint32_t n = 0, slot = 0, lap = 0;
-            auto load = [&](const Piece& p, int tile, const CUtensorMap* shared, const CUtensorMap* own) {
-                ok = ok && (lap == 0 || mbar_wait(&bars.empty[slot], (lap - 1) & 1, a.error, 41));
-                if (!ok) return;
-                mbar_expect_tx(&bars.full[slot], S::kSlot);
-#pragma unroll
-                for (int c = 0; c < S::kHalves; ++c) {
-                    const uint32_t dst = smem_u32(slots) + slot * S::kSlot + c * S::kHalf;
-                    const int key = p.key + tile * kKeys;
-                    if (p.prefix) tma_load_3d(dst, shared, c * 64, key, p.head, &bars.full[slot]);
-                    else tma_load_4d(dst, own, c * 64, key, p.head, p.row, &bars.full[slot]);
-                }
-                ++n;
-                if (++slot == S::kSlots) slot = 0, ++lap;
-            };
+            Counts counts;
+            uint32_t filled[2] = {0, 0}, changes = 0, slot[2] = {0, 0}, lap[2] = {0, 0};  // rings: of both, of this group
+            int kind = -1;
             for (;;) {
                 const Piece p = pieces.next(&ok, a.error);
-                if (p.tiles == 0) break;
-                load(p, 0, &prefix_k, &cache_k);
-                for (int tile = 0; tile < p.tiles && ok; ++tile) {
-                    const bool ahead = p.who == kAlternate && tile + 1 < p.tiles;
-                    if (ahead) load(p, tile + 1, &prefix_k, &cache_k);
-                    load(p, tile, &prefix_v, &cache_v);
-                    if (!ahead && tile + 1 < p.tiles) load(p, tile + 1, &prefix_k, &cache_k);
+                if (p.who == kEnd) break;
+                if (p.who == kNobody) continue;
+                if (kind >= 0 && p.kind != kind) {  // the memory is divided anew
+                    mbar_arrive(&bars.changed);
+                    ok = ok && mbar_wait(&bars.changed, changes++ & 1, a.error, 40);
+                    if (!ok) break;
                 }
+                kind = p.kind;
+                if (!p.of(g) || p.tiles == 0) {
+                    counts.pass(p, g);
+                    continue;
+                }
+                const uint32_t buffer = counts.buffer(p, a.rep);
+                const uint32_t fills = buffer ? filled[1]++ : filled[0]++;
+                ok = fills == 0 || mbar_wait(&bars.query_empty[g][buffer], (fills - 1) & 1, a.error, 47);
+                if (!ok) break;
+                // (batch rows past the last one read as zeros; rows of the buffer past the box are never looked at)
+                mbar_expect_tx(&bars.query_full[g][buffer], uint32_t(S::kHalves * 128 * a.rep * (p.kind == kOwn ? 1 : a.tile_rows)));
+                const int row = p.row + (p.who == kBoth ? g * a.tile_rows : 0);
+#pragma unroll
+                for (int c = 0; c < S::kHalves; ++c)
+                    tma_load_4d(smem_u32(smem) + g * S::kQuery + c * (kRows * 128) + buffer * (64 * 128), p.kind == kOwn ? &own_q : &prefix_q,
+                                c * 64, 0, p.head, row, &bars.query_full[g][buffer]);
+                if (p.who != kBoth || g == 0) {
+                    const bool both = p.who == kBoth;
+                    uint64_t* const full = both ? bars.full : bars.own_full[g];
+                    uint64_t* const empty = both ? bars.empty : bars.own_empty[g];
+                    const uint32_t ring = both ? S::kSlots : kOwnSlots, memory = smem_u32(slots) + (both ? 0 : g * kOwnSlots * S::kSlot);
+                    uint32_t at = both ? slot[0] : slot[1], round = both ? lap[0] : lap[1];
+                    auto load = [&](int tile, const CUtensorMap* shared, const CUtensorMap* own) {
+                        ok = ok && (round == 0 || mbar_wait(&empty[at], (round - 1) & 1, a.error, 41));
+                        if (!ok) return;
+                        mbar_expect_tx(&full[at], S::kSlot);
+#pragma unroll
+                        for (int c = 0; c < S::kHalves; ++c) {
+                            const uint32_t dst = memory + at * S::kSlot + c * S::kHalf;
+                            const int key = p.key + tile * kKeys;
+                            if (p.kind == kOwn) tma_load_4d(dst, own, c * 64, key, p.head, p.row, &full[at]);
+                            else tma_load_3d(dst, shared, c * 64, key, p.head, &full[at]);
+                        }
+                        if (++at == ring) at = 0, ++round;
+                    };
+                    load(0, &prefix_k, &cache_k);
+                    for (int tile = 0; tile < p.tiles && ok; ++tile) {
+                        if (tile + 1 < p.tiles) load(tile + 1, &prefix_k, &cache_k);
+                        load(tile, &prefix_v, &cache_v);
+                    }
+                    (both ? slot[0] : slot[1]) = at, (both ? lap[0] : lap[1]) = round;
+                }
+                counts.pass(p, g);
             }
-            if (!ok)  // what is in flight lands before the block leaves
-                for (uint32_t i = n > S::kSlots ? n - S::kSlots : 0; i < n; ++i) mbar_wait(&bars.full[i % S::kSlots], (i / S::kSlots) & 1, a.error, 42);
+            if (!ok) {  // what is in flight lands before the block leaves
+                auto land = [&](uint64_t* full, uint32_t ring, uint32_t at, uint32_t round) {
+                    for (uint32_t i = 0; i < ring; ++i)
+                        if (round > 0 || i < at) mbar_wait(&full[i], (i < at ? round : round - 1) & 1, a.error, 42);
+                };
+                if (g == 0) land(bars.full, S::kSlots, slot[0], lap[0]);
+                land(bars.own_full[g], kOwnSlots, slot[1], lap[1]);
+                for (int b = 0; b < 2; ++b)
+                    if (filled[b] > 0) mbar_wait(&bars.query_full[g][b], (filled[b] - 1) & 1, a.error, 42);
+            }
         }
         __syncwarp();
     } else if (warp == kIssuerWarp || warp == kIssuerWarp + 1) {
         // ---- the products of group g, from one thread ----
         if (elect_one()) {
             constexpr uint32_t kType = H::kDtype == B200Q_BF16 ? 1u : 0u;
-            constexpr uint32_t kScores = (1u << 4) | (kType << 7) | (kType << 10) | (uint32_t(kPart >> 3) << 17) | (uint32_t(kRows >> 4) << 24);
+            constexpr uint32_t kScores = (1u << 4) | (kType << 7) | (kType << 10) | (uint32_t(kKeys >> 3) << 17) | (uint32_t(kRows >> 4) << 24);
             constexpr uint32_t kValues = (1u << 4) | (kType << 7) | (kType << 10) | (1u << 16) | (uint32_t(HD >> 3) << 17) | (uint32_t(kRows >> 4) << 24);
             const int g = warp - kIssuerWarp;
-            const uint32_t s_at = tmem + uint32_t(g) * kKeys, o_at = tmem + 2 * kKeys + uint32_t(g) * HD;
-            // Both issuers see every load and every buffer of queries, piece by piece in order, and hand it back: a
-            // waiter that left one out could not tell a barrier's phase from the one after next.
-            uint32_t loads = 0, queries = 0;  // those handed back
-            auto take_load = [&](uint32_t load) {  // waits for it, hands back those before it; its slot
-                for (; ok && loads < load; ++loads) {
-                    ok = mbar_wait(&bars.full[loads % S::kSlots], (loads / S::kSlots) & 1, a.error, 44);
-                    if (ok) mbar_arrive(&bars.empty[loads % S::kSlots]);
-                }
-                const uint32_t slot = load % S::kSlots;
-                ok = ok && mbar_wait(&bars.full[slot], (load / S::kSlots) & 1, a.error, 44);
-                loads = load + 1;
-                return slot;
-            };
-            auto pass_queries = [&](uint32_t before) {
-                for (; ok && queries < before; ++queries) {
-                    ok = mbar_wait(&bars.query_full[queries & 1], (queries >> 1) & 1, a.error, 43);
-                    if (ok) mbar_arrive(&bars.query_empty[queries & 1]);
+            const uint32_t s_at = tmem + uint32_t(g) * 2 * kKeys, o_at = tmem + 4 * kKeys + uint32_t(g) * HD;
+            // A way through the group's tiles: `task` counts them, `epoch` the changes of kind that are behind.
+            struct Way {
+                Pieces pieces;
+                Counts counts;
+                Piece p;
+                int tile, kind;
+                uint32_t task, epoch, fills[2];   // fills: of the query buffers, before the piece
+                bool found;                       // p is the group's
+                __device__ __forceinline__ explicit Way(Barriers* bars) : pieces(bars) {
+                    tile = 0, kind = -1, task = epoch = fills[0] = fills[1] = 0, found = false;
                 }
             };
-            auto pass_piece = [&](const Piece& p, uint32_t filled) {
-                pass_queries(filled);
-                const uint32_t end = uint32_t(2 * (p.before + p.tiles));
-                if (ok && loads < end) mbar_arrive(&bars.empty[take_load(end - 1)]);
+            Way sums(&bars);
+            uint32_t changes = 0;
+            // Whether the piece just read is the group's, or the end; else it is passed.
+            auto taken = [&](Way& w) {
+                w.tile = 0;
+                if (w.p.who == kEnd) return true;
+                if (w.p.who == kNobody) return false;
+                if (w.kind >= 0 && w.p.kind != w.kind) ++w.epoch;
+                w.kind = w.p.kind;
+                if (w.p.of(g) && w.p.tiles > 0) return true;
+                w.counts.pass(w.p, g);
+                return false;
             };
-            Tasks task(&bars, g, &ok, a.error, pass_piece);
-            const Piece& p = task.p;
-            int ahead = 0;            // the tile whose scores are issued next; one ahead of the tile that is summed
-            uint32_t k_slot = 0, k_query = 0;
-            auto issue_scores = [&](int h) {  // of half h; after its last half, on to the next tile
-                if (h == 0) k_slot = take_load(load_of_k(p, ahead));
+            auto next_piece = [&]() {             // of the sums
+                do {
+                    sums.p = sums.pieces.next(&ok, a.error);
+                    sums.found = taken(sums);
+                    for (; changes < sums.epoch; ++changes) {  // the memory of one kind is free (not twice before all know)
+                        if (changes > 0) ok = ok && mbar_wait(&bars.changed, (changes - 1) & 1, a.error, 40);
+                        umma_commit(&bars.changed);
+                    }
+                } while (!sums.found);
+            };
+            next_piece();
+            Way scores = sums;
+            // The scores' next piece, if it is written down already and not two batches on.
+            auto look_on = [&]() {
+                while (!scores.found) {
+                    const uint32_t x = scores.pieces.i, batch = x / kBatch;
+                    if (x % kBatch == 0 && (batch > (sums.pieces.i - 1) / kBatch + 1 || !mbar_test(&bars.list_full[batch & 1], (batch >> 1) & 1))) return;
+                    ++scores.pieces.i;
+                    scores.p = bars.list[x % (2 * kBatch)];
+                    scores.found = taken(scores);
+                }
+            };
+            auto leave_piece = [&](Way& w) {
+                if (w.counts.buffer(w.p, a.rep)) ++w.fills[1];
+                else ++w.fills[0];
+                w.counts.pass(w.p, g);
+            };
+            // The barriers and the slot of a load of the piece at hand.
+            auto arrived = [&](const Way& w, uint32_t load, uint64_t** empty) {
+                const bool both = w.p.who == kBoth;
+                const uint32_t n = w.counts.base(w.p) + load, ring = both ? S::kSlots : kOwnSlots, slot = n % ring;
+                *empty = (both ? bars.empty : bars.own_empty[g]) + slot;
+                ok = ok && mbar_wait((both ? bars.full : bars.own_full[g]) + slot, (n / ring) & 1, a.error, 44);
+                return smem_u32(slots) + ((both ? 0 : g * kOwnSlots) + slot) * S::kSlot;
+            };
+            // Whether the next tile's scores could be issued without a wait.
+            auto ready = [&]() {
+                const Way& w = scores;
+                const bool both = w.p.who == kBoth;
+                const uint32_t buffer = w.counts.buffer(w.p, a.rep), n = w.counts.base(w.p) + load_of_k(w.tile), ring = both ? S::kSlots : kOwnSlots;
+                return (w.tile > 0 || mbar_test(&bars.query_full[g][buffer], (buffer ? w.fills[1] : w.fills[0]) & 1)) &&
+                       mbar_test((both ? bars.full : bars.own_full[g]) + n % ring, (n / ring) & 1);
+            };
+            auto issue_scores = [&]() {
+                const uint32_t buffer = scores.counts.buffer(scores.p, a.rep), b = scores.task & 1;
+                if (scores.tile == 0) ok = ok && mbar_wait(&bars.query_full[g][buffer], (buffer ? scores.fills[1] : scores.fills[0]) & 1, a.error, 43);
+                uint64_t* empty;
+                const uint32_t at = arrived(scores, load_of_k(scores.tile), &empty);
                 if (!ok) return;
                 tc_fence_after();
-                const uint64_t qd = smem_desc(smem_u32(smem) + k_query * S::kQuery);
-                const uint64_t kd = smem_desc(smem_u32(slots) + k_slot * S::kSlot + uint32_t(h) * (kPart * 128));
+                const uint64_t qd = smem_desc(smem_u32(smem) + g * S::kQuery + buffer * (64 * 128)), kd = smem_desc(at);
 #pragma unroll
-                for (int k = 0; k < HD / 16; ++k) {
-                    const uint32_t step = uint32_t(k / 4) * (S::kHalf >> 4) + uint32_t(k % 4) * 2;
-                    umma_f16_ss(s_at + uint32_t(h) * kPart, qd + step, kd + step, kScores, k > 0);
-                }
-                umma_commit(&bars.scores[g][h]);
-                if (h == 0 && p.keys - ahead * kKeys > kPart) return;
-                umma_commit(&bars.empty[k_slot]);
-                ahead += p.step();
-                if (ahead >= p.tiles) umma_commit(&bars.query_empty[k_query]);
+                for (int k = 0; k < HD / 16; ++k)
+                    umma_f16_ss(s_at + b * kKeys, qd + uint32_t(k / 4) * ((kRows * 128) >> 4) + uint32_t(k % 4) * 2,
+                                kd + uint32_t(k / 4) * (S::kHalf >> 4) + uint32_t(k % 4) * 2, kScores, k > 0);
+                umma_commit(&bars.scores[g][b]);
+                umma_commit(empty);
+                ++scores.task;
+                if (++scores.tile < scores.p.tiles) return;
+                umma_commit(&bars.query_empty[g][buffer]);
+                leave_piece(scores);
+                scores.found = false;
+                look_on();
             };
-            auto issue_rest = [&](int h) {  // of the next tile, from half h on
-                for (const int tile = ahead; ok && ahead == tile; ++h) issue_scores(h);
-            };
-            uint32_t given[2] = {0, 0};
-            while (ok && task.valid()) {
-                const bool begun = !task.starts();
-                if (!begun) {
-                    const uint32_t query = task.query + (p.who == kBoth ? uint32_t(g) : 0u);
-                    k_query = query & 1;
-                    pass_queries(query);
-                    ok = ok && mbar_wait(&bars.query_full[k_query], (query >> 1) & 1, a.error, 43);
-                    queries = query + 1;
-                    ahead = task.tile;
-                    issue_rest(0);
+            while (ok && sums.p.who != kEnd) {
+                // Scores two tiles ahead: not beyond a change of kind that the sums have not come to, and the sums do
+                // not wait for keys that are late.
+                if (!scores.found) {
+                    if (scores.task == sums.task) scores = sums;
+                    else look_on();
                 }
-                const int valid = p.keys - task.tile * kKeys;
-                const uint32_t slot = take_load(load_of_v(p, task.tile));
-                const uint64_t vd = value_desc(smem_u32(slots) + slot * S::kSlot, S::kHalf);
-                const int next = task.tile + p.step();
-                int issued = 0;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    if (h * kPart >= valid) break;
-                    ok = ok && mbar_wait(&bars.weights[g][h], given[h]++ & 1, a.error, 45);
-                    if (!ok) break;
-                    tc_fence_after();
-#pragma unroll
-                    for (int k = 4 * h; k < 4 * h + 4; ++k)
-                        if (k == 0 || k * 16 < valid)
-                            umma_f16_ts(o_at, s_at + h * kPart + (k - 4 * h) * 8, vd + uint32_t(k) * (2048 >> 4), kValues, k > 0 || begun);
-                    umma_commit(&bars.summed[g]);
-                    // the next tile's first half, unless it would have to be waited for
-                    if (h == 0 && next < p.tiles) {
-                        const uint32_t load = load_of_k(p, next);
-                        if (loads == load && mbar_test(&bars.full[load % S::kSlots], (load / S::kSlots) & 1)) issue_scores(0), issued = 1;
-                    }
-                }
+                while (ok && scores.found && scores.p.who != kEnd && scores.epoch == sums.epoch && scores.task < sums.task + 2 &&
+                       (scores.task == sums.task || ready()))
+                    issue_scores();
+                const uint32_t b = sums.task & 1;
+                uint64_t* empty;
+                const uint32_t at = arrived(sums, load_of_v(sums.tile, sums.p.tiles), &empty);
+                ok = ok && mbar_wait(&bars.weights[g][b], (sums.task >> 1) & 1, a.error, 45);
                 if (!ok) break;
-                umma_commit(&bars.empty[slot]);
-                if (task.ends()) umma_commit(&bars.result[g]);
-                if (ahead == next && next < p.tiles) issue_rest(issued);
-                task.advance(&ok, a.error, pass_piece);
+                tc_fence_after();
+                const uint64_t vd = value_desc(at, S::kHalf);
+                const int keys = sums.p.keys - sums.tile * kKeys;
+#pragma unroll
+                for (int k = 0; k < kKeys / 16; ++k)
+                    if (k == 0 || k * 16 < keys) umma_f16_ts(o_at, s_at + b * kKeys + k * 8, vd + uint32_t(k) * (2048 >> 4), kValues, k > 0 || sums.tile > 0);
+                umma_commit(empty);
+                umma_commit(&bars.summed[g]);
+                ++sums.task;
+                if (++sums.tile < sums.p.tiles) continue;
+                umma_commit(&bars.result[g]);
+                leave_piece(sums);
+                next_piece();
             }
         }
         __syncwarp();
-    } else if (warp == kQueryWarp) {
-        // ---- the pieces, a batch at a time, and their queries ----
-        int t = share.first, row = share.own_row, at = share.own_row_tile;
+    } else if (warp == kListWarp) {
+        // ---- the pieces, a batch at a time ----
+        int t = share.first, row = share.own_row, at = share.own_row_unit;
         int keys_of = 0, held = -1;            // own keys of rows 32 * held + lane
-        const int prefix_end = min(share.own_first, share.last);
-        uint32_t query = 0;
+        const int prefix_end = min(share.own_first, share.last), prefix_tiles = tiles_of(share.prefix_keys);
+        const int item_units = prefix_tiles * a.weight;
         for (uint32_t batch = 0; ok; ++batch) {
             if (batch >= 2) ok = wait(&bars.list_empty[batch & 1], ((batch >> 1) - 1) & 1, 52);
             if (!ok) break;
             Piece* list = bars.list + (batch & 1) * kBatch;
             int n = 0;
-            bool over = false;
-            while (n < kBatch && !over) {
+            while (n < kBatch && t < share.last) {
                 Piece p;
-                int begin, end;                // tiles of this lane's piece
-                if (t < prefix_end) {          // an item a lane
-                    const int item = t / share.prefix_tiles + lane, head = item / a.row_tiles, tile = item - head * a.row_tiles;
-                    const int first = item * share.prefix_tiles;
-                    begin = max(t, first), end = min(first + share.prefix_tiles, prefix_end);
+                int first_tile, end_tile, count;  // this lane's tiles of its item; lanes that write
+                if (t < prefix_end) {             // two lanes an item: both groups' piece, or a group's half of the keys each
+                    const int item0 = t / item_units, item = item0 + lane / 2, head = item / a.row_tiles, tile = item - head * a.row_tiles;
+                    const int first = item * item_units;
+                    first_tile = (max(t, first) - first + a.weight - 1) / a.weight;
+                    end_tile = (min(first + item_units, prefix_end) - first + a.weight - 1) / a.weight;
                     p.head = head, p.row = tile * 2 * a.tile_rows;
                     p.rows = short(min(2 * a.tile_rows, a.batch - p.row));
-                    p.who = p.rows > a.tile_rows ? kBoth : kAlternate, p.prefix = true;
-                    p.key = (begin - first) * kKeys, p.keys = share.prefix_keys - p.key;
                     p.place = item + int(blockIdx.x);
-                } else if (t < share.last) {   // a head of the row a lane
+                    const bool both = p.rows > a.tile_rows;
+                    p.kind = both ? kRowsOfBoth : kHalves;
+                    p.who = both ? (lane & 1 ? kNobody : kBoth) : (lane & 1 ? kGroup1 : kGroup0);
+                    if (!both) {
+                        const int middle = first_tile + (end_tile - first_tile + 1) / 2;
+                        (lane & 1 ? first_tile : end_tile) = middle;
+                    } else if (end_tile <= first_tile) {
+                        p.who = kNobody;
+                    }
+                    p.key = first_tile * kKeys, p.keys = share.prefix_keys - p.key;
+                    const int items = (prefix_end - item0 * item_units + item_units - 1) / item_units;
+                    count = min(kBatch - n, 2 * items);
+                    t = min(prefix_end, (item0 + count / 2) * item_units);
+                } else {                          // a head of the row a lane; one group's: the other is at the piece before or after
                     int keys, each;
-                    for (;; ++row) {           // (t is before the end of the sequence: some row has it)
+                    for (;; ++row) {              // (t is before the end of the sequence: some row has it)
                         if (row / 32 != held) {
                             held = row / 32;
                             const int r = held * 32 + lane;
                             keys_of = r < a.batch ? own_keys(a, ld_mutable(a.positions + r)) : 0;
                         }
                         keys = __shfl_sync(0xFFFFFFFFu, keys_of, row % 32);
-                        each = (keys + kKeys - 1) / kKeys;
+                        each = own_units(keys);
                         if (t < at + each * a.nkv) break;
                         at += each * a.nkv;
                     }
-                    const int head = (t - at) / each + lane, first = at + head * each;
-                    begin = max(t, first), end = head < a.nkv ? min(first + each, share.last) : begin;
-                    // (one group's: the other is done with the piece before meanwhile, or begins the next)
-                    p.head = head, p.row = row, p.rows = 1, p.who = (n + lane) & 1 ? kGroup1 : kGroup0, p.prefix = false;
-                    p.key = (begin - first) * kKeys, p.keys = keys - p.key;
+                    const int head0 = (t - at) / each, head = head0 + lane, first = at + head * each;
+                    first_tile = max(0, t - first - kOwnStart), end_tile = min(tiles_of(keys), share.last - first - kOwnStart);
+                    p.head = head, p.row = row, p.rows = 1, p.kind = kOwn;
+                    p.who = end_tile <= first_tile ? kNobody : (n + lane) & 1 ? kGroup1 : kGroup0;
+                    p.key = first_tile * kKeys, p.keys = keys - p.key;
                     p.place = row * a.nkv + head + int(blockIdx.x);
-                } else {
-                    over = true;
-                    begin = end = t;
-                    if (lane == 0) list[n].tiles = 0;
+                    const int left = min(a.nkv - head0, (share.last - (at + head0 * each) + each - 1) / each);
+                    count = min(kBatch - n, left);
+                    t = min(share.last, at + (head0 + count) * each);
                 }
-                const bool there = begin < end && n + lane < kBatch;
-                const int count = __popc(__ballot_sync(0xFFFFFFFFu, there));
-                if (there) {
-                    p.tiles = end - begin, p.before = begin - share.first;
-                    list[n + lane] = p;
-                }
-                if (count > 0) t = __shfl_sync(0xFFFFFFFFu, end, count - 1);
+                p.tiles = max(0, end_tile - first_tile);
+                if (lane < count) list[n + lane] = p;
                 n += count;
             }
+            const bool over = n < kBatch;
+            if (over && lane == 0) list[n].who = kEnd;
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars.list_full[batch & 1]);
-            for (int i = 0; i < n && ok; ++i) {
-                const Piece& p = list[i];
-                for (int half = 0; half < p.queries(); ++half, ++query) {
-                    const uint32_t buffer = query & 1;
-                    ok = query < 2 || wait(&bars.query_empty[buffer], ((query >> 1) - 1) & 1, 47);
-                    if (!ok) break;
-                    if (lane == 0) {
-                        // (batch rows past the last one read as zeros; rows of the buffer past the box are never looked at)
-                        mbar_expect_tx(&bars.query_full[buffer], uint32_t(S::kHalves * 128 * a.rep * (p.prefix ? a.tile_rows : 1)));
-#pragma unroll
-                        for (int h = 0; h < S::kHalves; ++h)
-                            tma_load_4d(smem_u32(smem) + buffer * S::kQuery + h * (kRows * 128), p.prefix ? &prefix_q : &own_q, h * 64, 0,
-                                        p.head, p.row + half * a.tile_rows, &bars.query_full[buffer]);
-                    }
-                    __syncwarp();
-                }
-            }
             if (over) break;
         }
-        if (!ok && lane == 0)
-            for (uint32_t i = query > 2 ? query - 2 : 0; i < query; ++i) mbar_wait(&bars.query_full[i & 1], (i >> 1) & 1, a.error, 42);
-        __syncwarp();
-    } else if (warp < kProducerWarp) {
+    } else {
         // ---- softmax: group g, one query row a thread ----
         const int g = warp / 4, row = threadIdx.x % 128;
         const uint32_t lanes = tmem + (uint32_t(warp & 3) << 21);
-        const uint32_t s_at = lanes + uint32_t(g) * kKeys, o_at = lanes + 2 * kKeys + uint32_t(g) * HD;
+        const uint32_t s_at = lanes + uint32_t(g) * 2 * kKeys, o_at = lanes + 4 * kKeys + uint32_t(g) * HD;
         Pieces list(&bars);
-        uint32_t pieces = 0;                      // that this group has had
-        uint32_t had = 0, had_first = 0;          // halves of tiles that this group has had, and first halves
+        Counts counts;
+        uint32_t task = 0, pieces = 0;            // that this group has had
         const float2 scale = make_float2(a.scale_log2, a.scale_log2);
         for (;;) {
             const Piece p = list.next_of_warp(&ok, a.error);
-            if (p.tiles == 0) break;
-            const int first = p.first(g), step = p.step();
-            if (p.who <= kGroup1 && p.who != g) continue;
+            if (p.who == kEnd) break;
+            if (!p.of(g)) continue;
             const int live = p.who == kBoth ? min(a.tile_rows, p.rows - g * a.tile_rows) * a.rep : p.rows * a.rep;
             const bool any = (warp & 3) * 32 < live;  // of this warp's rows
             float m = 0.0f, l = 0.0f;
-            for (int tile = first; tile < p.tiles && ok; tile += step) {
-                const int valid = p.keys - tile * kKeys;  // keys of the tile, and more
-#pragma unroll 1
-                for (int h = 0; h * kPart < min(valid, kKeys); ++h) {
-                    const int keys = valid - h * kPart;   // of this half, and more
-                    const uint32_t at = s_at + uint32_t(h) * kPart;
-                    const uint32_t turn = h == 0 ? had_first++ : had - had_first;
-                    ok = wait(&bars.scores[g][h], turn & 1, 48);
-                    if (!ok) break;
-                    ++had;
-                    tc_fence_after();
-                    if (any) {
-                        // Few warps run here, so every step is written as independent instructions in a row.
-                        uint32_t v[kPart];
-                        tmem_ask_32(v, at), tmem_ask_32(v + 32, at + 32);
-                        tmem_arrived(v), tmem_arrived(v + 32);
-                        if (keys < kPart) {
+            for (int tile = 0; tile < p.tiles && ok; ++tile, ++task) {
+                const int keys = p.keys - tile * kKeys;   // of the tile, and more
+                const uint32_t b = task & 1, at = s_at + b * kKeys;
+                ok = wait(&bars.scores[g][b], (task >> 1) & 1, 48);
+                if (!ok) break;
+                tc_fence_after();
+                if (any) {
+                    uint32_t v[kKeys];
+                    tmem_ask_32(v, at), tmem_ask_32(v + 32, at + 32);
+                    tmem_arrived(v), tmem_arrived(v + 32);
+                    if (keys < kKeys) {
 #pragma unroll
-                            for (int i = 0; i < kPart; ++i) v[i] = i < keys ? v[i] : 0xFF800000u;
-                        }
-                        float most[8];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) most[i] = __uint_as_float(v[i]);
-#pragma unroll
-                        for (int i = 8; i < kPart - 8; i += 16)
-#pragma unroll
-                            for (int k = 0; k < 8; ++k) most[k] = max3(most[k], __uint_as_float(v[i + k]), __uint_as_float(v[i + 8 + k]));
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) most[k] = fmaxf(most[k], __uint_as_float(v[kPart - 8 + k]));
-                        const float here = a.scale_log2 * fmaxf(max3(max3(most[0], most[1], most[2]), most[3], most[4]),
-                                                                max3(most[5], most[6], most[7]));
-                        if (tile == first && h == 0) {
-                            m = here == -INFINITY ? 0.0f : here;
-                        } else if (__any_sync(0xFFFFFFFFu, row < live && here > m + kStale)) {
-                            const float next = here > m + kStale ? here : m, by = exp2_approx(m - next);
-                            m = next;
-                            l *= by;
-                            // (these scores were asked for behind the sums before the last ones)
-                            ok = wait(&bars.summed[g], (had - 2) & 1, 53);
-                            tc_fence_after();
-#pragma unroll 1
-                            for (int c = 0; c < HD; c += 8) {
-                                uint32_t o[8];
-                                tmem_take_8(o, o_at + c);
-#pragma unroll
-                                for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * by);
-                                tmem_put_8(o_at + c, o);
-                            }
-                        }
-                        const float2 minus = make_float2(-m, -m);
-                        // Scaled scores run kAhead pairs ahead of the exponentials and the sums as far behind, so that
-                        // the exponential unit, which takes eight clocks an instruction, always has one to do.
-                        constexpr int kPairs = kPart / 2, kAhead = 4;
-                        float2 e[kPairs], sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-                        auto scaled = [&](int i) { e[i] = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), scale, minus); };
-                        auto added = [&](int i) {
-                            sum[i & 1] = add2(sum[i & 1], e[i]);
-                            v[i] = H::pack(e[i].x, e[i].y);
-                        };
-#pragma unroll
-                        for (int i = 0; i < kAhead; ++i) scaled(i);
-#pragma unroll
-                        for (int i = 0; i < kPairs; ++i) {
-                            if (i + kAhead < kPairs) scaled(i + kAhead);
-                            e[i] = make_float2(exp2_approx(e[i].x), exp2_approx(e[i].y));
-                            if (i >= kAhead) added(i - kAhead);
-                        }
-#pragma unroll
-                        for (int i = kPairs - kAhead; i < kPairs; ++i) added(i);
-                        tmem_put_32(at, v);
-                        const float2 pair = add2(sum[0], sum[1]);
-                        l += pair.x + pair.y;
-                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                        for (int i = 0; i < kKeys; ++i) v[i] = i < keys ? v[i] : 0xFF800000u;
                     }
-                    if (keys < kPart) {
-                        // Rows of V past the last key may hold anything, and 0 * NaN is no 0: those that the last
-                        // step of 16 keys takes in are cleared (by either group where both use the tile).
-                        const uint32_t load = load_of_v(p, tile), slot = load % S::kSlots;
-                        ok = ok && wait(&bars.full[slot], (load / S::kSlots) & 1, 49);
-                        if (!ok) break;
-                        uint8_t* tail = slots + slot * S::kSlot;
-                        const int rows = (16 - valid % 16) % 16;
-                        for (int i = row; i < rows * 8 * S::kHalves; i += 128) {
-                            const int c = S::kHalves == 1 ? 0 : (i >> 3) & 1, r = valid + (i >> 3) / S::kHalves;
-                            *reinterpret_cast<uint4*>(tail + c * S::kHalf + r * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    float most[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) most[i] = __uint_as_float(v[i]);
+#pragma unroll
+                    for (int i = 8; i < kKeys - 8; i += 16)
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) most[k] = max3(most[k], __uint_as_float(v[i + k]), __uint_as_float(v[i + 8 + k]));
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) most[k] = fmaxf(most[k], __uint_as_float(v[kKeys - 8 + k]));
+                    const float here = a.scale_log2 * fmaxf(max3(max3(most[0], most[1], most[2]), most[3], most[4]),
+                                                            max3(most[5], most[6], most[7]));
+                    if (tile == 0) {
+                        m = here == -INFINITY ? 0.0f : here;
+                    } else if (__any_sync(0xFFFFFFFFu, row < live && here > m + kStale)) {
+                        const float next = here > m + kStale ? here : m, by = exp2_approx(m - next);
+                        m = next;
+                        l *= by;
+                        // (these scores were asked for behind the sums before the last ones)
+                        ok = wait(&bars.summed[g], (task - 1) & 1, 53);
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < HD; c += 8) {
+                            uint32_t o[8];
+                            tmem_take_8(o, o_at + c);
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * by);
+                            tmem_put_8(o_at + c, o);
                         }
-                        fence_proxy_async();
                     }
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&bars.weights[g][h]);
+                    // Scaled scores run kAhead pairs ahead of the exponentials and the sums as far behind, so that
+                    // the exponential unit, which takes eight clocks an instruction, always has one to do.
+                    const float2 minus = make_float2(-m, -m);
+                    constexpr int kPairs = kKeys / 2, kAhead = 4;
+                    float2 e[kPairs], sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+                    auto scaled = [&](int i) { e[i] = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), scale, minus); };
+                    auto added = [&](int i) {
+                        sum[i & 1] = add2(sum[i & 1], e[i]);
+                        v[i] = H::pack(e[i].x, e[i].y);
+                    };
+#pragma unroll
+                    for (int i = 0; i < kAhead; ++i) scaled(i);
+#pragma unroll
+                    for (int i = 0; i < kPairs; ++i) {
+                        if (i + kAhead < kPairs) scaled(i + kAhead);
+                        e[i] = make_float2(exp2_approx(e[i].x), exp2_approx(e[i].y));
+                        if (i >= kAhead) added(i - kAhead);
+                    }
+#pragma unroll
+                    for (int i = kPairs - kAhead; i < kPairs; ++i) added(i);
+                    tmem_put_32(at, v);
+                    const float2 pair = add2(sum[0], sum[1]);
+                    l += pair.x + pair.y;
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 }
+                if (keys < kKeys) {
+                    // Rows of V past the last key may hold anything, and 0 * NaN is no 0: those that the last
+                    // step of 16 keys takes in are cleared (by either group where both use the tile).
+                    const bool both = p.who == kBoth;
+                    const uint32_t load = counts.base(p) + load_of_v(tile, p.tiles), ring = both ? S::kSlots : kOwnSlots, slot = load % ring;
+                    ok = ok && wait((both ? bars.full : bars.own_full[g]) + slot, (load / ring) & 1, 49);
+                    if (!ok) break;
+                    uint8_t* tail = slots + ((both ? 0 : g * kOwnSlots) + slot) * S::kSlot;
+                    const int rows = (16 - keys % 16) % 16;
+                    for (int i = row; i < rows * 8 * S::kHalves; i += 128) {
+                        const int c = S::kHalves == 1 ? 0 : (i >> 3) & 1, r = keys + (i >> 3) / S::kHalves;
+                        *reinterpret_cast<uint4*>(tail + c * S::kHalf + r * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    fence_proxy_async();
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars.weights[g][b]);
             }
             if (!ok) break;
+            counts.pass(p, g);
             // ---- the piece's result ----
-            const int span = p.prefix ? kRows : a.rep;  // rows of a group in the scratch memory
-            float* to = a.scratch + (p.prefix ? 0 : a.own_at) + (p.prefix ? 2 * int64_t(p.place) + g : int64_t(p.place)) * group_floats(span, HD);
-            const bool worked = first < p.tiles;
-            if (worked) {
+            const int span = p.kind == kOwn ? a.rep : kRows;  // rows of a group in the scratch memory
+            float* to = a.scratch + (p.kind == kOwn ? a.own_at + p.place * group_floats(a.rep, HD) : (2 * int64_t(p.place) + g) * group_floats(kRows, HD));
+            if (p.tiles > 0) {
                 ok = wait(&bars.result[g], pieces & 1, 50);
                 if (!ok) break;
                 ++pieces;
@@ -779,7 +807,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
                 }
             }
             if (row < live) {
-                to[int64_t(HD) * span + row] = worked ? m : -INFINITY;
+                to[int64_t(HD) * span + row] = p.tiles > 0 ? m : -INFINITY;
                 to[int64_t(HD + 1) * span + row] = l;
             }
         }
@@ -819,7 +847,8 @@ prefix_join_kernel(const __grid_constant__ PrefixArgs a, int blocks) {
     const int b = live ? row / a.rep : 0, r = row - b * a.rep;
     auto word = [&](int i) { return int(ld_mutable(reinterpret_cast<const uint32_t*>(a.cum) + i)); };
     const int total = word(a.batch), prefix_tiles = word(a.batch + 1), before = word(b);
-    const int each = own_tiles(a, ld_mutable(a.positions + b));
+    const int keys = own_keys(a, ld_mutable(a.positions + b));
+    blocks = used_blocks(total, blocks);
 
     struct Item {              // the prefix, and the row's own keys
         const float* base;     // of the first group that has the row, in the first piece
@@ -829,16 +858,16 @@ prefix_join_kernel(const __grid_constant__ PrefixArgs a, int blocks) {
     if (live && prefix_tiles > 0) {
         const int pair = b / (2 * a.tile_rows), within = b - pair * 2 * a.tile_rows;
         const bool both = min(2 * a.tile_rows, a.batch - pair * 2 * a.tile_rows) > a.tile_rows;
-        const int item = head * a.row_tiles + pair, first = item * prefix_tiles;
-        const int from = block_of(first, total, blocks), to = block_of(first + prefix_tiles - 1, total, blocks);
+        const int item = head * a.row_tiles + pair, first = item * prefix_tiles * a.weight;
+        const int from = block_of(first, total, blocks), to = block_of(first + (prefix_tiles - 1) * a.weight, total, blocks);
         const int g = both && within >= a.tile_rows, groups = both ? 1 : 2;
         shared.base = a.scratch + (2 * int64_t(item + from) + g) * group_floats(kRows, HD);
         shared.parts = (to - from + 1) * groups, shared.skip = int(group_floats(kRows, HD)) * (2 / groups);
         shared.span = kRows, shared.at = (within - g * a.tile_rows) * a.rep + r;
     }
-    if (live && each > 0) {
-        const int first = a.items * prefix_tiles + before * a.nkv + head * each;
-        const int from = block_of(first, total, blocks), to = block_of(first + each - 1, total, blocks);
+    if (live && keys > 0) {
+        const int first = a.items * prefix_tiles * a.weight + before * a.nkv + head * own_units(keys) + kOwnStart;
+        const int from = block_of(first, total, blocks), to = block_of(first + tiles_of(keys) - 1, total, blocks);
         own.base = a.scratch + a.own_at + int64_t(b * a.nkv + head + from) * group_floats(a.rep, HD);
         own.parts = to - from + 1, own.skip = int(group_floats(a.rep, HD));
         own.span = a.rep, own.at = r;
@@ -911,7 +940,7 @@ prefix_join_kernel(const __grid_constant__ PrefixArgs a, int blocks) {
 // ---- host -----------------------------------------------------------------------------------------
 
 struct PrefixPlan {
-    int tile_rows, row_tiles, items, blocks;
+    int tile_rows, row_tiles, items, weight, blocks;
     bool many;                             // parts of a row
     int64_t own_at, cum_at, floats;
 };
@@ -921,13 +950,14 @@ PrefixPlan plan_of(int64_t batch, int64_t nkv, int64_t rep, int64_t hd, int64_t 
     p.tile_rows = int(kRows / rep);
     p.row_tiles = prefix > 0 ? int((batch + 2 * p.tile_rows - 1) / (2 * p.tile_rows)) : 0;
     p.items = int(nkv) * p.row_tiles;
+    p.weight = batch > p.tile_rows ? 2 : 1;
     p.blocks = sm_count();
-    const int64_t tiles = p.items * ((prefix + kKeys - 1) / kKeys) + batch * nkv * ((slots + kKeys - 1) / kKeys);
-    if (tiles < p.blocks) p.blocks = tiles < 1 ? 1 : int(tiles);
+    const int64_t of_prefix = (prefix + kKeys - 1) / kKeys, of_own = (slots + kKeys - 1) / kKeys;
+    const int64_t units = p.items * of_prefix * p.weight + batch * nkv * (of_own + kOwnStart);
+    if (units / 2 < p.blocks) p.blocks = units < 2 ? 1 : int(units / 2);
     // Parts of a row, were all rows' caches full: blocks an item's tiles are spread over, and a block at either end.
-    const int64_t share = tiles < 1 ? 1 : (tiles + p.blocks - 1) / p.blocks, of_prefix = ((prefix + kKeys - 1) / kKeys + share - 1) / share + 1;
-    const int64_t of_own = ((slots + kKeys - 1) / kKeys + share - 1) / share + 1;
-    p.many = (p.items > 0 ? of_prefix * (batch > p.tile_rows ? 1 : 2) : 0) + of_own > kManyParts;
+    const int64_t share = units < 1 ? 1 : (units + p.blocks - 1) / p.blocks;
+    p.many = (p.items > 0 ? ((of_prefix * p.weight + share - 1) / share + 1) * (batch > p.tile_rows ? 1 : 2) : 0) + (of_own + share - 1) / share + 1 > kManyParts;
     p.own_at = (p.items > 0 ? p.items + p.blocks : 0) * 2 * group_floats(kRows, int(hd));
     p.cum_at = p.own_at + (batch * nkv + p.blocks) * group_floats(int(rep), int(hd));
     p.floats = p.cum_at + (batch + 2 + 3) / 4 * 4;
@@ -942,9 +972,9 @@ int32_t check_prefix(int64_t batch, int64_t nq, int64_t nkv, int64_t hd, int64_t
     B200Q_REQUIRE(prefix >= 0 && prefix < (int64_t(1) << 30) && slots >= 0 && slots < (int64_t(1) << 30),
                   "prefix_attention: bad length of the prefix or the cache");
     const int64_t row_tiles = batch / (2 * (kRows / (nq / nkv))) + 1;
-    B200Q_REQUIRE(nkv * row_tiles * (prefix / kKeys + 1) + batch * nkv * (slots / kKeys + 1) < (int64_t(1) << 30) &&
+    B200Q_REQUIRE(2 * nkv * row_tiles * (prefix / kKeys + 1) + batch * nkv * (slots / kKeys + 2) < (int64_t(1) << 30) &&
                       batch * nq < (int64_t(1) << 30),
-                  "prefix_attention: more than 2^30 tiles of 128 keys, or rows times heads");
+                  "prefix_attention: more than 2^30 tiles of 64 keys, or rows times heads");
     return B200Q_OK;
 }
 
@@ -1030,7 +1060,7 @@ extern "C" int32_t b200q_prefix_attention(const void* q, const void* prefix_k, c
     a.scratch = static_cast<float*>(scratch), a.cum = static_cast<int*>(scratch) + p.cum_at;
     a.batch = int(batch), a.nq = int(nq), a.nkv = int(nkv), a.rep = int(nq / nkv);
     a.prefix = int(prefix), a.slots = int(max_seq);
-    a.tile_rows = p.tile_rows, a.row_tiles = p.row_tiles, a.items = p.items, a.own_at = p.own_at;
+    a.tile_rows = p.tile_rows, a.row_tiles = p.row_tiles, a.items = p.items, a.weight = p.weight, a.own_at = p.own_at;
     a.scale_log2 = scale * 1.4426950408889634f;
     a.status = decoder_error_word(), a.error = gemm_error_word();
     cudaStream_t s = static_cast<cudaStream_t>(stream);
