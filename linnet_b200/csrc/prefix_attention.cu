@@ -109,11 +109,23 @@ enum Who : unsigned char { kGroup0, kGroup1, kBoth, kNobody, kEnd };
 enum Kind : unsigned char { kRowsOfBoth, kHalves, kOwn };  // both groups its rows; its keys halved between them; own keys, one group's
 struct __align__(16) Piece {
     int place;                // item + block: of the scratch memory
-    int head, row;            // KV head, first batch row
-    int key, keys, tiles;     // first key, keys to the end of the item, tiles
-    short rows;               // batch rows
+    int row, key, keys;       // first batch row, first key, keys to the end of the item
+    int tiles;
+    uint32_t base;            // loads before it in its ring: of both groups, or of its group
+    unsigned short head, rows;    // KV head, batch rows
     unsigned char who, kind;
+    unsigned char epoch;      // changes of kind before it
+    unsigned char query;      // where its queries are, of group 0 in bits 0..2, of group 1 in bits 4..6: see Query
     __device__ __forceinline__ bool of(int g) const { return who == g || who == kBoth; }
+};
+// A group's two buffers of queries: which one, whether it has been filled an odd number of times before, or at all.
+// Queries of up to 64 rows take half of a group's memory, so that the next piece's can be there early.
+struct Query {
+    uint32_t bits;
+    __device__ __forceinline__ Query(const Piece& p, int g) { bits = uint32_t(p.query) >> (4 * g); }
+    __device__ __forceinline__ uint32_t buffer() const { return bits & 1; }
+    __device__ __forceinline__ uint32_t parity() const { return (bits >> 1) & 1; }
+    __device__ __forceinline__ bool first() const { return (bits & 4) == 0; }
 };
 constexpr int kBatch = 8;     // pieces that are written down at a time; there are two such batches (even: pairs stay together)
 
@@ -124,12 +136,6 @@ __host__ __device__ constexpr int64_t group_floats(int rows, int hd) { return (i
 
 // ---- instructions --------------------------------------------------------------------------------
 
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
-        "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
-        : "memory");
-}
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint64_t* bar) {
     asm volatile(
         "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
@@ -238,6 +244,15 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {  // 
     return ok != 0;
 }
 
+// The bounded wait, once in the code for all roles: with its slow path written out at every use the
+// kernel was 80 KB, and its short turns went by the instruction cache.
+__device__ __noinline__ bool mbar_wait_long(uint64_t* bar, uint32_t parity, int* error, int code) {
+    return mbar_wait(bar, parity, error, code);
+}
+__device__ __forceinline__ bool mbar_watch(uint64_t* bar, uint32_t parity, int* error, int code) {
+    return mbar_try_wait(bar, parity) || mbar_wait_long(bar, parity, error, code);
+}
+
 struct Barriers {
     uint64_t full[20], empty[20];              // tiles of K and V that both groups take
     uint64_t own_full[2][10], own_empty[2][10];    // ... that one takes: half of the slots each
@@ -263,7 +278,7 @@ struct Pieces {
         const uint32_t batch = i / kBatch;
         if (i % kBatch == 0) {
             if (batch > 0) mbar_arrive(&bars->list_empty[(batch - 1) & 1]);
-            *ok = *ok && mbar_wait(&bars->list_full[batch & 1], (batch >> 1) & 1, error, 51);
+            *ok = *ok && mbar_watch(&bars->list_full[batch & 1], (batch >> 1) & 1, error, 51);
         }
         Piece p = bars->list[i % (2 * kBatch)];
         if (!*ok) p.who = kEnd;
@@ -276,7 +291,7 @@ struct Pieces {
         if (i % kBatch == 0) {
             __syncwarp();
             if (batch > 0 && threadIdx.x % 32 == 0) mbar_arrive(&bars->list_empty[(batch - 1) & 1]);
-            *ok = *ok && __all_sync(0xFFFFFFFFu, mbar_wait(&bars->list_full[batch & 1], (batch >> 1) & 1, error, 51));
+            *ok = *ok && __all_sync(0xFFFFFFFFu, mbar_watch(&bars->list_full[batch & 1], (batch >> 1) & 1, error, 51));
         }
         Piece p = bars->list[i % (2 * kBatch)];
         if (!*ok) p.who = kEnd;
@@ -285,20 +300,6 @@ struct Pieces {
     }
 };
 
-// What a group's roles count alike: the loads of the two rings, and the pieces of own keys, before the piece at hand.
-struct Counts {
-    uint32_t both, mine, own;
-    __device__ __forceinline__ Counts() : both(0), mine(0), own(0) {}
-    __device__ __forceinline__ uint32_t base(const Piece& p) const { return p.who == kBoth ? both : mine; }
-    __device__ __forceinline__ void pass(const Piece& p, int g) {
-        if (!p.of(g)) return;
-        (p.who == kBoth ? both : mine) += uint32_t(2 * p.tiles);
-        if (p.kind == kOwn && p.tiles > 0) ++own;
-    }
-    // Which buffer the piece's queries are in, and how many times it has been filled before.  Those of up to 64 rows take
-    // half of the memory, so that the next piece's can be there early.
-    __device__ __forceinline__ uint32_t buffer(const Piece& p, int rep) const { return p.kind == kOwn && rep <= 64 ? own & 1 : 0; }
-};
 // K and V of a tile are these loads of the piece, in the order in which the products want them: S of the tile
 // after next comes before P . V of the next one.
 __device__ __forceinline__ uint32_t load_of_k(int tile) { return tile == 0 ? 0u : uint32_t(2 * tile - 1); }
@@ -352,6 +353,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
         const int per = (a.batch + kThreads - 1) / kThreads, from = min(int(threadIdx.x) * per, a.batch), to = min(from + per, a.batch);
         int mine = 0;
         const int keys = prefix_length(a);
+#pragma unroll 1
         for (int b = from; b < to; ++b) {
             const int64_t position = ld_mutable(a.positions + b);
             if (blockIdx.x == 0 && (position < -1 || position >= a.slots)) record_bad_position(a.status, b);
@@ -380,6 +382,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
         const int begin = own_first + before * a.nkv, end = begin + mine * a.nkv;
         if (look >= begin && look < end) {
             int row = from, at = begin;
+#pragma unroll 1
             for (; per > 1; ++row) {  // (one row a thread: it is this one)
                 const int each = own_units(own_keys(a, ld_mutable(a.positions + row)));
                 if (look < at + each * a.nkv) break;
@@ -389,6 +392,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
         }
         if (blockIdx.x == 0) {  // for the joining kernel
             int c = before;
+#pragma unroll 1
             for (int b = from; b < to; ++b) {
                 a.cum[b] = c;
                 if (b + 1 < to) c += own_units(own_keys(a, ld_mutable(a.positions + b)));
@@ -406,7 +410,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&bars.tmem_base);
 
     auto wait = [&](uint64_t* bar, uint32_t parity, int code) {  // of a whole warp; bounded
-        return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, a.error, code));
+        return __all_sync(0xFFFFFFFFu, mbar_watch(bar, parity, a.error, code));
     };
     bool ok = true;
 
@@ -415,71 +419,58 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
         if (lane == 0) {
             const int g = warp - kProducerWarp;
             Pieces pieces(&bars);
-            Counts counts;
-            uint32_t filled[2] = {0, 0}, changes = 0, slot[2] = {0, 0}, lap[2] = {0, 0};  // rings: of both, of this group
-            int kind = -1;
+            uint32_t changes = 0, both_end = 0, own_end = 0;  // loads so far
+            uint32_t filled = 0;                              // query buffers that were ever filled, and the last fills' parities
             for (;;) {
                 const Piece p = pieces.next(&ok, a.error);
                 if (p.who == kEnd) break;
-                if (p.who == kNobody) continue;
-                if (kind >= 0 && p.kind != kind) {  // the memory is divided anew
+                for (; ok && changes != p.epoch; changes = (changes + 1) & 255) {  // the memory is divided anew
                     mbar_arrive(&bars.changed);
-                    ok = ok && mbar_wait(&bars.changed, changes++ & 1, a.error, 40);
-                    if (!ok) break;
+                    ok = mbar_watch(&bars.changed, changes & 1, a.error, 40);
                 }
-                kind = p.kind;
-                if (!p.of(g) || p.tiles == 0) {
-                    counts.pass(p, g);
-                    continue;
-                }
-                const uint32_t buffer = counts.buffer(p, a.rep);
-                const uint32_t fills = buffer ? filled[1]++ : filled[0]++;
-                ok = fills == 0 || mbar_wait(&bars.query_empty[g][buffer], (fills - 1) & 1, a.error, 47);
                 if (!ok) break;
+                if (!p.of(g) || p.tiles == 0) continue;
+                const Query query(p, g);
+                const uint32_t buffer = query.buffer();
+                ok = query.first() || mbar_watch(&bars.query_empty[g][buffer], query.parity() ^ 1, a.error, 47);
+                if (!ok) break;
+                const bool own = p.kind == kOwn, both = p.who == kBoth;
                 // (batch rows past the last one read as zeros; rows of the buffer past the box are never looked at)
-                mbar_expect_tx(&bars.query_full[g][buffer], uint32_t(S::kHalves * 128 * a.rep * (p.kind == kOwn ? 1 : a.tile_rows)));
-                const int row = p.row + (p.who == kBoth ? g * a.tile_rows : 0);
+                mbar_expect_tx(&bars.query_full[g][buffer], uint32_t(S::kHalves * 128 * a.rep * (own ? 1 : a.tile_rows)));
 #pragma unroll
                 for (int c = 0; c < S::kHalves; ++c)
-                    tma_load_4d(smem_u32(smem) + g * S::kQuery + c * (kRows * 128) + buffer * (64 * 128), p.kind == kOwn ? &own_q : &prefix_q,
-                                c * 64, 0, p.head, row, &bars.query_full[g][buffer]);
-                if (p.who != kBoth || g == 0) {
-                    const bool both = p.who == kBoth;
-                    uint64_t* const full = both ? bars.full : bars.own_full[g];
-                    uint64_t* const empty = both ? bars.empty : bars.own_empty[g];
-                    const uint32_t ring = both ? S::kSlots : kOwnSlots, memory = smem_u32(slots) + (both ? 0 : g * kOwnSlots * S::kSlot);
-                    uint32_t at = both ? slot[0] : slot[1], round = both ? lap[0] : lap[1];
-                    auto load = [&](int tile, const CUtensorMap* shared, const CUtensorMap* own) {
-                        ok = ok && (round == 0 || mbar_wait(&empty[at], (round - 1) & 1, a.error, 41));
-                        if (!ok) return;
-                        mbar_expect_tx(&full[at], S::kSlot);
+                    tma_load_4d(smem_u32(smem) + g * S::kQuery + c * (kRows * 128) + buffer * (64 * 128), own ? &own_q : &prefix_q, c * 64, 0,
+                                p.head, p.row + (both && g == 1 ? a.tile_rows : 0), &bars.query_full[g][buffer]);
+                filled = (filled & ~(0x11u << buffer)) | (1u << buffer) | (query.parity() << (4 + buffer));
+                if (both && g == 1) continue;
+                uint64_t* const full = both ? bars.full : bars.own_full[g];
+                uint64_t* const empty = both ? bars.empty : bars.own_empty[g];
+                const uint32_t memory = smem_u32(slots) + (both ? 0 : g * kOwnSlots * S::kSlot), ring = both ? S::kSlots : kOwnSlots;
+                uint32_t slot = p.base % ring, lap = p.base / ring;
+                const int loads = 2 * p.tiles;
+#pragma unroll 1
+                for (int i = 0; i < loads; ++i) {
+                    const bool value = i > 0 && ((i & 1) == 0 || i == loads - 1);
+                    const int tile = i == 0 ? 0 : i == loads - 1 ? p.tiles - 1 : value ? i / 2 - 1 : (i + 1) / 2;
+                    ok = lap == 0 || mbar_watch(&empty[slot], (lap - 1) & 1, a.error, 41);
+                    if (!ok) break;
+                    mbar_expect_tx(&full[slot], S::kSlot);
+                    const CUtensorMap* map = own ? (value ? &cache_v : &cache_k) : value ? &prefix_v : &prefix_k;
 #pragma unroll
-                        for (int c = 0; c < S::kHalves; ++c) {
-                            const uint32_t dst = memory + at * S::kSlot + c * S::kHalf;
-                            const int key = p.key + tile * kKeys;
-                            if (p.kind == kOwn) tma_load_4d(dst, own, c * 64, key, p.head, p.row, &full[at]);
-                            else tma_load_3d(dst, shared, c * 64, key, p.head, &full[at]);
-                        }
-                        if (++at == ring) at = 0, ++round;
-                    };
-                    load(0, &prefix_k, &cache_k);
-                    for (int tile = 0; tile < p.tiles && ok; ++tile) {
-                        if (tile + 1 < p.tiles) load(tile + 1, &prefix_k, &cache_k);
-                        load(tile, &prefix_v, &cache_v);
-                    }
-                    (both ? slot[0] : slot[1]) = at, (both ? lap[0] : lap[1]) = round;
+                    for (int c = 0; c < S::kHalves; ++c)
+                        tma_load_4d(memory + slot * S::kSlot + c * S::kHalf, map, c * 64, p.key + tile * kKeys, p.head, own ? p.row : 0, &full[slot]);
+                    ++(both ? both_end : own_end);
+                    if (++slot == ring) slot = 0, ++lap;
                 }
-                counts.pass(p, g);
+                if (!ok) break;
             }
             if (!ok) {  // what is in flight lands before the block leaves
-                auto land = [&](uint64_t* full, uint32_t ring, uint32_t at, uint32_t round) {
-                    for (uint32_t i = 0; i < ring; ++i)
-                        if (round > 0 || i < at) mbar_wait(&full[i], (i < at ? round : round - 1) & 1, a.error, 42);
-                };
-                if (g == 0) land(bars.full, S::kSlots, slot[0], lap[0]);
-                land(bars.own_full[g], kOwnSlots, slot[1], lap[1]);
+                for (uint32_t i = both_end > S::kSlots ? both_end - S::kSlots : 0; i < both_end; ++i)
+                    mbar_watch(&bars.full[i % S::kSlots], (i / S::kSlots) & 1, a.error, 42);
+                for (uint32_t i = own_end > kOwnSlots ? own_end - kOwnSlots : 0; i < own_end; ++i)
+                    mbar_watch(&bars.own_full[g][i % kOwnSlots], (i / kOwnSlots) & 1, a.error, 42);
                 for (int b = 0; b < 2; ++b)
-                    if (filled[b] > 0) mbar_wait(&bars.query_full[g][b], (filled[b] - 1) & 1, a.error, 42);
+                    if (filled >> b & 1) mbar_watch(&bars.query_full[g][b], filled >> (4 + b) & 1, a.error, 42);
             }
         }
         __syncwarp();
@@ -491,123 +482,93 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
             constexpr uint32_t kValues = (1u << 4) | (kType << 7) | (kType << 10) | (1u << 16) | (uint32_t(HD >> 3) << 17) | (uint32_t(kRows >> 4) << 24);
             const int g = warp - kIssuerWarp;
             const uint32_t s_at = tmem + uint32_t(g) * 2 * kKeys, o_at = tmem + 4 * kKeys + uint32_t(g) * HD;
-            // A way through the group's tiles: `task` counts them, `epoch` the changes of kind that are behind.
-            struct Way {
-                Pieces pieces;
-                Counts counts;
-                Piece p;
-                int tile, kind;
-                uint32_t task, epoch, fills[2];   // fills: of the query buffers, before the piece
-                bool found;                       // p is the group's
-                __device__ __forceinline__ explicit Way(Barriers* bars) : pieces(bars) {
-                    tile = 0, kind = -1, task = epoch = fills[0] = fills[1] = 0, found = false;
-                }
-            };
-            Way sums(&bars);
-            uint32_t changes = 0;
-            // Whether the piece just read is the group's, or the end; else it is passed.
-            auto taken = [&](Way& w) {
-                w.tile = 0;
-                if (w.p.who == kEnd) return true;
-                if (w.p.who == kNobody) return false;
-                if (w.kind >= 0 && w.p.kind != w.kind) ++w.epoch;
-                w.kind = w.p.kind;
-                if (w.p.of(g) && w.p.tiles > 0) return true;
-                w.counts.pass(w.p, g);
-                return false;
-            };
+            // Two ways through the group's tiles: the sums', and the scores' up to two tiles ahead of it.
+            Pieces pieces(&bars);
+            Piece p, q;                           // the sums' and the scores' piece
+            int tile = 0, q_tile = 0;
+            uint32_t task = 0, q_task = 0, q_index = 0, changes = 0;
+            bool found = false;                   // q is the scores' next piece, or the end
+            bool any_change = false;
             auto next_piece = [&]() {             // of the sums
                 do {
-                    sums.p = sums.pieces.next(&ok, a.error);
-                    sums.found = taken(sums);
-                    for (; changes < sums.epoch; ++changes) {  // the memory of one kind is free (not twice before all know)
-                        if (changes > 0) ok = ok && mbar_wait(&bars.changed, (changes - 1) & 1, a.error, 40);
+                    p = pieces.next(&ok, a.error);
+                    if (p.who == kEnd) break;
+                    for (; changes != p.epoch; changes = (changes + 1) & 255) {  // the memory of one kind is free (not twice before all know)
+                        if (any_change) ok = ok && mbar_watch(&bars.changed, (changes - 1) & 1, a.error, 40);
                         umma_commit(&bars.changed);
+                        any_change = true;
                     }
-                } while (!sums.found);
+                } while (!p.of(g) || p.tiles == 0);
+                tile = 0;
+            };
+            // The slot of a load of a piece, and the barriers that go with it.
+            auto slot_of = [&](const Piece& p, uint32_t load, uint64_t** full, uint64_t** empty, uint32_t* parity) {
+                const uint32_t n = p.base + load, ring = p.who == kBoth ? S::kSlots : kOwnSlots, lap = n / ring, slot = n - lap * ring;
+                *full = (p.who == kBoth ? bars.full : bars.own_full[g]) + slot;
+                *empty = (p.who == kBoth ? bars.empty : bars.own_empty[g]) + slot;
+                *parity = lap & 1;
+                return smem_u32(slots) + ((p.who == kBoth ? 0 : g * kOwnSlots) + slot) * S::kSlot;
             };
             next_piece();
-            Way scores = sums;
-            // The scores' next piece, if it is written down already and not two batches on.
-            auto look_on = [&]() {
-                while (!scores.found) {
-                    const uint32_t x = scores.pieces.i, batch = x / kBatch;
-                    if (x % kBatch == 0 && (batch > (sums.pieces.i - 1) / kBatch + 1 || !mbar_test(&bars.list_full[batch & 1], (batch >> 1) & 1))) return;
-                    ++scores.pieces.i;
-                    scores.p = bars.list[x % (2 * kBatch)];
-                    scores.found = taken(scores);
-                }
-            };
-            auto leave_piece = [&](Way& w) {
-                if (w.counts.buffer(w.p, a.rep)) ++w.fills[1];
-                else ++w.fills[0];
-                w.counts.pass(w.p, g);
-            };
-            // The barriers and the slot of a load of the piece at hand.
-            auto arrived = [&](const Way& w, uint32_t load, uint64_t** empty) {
-                const bool both = w.p.who == kBoth;
-                const uint32_t n = w.counts.base(w.p) + load, ring = both ? S::kSlots : kOwnSlots, slot = n % ring;
-                *empty = (both ? bars.empty : bars.own_empty[g]) + slot;
-                ok = ok && mbar_wait((both ? bars.full : bars.own_full[g]) + slot, (n / ring) & 1, a.error, 44);
-                return smem_u32(slots) + ((both ? 0 : g * kOwnSlots) + slot) * S::kSlot;
-            };
-            // Whether the next tile's scores could be issued without a wait.
-            auto ready = [&]() {
-                const Way& w = scores;
-                const bool both = w.p.who == kBoth;
-                const uint32_t buffer = w.counts.buffer(w.p, a.rep), n = w.counts.base(w.p) + load_of_k(w.tile), ring = both ? S::kSlots : kOwnSlots;
-                return (w.tile > 0 || mbar_test(&bars.query_full[g][buffer], (buffer ? w.fills[1] : w.fills[0]) & 1)) &&
-                       mbar_test((both ? bars.full : bars.own_full[g]) + n % ring, (n / ring) & 1);
-            };
-            auto issue_scores = [&]() {
-                const uint32_t buffer = scores.counts.buffer(scores.p, a.rep), b = scores.task & 1;
-                if (scores.tile == 0) ok = ok && mbar_wait(&bars.query_full[g][buffer], (buffer ? scores.fills[1] : scores.fills[0]) & 1, a.error, 43);
-                uint64_t* empty;
-                const uint32_t at = arrived(scores, load_of_k(scores.tile), &empty);
-                if (!ok) return;
-                tc_fence_after();
-                const uint64_t qd = smem_desc(smem_u32(smem) + g * S::kQuery + buffer * (64 * 128)), kd = smem_desc(at);
+            while (ok && p.who != kEnd) {
+                // Scores: not beyond a change of kind that the sums have not come to, nor two batches on, and the sums
+                // do not wait for keys that are late.
+                while (ok && q_task < task + 2) {
+                    if (!found) {
+                        if (q_task == task) {
+                            q = p, q_index = pieces.i, found = true;
+                        } else {
+                            const uint32_t batch = q_index / kBatch;
+                            if (q_index % kBatch == 0 && (batch > (pieces.i - 1) / kBatch + 1 || !mbar_test(&bars.list_full[batch & 1], (batch >> 1) & 1))) break;
+                            q = bars.list[q_index++ % (2 * kBatch)];
+                            found = q.who == kEnd || (q.of(g) && q.tiles > 0);
+                            if (!found) continue;
+                        }
+                        q_tile = 0;
+                    }
+                    if (q.who == kEnd || q.epoch != p.epoch) break;
+                    const Query query(q, g);
+                    uint64_t* const query_full = &bars.query_full[g][query.buffer()];
+                    uint64_t *full, *empty;
+                    uint32_t parity;
+                    const uint32_t at = slot_of(q, load_of_k(q_tile), &full, &empty, &parity);
+                    if (q_task != task && !((q_tile > 0 || mbar_test(query_full, query.parity())) && mbar_test(full, parity))) break;
+                    if (q_tile == 0) ok = mbar_watch(query_full, query.parity(), a.error, 43);
+                    ok = ok && mbar_watch(full, parity, a.error, 44);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t b = q_task & 1;
+                    const uint64_t qd = smem_desc(smem_u32(smem) + g * S::kQuery + query.buffer() * (64 * 128)), kd = smem_desc(at);
 #pragma unroll
-                for (int k = 0; k < HD / 16; ++k)
-                    umma_f16_ss(s_at + b * kKeys, qd + uint32_t(k / 4) * ((kRows * 128) >> 4) + uint32_t(k % 4) * 2,
-                                kd + uint32_t(k / 4) * (S::kHalf >> 4) + uint32_t(k % 4) * 2, kScores, k > 0);
-                umma_commit(&bars.scores[g][b]);
-                umma_commit(empty);
-                ++scores.task;
-                if (++scores.tile < scores.p.tiles) return;
-                umma_commit(&bars.query_empty[g][buffer]);
-                leave_piece(scores);
-                scores.found = false;
-                look_on();
-            };
-            while (ok && sums.p.who != kEnd) {
-                // Scores two tiles ahead: not beyond a change of kind that the sums have not come to, and the sums do
-                // not wait for keys that are late.
-                if (!scores.found) {
-                    if (scores.task == sums.task) scores = sums;
-                    else look_on();
+                    for (int k = 0; k < HD / 16; ++k)
+                        umma_f16_ss(s_at + b * kKeys, qd + uint32_t(k / 4) * ((kRows * 128) >> 4) + uint32_t(k % 4) * 2,
+                                    kd + uint32_t(k / 4) * (S::kHalf >> 4) + uint32_t(k % 4) * 2, kScores, k > 0);
+                    umma_commit(&bars.scores[g][b]);
+                    umma_commit(empty);
+                    ++q_task;
+                    if (++q_tile == q.tiles) {
+                        umma_commit(&bars.query_empty[g][query.buffer()]);
+                        found = false;
+                    }
                 }
-                while (ok && scores.found && scores.p.who != kEnd && scores.epoch == sums.epoch && scores.task < sums.task + 2 &&
-                       (scores.task == sums.task || ready()))
-                    issue_scores();
-                const uint32_t b = sums.task & 1;
-                uint64_t* empty;
-                const uint32_t at = arrived(sums, load_of_v(sums.tile, sums.p.tiles), &empty);
-                ok = ok && mbar_wait(&bars.weights[g][b], (sums.task >> 1) & 1, a.error, 45);
+                uint64_t *full, *empty;
+                uint32_t parity;
+                const uint32_t at = slot_of(p, load_of_v(tile, p.tiles), &full, &empty, &parity), b = task & 1;
+                ok = ok && mbar_watch(full, parity, a.error, 44) && mbar_watch(&bars.weights[g][b], (task >> 1) & 1, a.error, 45);
                 if (!ok) break;
                 tc_fence_after();
                 const uint64_t vd = value_desc(at, S::kHalf);
-                const int keys = sums.p.keys - sums.tile * kKeys;
+                const int keys = p.keys - tile * kKeys;
 #pragma unroll
                 for (int k = 0; k < kKeys / 16; ++k)
-                    if (k == 0 || k * 16 < keys) umma_f16_ts(o_at, s_at + b * kKeys + k * 8, vd + uint32_t(k) * (2048 >> 4), kValues, k > 0 || sums.tile > 0);
+                    if (k == 0 || k * 16 < keys) umma_f16_ts(o_at, s_at + b * kKeys + k * 8, vd + uint32_t(k) * (2048 >> 4), kValues, k > 0 || tile > 0);
                 umma_commit(empty);
                 umma_commit(&bars.summed[g]);
-                ++sums.task;
-                if (++sums.tile < sums.p.tiles) continue;
-                umma_commit(&bars.result[g]);
-                leave_piece(sums);
-                next_piece();
+                ++task;
+                if (++tile == p.tiles) {
+                    umma_commit(&bars.result[g]);
+                    next_piece();
+                }
             }
         }
         __syncwarp();
@@ -617,6 +578,10 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
         int keys_of = 0, held = -1;            // own keys of rows 32 * held + lane
         const int prefix_end = min(share.own_first, share.last), prefix_tiles = tiles_of(share.prefix_keys);
         const int item_units = prefix_tiles * a.weight;
+        uint32_t loads_both = 0, loads_0 = 0, loads_1 = 0;     // before the batch's next piece: loads of the rings,
+        uint32_t fills = 0, own_fills = 0;                     // pieces of the groups (16 bits each): of a prefix, of own keys
+        int kind = -1;
+        uint32_t epoch = 0;
         for (uint32_t batch = 0; ok; ++batch) {
             if (batch >= 2) ok = wait(&bars.list_empty[batch & 1], ((batch >> 1) - 1) & 1, 52);
             if (!ok) break;
@@ -630,8 +595,8 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
                     const int first = item * item_units;
                     first_tile = (max(t, first) - first + a.weight - 1) / a.weight;
                     end_tile = (min(first + item_units, prefix_end) - first + a.weight - 1) / a.weight;
-                    p.head = head, p.row = tile * 2 * a.tile_rows;
-                    p.rows = short(min(2 * a.tile_rows, a.batch - p.row));
+                    p.head = static_cast<unsigned short>(head), p.row = tile * 2 * a.tile_rows;
+                    p.rows = static_cast<unsigned short>(max(0, min(2 * a.tile_rows, a.batch - p.row)));
                     p.place = item + int(blockIdx.x);
                     const bool both = p.rows > a.tile_rows;
                     p.kind = both ? kRowsOfBoth : kHalves;
@@ -661,7 +626,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
                     }
                     const int head0 = (t - at) / each, head = head0 + lane, first = at + head * each;
                     first_tile = max(0, t - first - kOwnStart), end_tile = min(tiles_of(keys), share.last - first - kOwnStart);
-                    p.head = head, p.row = row, p.rows = 1, p.kind = kOwn;
+                    p.head = static_cast<unsigned short>(head), p.row = row, p.rows = 1, p.kind = kOwn;
                     p.who = end_tile <= first_tile ? kNobody : (n + lane) & 1 ? kGroup1 : kGroup0;
                     p.key = first_tile * kKeys, p.keys = keys - p.key;
                     p.place = row * a.nkv + head + int(blockIdx.x);
@@ -670,6 +635,39 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
                     t = min(share.last, at + (head0 + count) * each);
                 }
                 p.tiles = max(0, end_tile - first_tile);
+                // Sums over the pieces before: of the lanes before this one, and of those written before.
+                const bool counts = lane < count && p.tiles > 0 && p.who <= kBoth, own = p.kind == kOwn;
+                const uint32_t n_loads = counts ? 2 * p.tiles : 0, which = !counts ? 0u : p.who == kBoth ? 0x10001u : p.who == kGroup0 ? 1u : 0x10000u;
+                uint32_t sum_both = p.who == kBoth ? n_loads : 0, sum_0 = p.who == kGroup0 ? n_loads : 0, sum_1 = p.who == kGroup1 ? n_loads : 0;
+                uint32_t sum_fills = own ? 0 : which, sum_own = own ? which : 0;
+                const uint32_t mine_both = sum_both, mine_0 = sum_0, mine_1 = sum_1, mine_fills = sum_fills, mine_own = sum_own;
+                auto before = [&](uint32_t& sum, uint32_t mine, uint32_t& total) {  // exclusive over the lanes; adds up the total
+#pragma unroll
+                    for (int d = 1; d < kBatch; d <<= 1) {
+                        const uint32_t other = __shfl_up_sync(0xFFFFFFFFu, sum, d);
+                        if (lane >= d) sum += other;
+                    }
+                    const uint32_t all = __shfl_sync(0xFFFFFFFFu, sum, count - 1);
+                    sum = total + sum - mine;
+                    total += all;
+                };
+                before(sum_both, mine_both, loads_both), before(sum_0, mine_0, loads_0), before(sum_1, mine_1, loads_1);
+                before(sum_fills, mine_fills, fills), before(sum_own, mine_own, own_fills);
+                p.base = p.who == kBoth ? sum_both : p.who == kGroup0 ? sum_0 : sum_1;
+                p.query = 0;
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    const uint32_t f = sum_fills >> (16 * g) & 0xFFFFu, o = sum_own >> (16 * g) & 0xFFFFu;
+                    const uint32_t buffer = own && a.rep <= 64 ? o & 1 : 0, times = buffer ? o / 2 : f + (a.rep <= 64 ? (o + 1) / 2 : o);
+                    p.query |= static_cast<unsigned char>((buffer | (times & 1) << 1 | (times > 0 ? 4 : 0)) << (4 * g));
+                }
+                // a change of kind: against the lane before, and of the first lane against what was written last
+                const int kind_up = __shfl_up_sync(0xFFFFFFFFu, int(p.kind), 1);
+                const bool changes = lane < count && (lane == 0 ? kind >= 0 && p.kind != kind : int(p.kind) != kind_up);
+                const uint32_t change_mask = __ballot_sync(0xFFFFFFFFu, changes);
+                p.epoch = static_cast<unsigned char>(epoch + __popc(change_mask & (0xFFFFFFFFu >> (31 - lane))));
+                epoch += __popc(change_mask);
+                kind = __shfl_sync(0xFFFFFFFFu, int(p.kind), count - 1);
                 if (lane < count) list[n + lane] = p;
                 n += count;
             }
@@ -685,7 +683,6 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
         const uint32_t lanes = tmem + (uint32_t(warp & 3) << 21);
         const uint32_t s_at = lanes + uint32_t(g) * 2 * kKeys, o_at = lanes + 4 * kKeys + uint32_t(g) * HD;
         Pieces list(&bars);
-        Counts counts;
         uint32_t task = 0, pieces = 0;            // that this group has had
         const float2 scale = make_float2(a.scale_log2, a.scale_log2);
         for (;;) {
@@ -767,11 +764,12 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
                     // Rows of V past the last key may hold anything, and 0 * NaN is no 0: those that the last
                     // step of 16 keys takes in are cleared (by either group where both use the tile).
                     const bool both = p.who == kBoth;
-                    const uint32_t load = counts.base(p) + load_of_v(tile, p.tiles), ring = both ? S::kSlots : kOwnSlots, slot = load % ring;
+                    const uint32_t load = p.base + load_of_v(tile, p.tiles), ring = both ? S::kSlots : kOwnSlots, slot = load % ring;
                     ok = ok && wait((both ? bars.full : bars.own_full[g]) + slot, (load / ring) & 1, 49);
                     if (!ok) break;
                     uint8_t* tail = slots + ((both ? 0 : g * kOwnSlots) + slot) * S::kSlot;
                     const int rows = (16 - keys % 16) % 16;
+#pragma unroll 1
                     for (int i = row; i < rows * 8 * S::kHalves; i += 128) {
                         const int c = S::kHalves == 1 ? 0 : (i >> 3) & 1, r = keys + (i >> 3) / S::kHalves;
                         *reinterpret_cast<uint4*>(tail + c * S::kHalf + r * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
@@ -783,7 +781,6 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
                 if (lane == 0) mbar_arrive(&bars.weights[g][b]);
             }
             if (!ok) break;
-            counts.pass(p, g);
             // ---- the piece's result ----
             const int span = p.kind == kOwn ? a.rep : kRows;  // rows of a group in the scratch memory
             float* to = a.scratch + (p.kind == kOwn ? a.own_at + p.place * group_floats(a.rep, HD) : (2 * int64_t(p.place) + g) * group_floats(kRows, HD));
@@ -1044,9 +1041,9 @@ extern "C" int32_t b200q_prefix_attention(const void* q, const void* prefix_k, c
     CUtensorMap maps[6] = {};
     // strides: q (row, head), then (key, head) of the prefix's keys and values, (key, head, row) of the caches'
     for (int v = 0; v < 2; ++v) {
-        const int64_t shared[3] = {head_dim, prefix, nkv}, alone[4] = {head_dim, max_seq, nkv, batch};
+        const int64_t shared[4] = {head_dim, prefix, nkv, 1}, alone[4] = {head_dim, max_seq, nkv, batch};
         CUresult made = CUDA_SUCCESS;
-        if (prefix > 0) made = make_map(encode, &maps[v], v ? prefix_v : prefix_k, dtype, 3, shared, strides + 2 + 2 * v, kKeys, 1);
+        if (prefix > 0) made = make_map(encode, &maps[v], v ? prefix_v : prefix_k, dtype, 4, shared, strides + 2 + 2 * v, kKeys, 1);
         if (made == CUDA_SUCCESS && max_seq > 0)
             made = make_map(encode, &maps[2 + v], v ? cache_v : cache_k, dtype, 4, alone, strides + 6 + 3 * v, kKeys, 1);
         // queries of a KV head: of as many batch rows as a group takes, and of one
