@@ -13,8 +13,9 @@
 // The alternatives cost the pass one reduction a group: its largest logit, kept in shared memory.
 // The `top` first logits, larger ones first and the lower index first among equals, lie in the `top`
 // first groups by (largest logit, index), since each group ahead of an element's own holds an
-// element ahead of it.  So the first block finds a threshold that at most kPicked groups reach, by
-// bisection over the floats' order, reads those groups once more and ranks what exceeds it.
+// element ahead of it.  So the first block finds a threshold that `top` groups reach and not many more
+// (by bisection over the floats' order where the first guess has too many), reads those groups once
+// more and ranks what reaches it.
 #include <cooperative_groups.h>
 
 #include "mma.cuh"
@@ -43,25 +44,6 @@ struct LogprobArgs {
     int* status;
 };
 
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 r;
-    asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2,%3};\nmov.b64 y, {%4,%5};\nadd.rn.f32x2 z, x, y;\nmov.b64 {%0,%1}, z;\n}"
-        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return r;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    float2 r;
-    asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2,%3};\nmov.b64 y, {%4,%5};\nmul.rn.f32x2 z, x, y;\nmov.b64 {%0,%1}, z;\n}"
-        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return r;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 r;
-    asm("{\n.reg .b64 x, y, z, w;\nmov.b64 x, {%2,%3};\nmov.b64 y, {%4,%5};\nmov.b64 z, {%6,%7};\n"
-        "fma.rn.f32x2 w, x, y, z;\nmov.b64 {%0,%1}, w;\n}"
-        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return r;
-}
 __device__ __forceinline__ float exp2_approx(float x) {  // relative error 2^-22; 2^-289 is 0
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -72,6 +54,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either i
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {  // leaves NaN out
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 // The order of floats as unsigned numbers, -0 with 0, NaN with -inf (so that no element is ahead of
 // the largest of its group, which leaves NaN out).
 __device__ __forceinline__ uint32_t order_of(float x) {
@@ -79,6 +66,8 @@ __device__ __forceinline__ uint32_t order_of(float x) {
     const uint32_t bits = __float_as_uint(x + 0.0f);
     return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
+
+__device__ __forceinline__ float of_order(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 
 template <typename T>
 struct Logit;  // E elements a 16-byte piece
@@ -137,7 +126,8 @@ struct Row {
         vocab = a.vocab;
         pieces = (shift + vocab + E - 1) / E;
     }
-    // The elements of piece p; those outside the row read `outside`.
+    __device__ __forceinline__ const uint4* pieces_at() const { return reinterpret_cast<const uint4*>(base - shift); }
+    // The elements of piece p; those outside the row read -inf.
     __device__ __forceinline__ bool whole(int p) const { return p * E >= shift && p * E - shift + E <= vocab; }
     __device__ __forceinline__ uint4 load(int p) const {
         return ld_mutable(reinterpret_cast<const uint4*>(base - shift + int64_t(p) * E));
@@ -154,21 +144,19 @@ struct Row {
 // Adds E logits to a thread's sums; returns the largest.
 template <int E>
 __device__ __forceinline__ float largest(const float (&x)[E]) {
-    float m = x[0];
-#pragma unroll
-    for (int e = 1; e < E; ++e) m = fmaxf(m, x[e]);
-    return m;
+    if constexpr (E == 4) return fmaxf(max3(x[0], x[1], x[2]), x[3]);
+    else return max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), fmaxf(x[6], x[7]));
 }
 template <int E>
 __device__ __forceinline__ void add(const float (&x)[E], float m, float2& l, float2& s) {
     const float2 minus = make_float2(-m, -m), log2e = make_float2(1.4426950408889634f, 1.4426950408889634f);
 #pragma unroll
     for (int e = 0; e < E; e += 2) {
-        float2 d = add2(make_float2(x[e], x[e + 1]), minus);
+        float2 d = __fadd2_rn(make_float2(x[e], x[e + 1]), minus);
         d.x = max_nan(d.x, kNothing), d.y = max_nan(d.y, kNothing);
-        const float2 t = mul2(d, log2e), w = make_float2(exp2_approx(t.x), exp2_approx(t.y));
-        l = add2(l, w);
-        s = fma2(w, d, s);
+        const float2 t = __fmul2_rn(d, log2e), w = make_float2(exp2_approx(t.x), exp2_approx(t.y));
+        l = __fadd2_rn(l, w);
+        s = __ffma2_rn(w, d, s);
     }
 }
 
@@ -182,7 +170,7 @@ token_logprobs_kernel(const __grid_constant__ LogprobArgs a) {
     __shared__ int picked[kPicked];
     __shared__ uint64_t ranked[kRanked];
     __shared__ uint32_t threshold;
-    __shared__ int picked_count, ranked_count, reached;
+    __shared__ int picked_count, ranked_count, reached, in_order;  // in_order: the picked groups are, by index
     pdl_launch_dependents();
     pdl_wait();
     cg::cluster_group cluster = cg::this_cluster();
@@ -195,31 +183,13 @@ token_logprobs_kernel(const __grid_constant__ LogprobArgs a) {
 
     float m = kLowest;
     float2 l = make_float2(0.0f, 0.0f), s = l;
-    for (int g0 = first + warp * kHeld; g0 < last; g0 += kWarps * kHeld) {
-        uint4 held[kHeld];
+    // kHeld pieces a lane; the first group's number, and of how many groups the largest are kept
+    auto take = [&](float (&x)[kHeld][E], int g0, int kept) {
+        float peak[kHeld], most = m;
 #pragma unroll
-        for (int u = 0; u < kHeld; ++u) {
-            const int p = (g0 + u) * 32 + lane;
-            if (g0 + u < last && logits.whole(p)) held[u] = logits.load(p);
-        }
-        float x[kHeld][E], peak[kHeld], most = m;
-#pragma unroll
-        for (int u = 0; u < kHeld; ++u) {
-            const int p = (g0 + u) * 32 + lane;
-            if (g0 + u < last && logits.whole(p)) {
-                Logit<T>::widen(held[u], x[u]);
-            } else if (g0 + u < last && p < logits.pieces) {
-                logits.edge(p, x[u]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < E; ++e) x[u][e] = -INFINITY;
-            }
-            peak[u] = largest(x[u]);
-            most = fmaxf(most, peak[u]);
-        }
-        const float d = m - most, c = exp2_approx(d * 1.4426950408889634f);
-        if (c != 1.0f) {
-            const float by = fmaxf(d, kNothing);
+        for (int u = 0; u < kHeld; ++u) peak[u] = largest(x[u]), most = fmaxf(most, peak[u]);
+        if (most > m) {  // (else all of them are at most m, or NaN, which the sums take in)
+            const float d = m - most, c = exp2_approx(d * 1.4426950408889634f), by = fmaxf(d, kNothing);
             s = make_float2(c * (s.x + by * l.x), c * (s.y + by * l.y));
             l = make_float2(c * l.x, c * l.y);
             m = most;
@@ -231,9 +201,40 @@ token_logprobs_kernel(const __grid_constant__ LogprobArgs a) {
             for (int u = 0; u < kHeld; ++u) {
                 float peak_all;
                 asm volatile("redux.sync.max.f32 %0, %1, 0xFFFFFFFF;" : "=f"(peak_all) : "f"(peak[u]));
-                if (lane == 0 && g0 + u < last) group_max[g0 + u - first] = peak_all;
+                if (lane == u) peak[0] = peak_all;
             }
+            if (lane < kept) group_max[g0 + lane - first] = peak[0];
         }
+    };
+    // Groups without an edge of the row, kHeld at a time; what is left of them, and the edges, after that.
+    const int inner_first = max(first, logits.shift > 0 ? 1 : 0), inner_last = min(last, (logits.shift + logits.vocab) / (32 * E));
+    const int rounds = max(0, inner_last - inner_first) / kHeld;
+    {
+        const uint4* from = logits.pieces_at() + (inner_first + warp * kHeld) * 32 + lane;
+        for (int r = warp; r < rounds; r += kWarps, from += kWarps * kHeld * 32) {
+            uint4 held[kHeld];
+#pragma unroll
+            for (int u = 0; u < kHeld; ++u) held[u] = ld_mutable(from + u * 32);
+            float x[kHeld][E];
+#pragma unroll
+            for (int u = 0; u < kHeld; ++u) Logit<T>::widen(held[u], x[u]);
+            take(x, inner_first + r * kHeld, kHeld);
+        }
+    }
+    // The groups left, one a warp: the first one's edge, the last one's, and those of an unfinished round.
+    const int tail = inner_first + rounds * kHeld, left = (inner_first - first) + (last - tail);
+    for (int i = warp; i < left; i += kWarps) {
+        const int g = i < inner_first - first ? first + i : tail + i - (inner_first - first), p = g * 32 + lane;
+        float x[kHeld][E];
+#pragma unroll
+        for (int u = 0; u < kHeld; ++u)
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[u][e] = -INFINITY;
+        if (p < logits.pieces) {
+            if (logits.whole(p)) Logit<T>::widen(logits.load(p), x[0]);
+            else logits.edge(p, x[0]);
+        }
+        take(x, g, 1);
     }
     Sums mine = {m, l.x + l.y, s.x + s.y};
 #pragma unroll
@@ -243,92 +244,125 @@ token_logprobs_kernel(const __grid_constant__ LogprobArgs a) {
         mine = join(mine, theirs);
     }
     if (lane == 0) warp_sums[warp] = mine;
+    if (threadIdx.x == 0) ranked_count = picked_count = 0;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        mine = warp_sums[0];
-#pragma unroll
-        for (int w = 1; w < kWarps; ++w) mine = join(mine, warp_sums[w]);
-        block_sums = mine;
-        ranked_count = 0;
+    auto join_lanes = [&](int count) {  // the sums of the first `count` lanes (a power of two), in lane 0
+        for (int d = count / 2; d >= 1; d >>= 1) {
+            const Sums theirs = {__shfl_xor_sync(0xFFFFFFFFu, mine.m, d), __shfl_xor_sync(0xFFFFFFFFu, mine.l, d),
+                                 __shfl_xor_sync(0xFFFFFFFFu, mine.s, d)};
+            mine = join(mine, theirs);
+        }
+    };
+    if (warp == kWarps - 1) {
+        mine = warp_sums[lane % kWarps];
+        join_lanes(kWarps);
+        if (lane == 0) block_sums = mine;
     }
-    if (blocks > 1) cluster.sync();  // every block's sums and groups are in its shared memory
-    else __syncthreads();
-
     float* all_max = group_max;
-    if (rank == 0) {
-        if (threadIdx.x == 0) {
-            mine = block_sums;
-            for (int r = 1; r < blocks; ++r) mine = join(mine, *cluster.map_shared_rank(&block_sums, r));
-            const double most = double(mine.m), norm = log(double(mine.l));
-            row_max = most, row_log = norm;
-            const int64_t token = ld_mutable(a.tokens + row);
-            float given = 0.0f;  // none given
-            if (token >= a.vocab) {
-                record_bad_position(a.status, row);
-                given = __int_as_float(0x7FC00000);
-            } else if (token >= 0) {
-                given = float(double(Logit<T>::one(logits.base, token)) - most - norm);
-            }
-            a.logprob[row] = given;
-            a.entropy[row] = float(norm - double(mine.s) / double(mine.l));
+    if (blocks > 1) {
+        cluster.sync();  // every block's sums and groups are in its shared memory
+        if (rank == 0 && warp == kWarps - 1) {
+            mine = *cluster.map_shared_rank(&block_sums, lane % blocks);
+            join_lanes(blocks);
         }
-        if (TOP && blocks > 1) {
+        if (TOP && rank == 0) {
             all_max = group_max + (groups + blocks - 1) / blocks;
-            for (int r = 0; r < blocks; ++r) {
-                const int from = int(int64_t(groups) * r / blocks), to = int(int64_t(groups) * (r + 1) / blocks);
-                const float* theirs = cluster.map_shared_rank(group_max, r);
-                for (int g = from + threadIdx.x; g < to; g += kThreads) all_max[g] = theirs[g - from];
+            for (int g = threadIdx.x; g < groups; g += kThreads) {
+                const int r = int(((int64_t(g) + 1) * blocks - 1) / groups), from = int(int64_t(groups) * r / blocks);
+                all_max[g] = cluster.map_shared_rank(group_max, r)[g - from];
             }
         }
+        cluster.sync();  // the others' shared memory is no longer read
+    } else {
+        __syncthreads();
     }
-    if (blocks > 1) cluster.sync();  // the others' shared memory is no longer read
-    else __syncthreads();
-    if (!TOP || rank != 0) return;
+    if (rank != 0) return;
+    if (threadIdx.x == (kWarps - 1) * 32) {  // (the first warp has the alternatives to look for)
+        const double most = double(mine.m), norm = log(double(mine.l));
+        row_max = most, row_log = norm;
+        const int64_t token = ld_mutable(a.tokens + row);
+        float given = 0.0f;  // none given
+        if (token >= a.vocab) {
+            record_bad_position(a.status, row);
+            given = __int_as_float(0x7FC00000);
+        } else if (token >= 0) {
+            given = float(double(Logit<T>::one(logits.base, token)) - most - norm);
+        }
+        a.logprob[row] = given;
+        a.entropy[row] = float(norm - double(mine.s) / double(mine.l));
+    }
+    if (!TOP) return;
 
-    // ---- the groups that are read again ----
+    // ---- the groups that are read again: those above `low` ----
     const int top = a.top;
     if (warp == 0) {
-        // low: at least min(top, groups) groups reach it; high: fewer do
-        uint32_t least = 0xFFFFFFFFu, most = 0;
-        for (int g = lane; g < groups; g += 32) {
-            const uint32_t k = order_of(all_max[g]);
-            least = min(least, k), most = max(most, k);
+        // Each lane's largest of every 32nd group: the top-th of the lanes' is reached by `top` groups at least,
+        // and seldom by many more.
+        uint32_t best = 0;
+        for (int g = lane; g < groups; g += 32) best = max(best, order_of(all_max[g]));
+        int ahead = 0;
+#pragma unroll
+        for (int other = 0; other < 32; ++other) {
+            const uint32_t theirs = __shfl_sync(0xFFFFFFFFu, best, other);
+            ahead += theirs > best || (theirs == best && other < lane);
         }
-        least = __reduce_min_sync(0xFFFFFFFFu, least), most = __reduce_max_sync(0xFFFFFFFFu, most);
-        uint32_t low = least, high = most + 1;
-        int reach = groups;
-        if (groups <= top) low = 0;
-        while (groups > top && reach > kPicked && high - low > 1) {
-            const uint32_t mid = low + (high - low) / 2;
-            int c = 0;
-            for (int g = lane; g < groups; g += 32) c += order_of(all_max[g]) >= mid;
-            c = __reduce_add_sync(0xFFFFFFFFu, c);
-            if (c >= top) low = mid, reach = c;
-            else high = mid;
+        const uint32_t reached_by_top = __shfl_sync(0xFFFFFFFFu, best, __ffs(__ballot_sync(0xFFFFFFFFu, ahead == top - 1)) - 1);
+        int reach = 0;
+        for (int g = lane; g < groups; g += 32) reach += order_of(all_max[g]) >= reached_by_top;
+        reach = __reduce_add_sync(0xFFFFFFFFu, reach);
+        const bool few = groups >= 32 && reach <= kPicked;
+        if (few) {
+            if (lane == 0) threshold = reached_by_top - 1, in_order = 0;
+        } else {
+            // low: at least min(top, groups) groups reach it; high: fewer do
+            uint32_t least = 0xFFFFFFFFu, most = 0;
+            for (int g = lane; g < groups; g += 32) {
+                const uint32_t k = order_of(all_max[g]);
+                least = min(least, k), most = max(most, k);
+            }
+            least = __reduce_min_sync(0xFFFFFFFFu, least), most = __reduce_max_sync(0xFFFFFFFFu, most);
+            uint32_t low = least, high = most + 1;
+            reach = groups;
+            if (groups <= top) low = 0;
+            while (groups > top && reach > kPicked && high - low > 1) {
+                const uint32_t mid = low + (high - low) / 2;
+                int c = 0;
+                for (int g = lane; g < groups; g += 32) c += order_of(all_max[g]) >= mid;
+                c = __reduce_add_sync(0xFFFFFFFFu, c);
+                if (c >= top) low = mid, reach = c;
+                else high = mid;
+            }
+            // All groups above `low`; of those that just reach it as many as there is room for, the first ones.
+            int above = 0;
+            for (int g = lane; g < groups; g += 32) above += order_of(all_max[g]) > low;
+            above = __reduce_add_sync(0xFFFFFFFFu, above);
+            int room = kPicked - above, n = 0;
+            for (int g0 = 0; g0 < groups; g0 += 32) {
+                const int g = g0 + lane;
+                const uint32_t k = g < groups ? order_of(all_max[g]) : 0;
+                const bool just = g < groups && k == low;
+                const uint32_t ties = __ballot_sync(0xFFFFFFFFu, just);
+                const bool take = (g < groups && k > low) || (just && __popc(ties & ((1u << lane) - 1)) < room);
+                const uint32_t taken = __ballot_sync(0xFFFFFFFFu, take);
+                if (take) picked[n + __popc(taken & ((1u << lane) - 1))] = g;
+                n += __popc(taken);
+                room -= min(room, __popc(ties));
+            }
+            if (lane == 0) picked_count = n, threshold = low, in_order = 1;
         }
-        // All groups above `low`; of those that just reach it as many as there is room for, the first ones.
-        int above = 0;
-        for (int g = lane; g < groups; g += 32) above += order_of(all_max[g]) > low;
-        above = __reduce_add_sync(0xFFFFFFFFu, above);
-        int room = kPicked - above, n = 0;
-        for (int g0 = 0; g0 < groups; g0 += 32) {
-            const int g = g0 + lane;
-            const uint32_t k = g < groups ? order_of(all_max[g]) : 0;
-            const bool just = g < groups && k == low;
-            const uint32_t ties = __ballot_sync(0xFFFFFFFFu, just);
-            const bool take = (g < groups && k > low) || (just && __popc(ties & ((1u << lane) - 1)) < room);
-            const uint32_t taken = __ballot_sync(0xFFFFFFFFu, take);
-            if (take) picked[n + __popc(taken & ((1u << lane) - 1))] = g;
-            n += __popc(taken);
-            room -= min(room, __popc(ties));
-        }
-        if (lane == 0) picked_count = n, threshold = low;
     }
     __syncthreads();
+    if (!in_order) {
+        const uint32_t above = threshold;
+        for (int g = threadIdx.x; g < groups; g += kThreads)
+            if (order_of(all_max[g]) > above) picked[atomicAdd(&picked_count, 1)] = g;
+        __syncthreads();
+    }
 
     // Calls `f(order, element)` for every element of the picked groups; one warp a group.
     const int picks = picked_count;
     auto each = [&](auto f) {
+#pragma unroll 1
         for (int i = warp; i < picks; i += kWarps) {
             const int p = picked[i] * 32 + lane;
             float x[E];
@@ -355,6 +389,16 @@ token_logprobs_kernel(const __grid_constant__ LogprobArgs a) {
     uint32_t low = threshold;
     collect(low);
     if (ranked_count > kRanked) {  // many above a threshold made for groups: bisect over the elements
+        if (!in_order) {           // (ties at the end of that go by index)
+            int mine_at = 0, mine_group = 0;
+            if (int(threadIdx.x) < picks) {
+                mine_group = picked[threadIdx.x];
+                for (int i = 0; i < picks; ++i) mine_at += picked[i] < mine_group;
+            }
+            __syncthreads();
+            if (int(threadIdx.x) < picks) picked[mine_at] = mine_group;
+            __syncthreads();
+        }
         uint32_t high = 0xFFFFFFFFu;
         while (high - low > 1) {
             if (threadIdx.x == 0) reached = 0;
@@ -386,13 +430,13 @@ token_logprobs_kernel(const __grid_constant__ LogprobArgs a) {
         int ahead = 0;
         for (int j = 0; j < above; ++j) ahead += ranked[j] > own;
         if (ahead < top) {
-            const int i = int(~uint32_t(own));
-            emit(ahead, Logit<T>::one(logits.base, i), i);
+            emit(ahead, of_order(uint32_t(own >> 32)), int(~uint32_t(own)));
         }
     }
     // Those that just reach the threshold fill what is left, the lower index first.
     if (above < top && warp == 0) {
         int n = above;
+#pragma unroll 1
         for (int g = 0; g < picks && n < top; ++g) {
             const int p = picked[g] * 32 + lane;
             uint32_t ties = 0;
