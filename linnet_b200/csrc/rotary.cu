@@ -6,17 +6,19 @@
 // is formed in f64 turns and reduced to half a turn before it becomes f32: at position 10^6 an f32
 // angle is off by up to 0.03 radians, this one by 2^-24 of itself.
 //
-// The kernel reads q and k once and writes them once, so it is bound by HBM: with 16-byte pieces a
-// thread has four units (64 bytes read, 64 written a unit pair of pieces) in flight before it needs
-// the cosines.  A block takes a few tokens, all heads, and computes cosine and sine of a token's
-// pairs once for all of its heads; with few tokens the heads of one are divided among blocks too.
+// The kernel reads q and k once and writes them once, so it is bound by HBM.  A block takes a few
+// tokens and computes cosine and sine of a token's pairs once for all of its heads; a thread takes the
+// same pairs (a unit: two 16-byte pieces) of several heads, so that it reads their cosines and sines
+// from shared memory once, and has five heads in flight before it needs them.  (With a unit of any
+// head a thread, reading the cosines took 60 % of the shared memory's time.)  With few tokens the heads
+// of one are divided among blocks too.
 #include "mma.cuh"
 
 namespace b200q {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kHeld = 4;           // units a thread has in flight
+constexpr int kHeld = 5;           // heads a thread has in flight; 1 where a thread has no more, the shorter kernel
 constexpr int kMaxTokens = 16;     // of a block
 constexpr int kMaxTurns = 4096;    // (cos, sin) pairs of a block: 32 KB
 
@@ -31,6 +33,7 @@ struct RotaryArgs {
     int64_t slots;                 // > 0: k and v go to slot `position` of caches that long
     int tokens, nq, nkv, heads;    // heads: all that are written, v's among them
     int pairs, units, turning;     // units of a head: `turning` of them hold pairs, the others are copied
+    int token_threads, step;       // threads of a token; heads they take at a time
     int head_dim, block_tokens, block_heads;
     float factor;
     int* status;
@@ -66,7 +69,7 @@ __device__ __forceinline__ float low(uint32_t w) { return Half16<T>::to_float(w 
 template <typename T>
 __device__ __forceinline__ float high(uint32_t w) { return Half16<T>::to_float(w >> 16); }
 
-template <typename T, bool NEIGHBOURS, int W>
+template <typename T, bool NEIGHBOURS, int W, int HELD>
 __global__ void __launch_bounds__(kThreads)
 rotary_kernel(const __grid_constant__ RotaryArgs a) {
     extern __shared__ float2 turns[];          // [token of the block][pair]
@@ -75,43 +78,43 @@ rotary_kernel(const __grid_constant__ RotaryArgs a) {
     pdl_wait();
     const int token0 = blockIdx.x * a.block_tokens, tokens = min(a.block_tokens, a.tokens - token0);
     const int head0 = blockIdx.y * a.block_heads, heads = min(a.block_heads, a.heads - head0);
-    const int per_token = heads * a.units, total = tokens * per_token;
-
-    struct Where {
-        int token, kind, head, first, second;  // numbers of the unit's two pieces within the head; second < 0: none
+    // Numbers of the unit's two pieces within a head of q or k, and of v; none: < 0.
+    struct Unit {
+        int first, second;
         bool turns;
     };
-    auto locate = [&](int i) {
-        Where u;
-        u.token = i / per_token;
-        const int rest = i - u.token * per_token, h = rest / a.units, unit = rest - h * a.units;
-        const int head = head0 + h;
-        u.kind = head < a.nq ? 0 : head < a.nq + a.nkv ? 1 : 2;
-        u.head = u.kind == 0 ? head : u.kind == 1 ? head - a.nq : head - a.nq - a.nkv;
-        u.turns = u.kind < 2 && unit < a.turning;
-        if (u.turns) {
-            u.first = NEIGHBOURS ? 2 * W * unit : W * unit;
-            u.second = NEIGHBOURS ? 2 * W * unit + W : a.pairs + W * unit;
-        } else {
-            const int past = u.kind < 2 ? 2 * a.pairs + 2 * W * (unit - a.turning) : 2 * W * unit;
-            u.first = past < a.head_dim ? past : -1;
-            u.second = past + W < a.head_dim ? past + W : -1;
-        }
+    auto of_head = [&](int unit) {
+        Unit u;
+        u.turns = unit < a.turning;
+        const int past = 2 * a.pairs + 2 * W * (unit - a.turning);
+        u.first = u.turns ? (NEIGHBOURS ? 2 * W * unit : W * unit) : past < a.head_dim ? past : -1;
+        u.second = u.turns ? (NEIGHBOURS ? 2 * W * unit + W : a.pairs + W * unit) : past + W < a.head_dim ? past + W : -1;
         return u;
     };
-    Piece<W> one[kHeld], two[kHeld];
-    auto load = [&](int base) {
+    auto of_value = [&](int unit) {
+        const int at = 2 * W * unit;
+        return Unit{at < a.head_dim ? at : -1, at + W < a.head_dim ? at + W : -1, false};
+    };
+    const int mine = threadIdx.x / a.token_threads, within = threadIdx.x - mine * a.token_threads;
+    const int lane_head = a.step > 1 ? within / a.units : 0;
+    const bool works = mine < tokens && lane_head < a.step;
+    Piece<W> one[HELD], two[HELD];
+    auto kind_of = [&](int head) { return head < a.nq ? 0 : head < a.nq + a.nkv ? 1 : 2; };
+    auto load = [&](int unit, int h0) {
 #pragma unroll
-        for (int s = 0; s < kHeld; ++s) {
-            const int i = base + s * kThreads;
-            if (i >= total) continue;
-            const Where u = locate(i);
-            const uint16_t* p = a.src[u.kind] + (token0 + u.token) * a.src_token[u.kind] + u.head * a.src_head[u.kind];
+        for (int s = 0; s < HELD; ++s) {
+            const int h = h0 + s * a.step;
+            if (h >= heads) continue;
+            const int head = head0 + h, kind = kind_of(head);
+            const Unit u = kind < 2 ? of_head(unit) : of_value(unit);
+            const uint16_t* p = a.src[kind] + (token0 + mine) * a.src_token[kind] +
+                                (head - (kind > 0 ? a.nq : 0) - (kind > 1 ? a.nkv : 0)) * a.src_head[kind];
             if (u.first >= 0) one[s].load(p + u.first);
             if (u.second >= 0) two[s].load(p + u.second);
         }
     };
-    load(threadIdx.x);
+    const int unit0 = within - lane_head * a.units;
+    if (works && unit0 < a.units) load(unit0, lane_head);
 
     const int64_t offset = a.offset_at != nullptr ? ld_mutable(a.offset_at) : a.offset;
     for (int i = threadIdx.x; i < tokens * a.pairs; i += kThreads) {
@@ -132,47 +135,57 @@ rotary_kernel(const __grid_constant__ RotaryArgs a) {
         at[threadIdx.x] = bad ? -1 : position;
     }
     __syncthreads();
+    if (!works) return;
 
-    for (int base = threadIdx.x; base < total; base += kHeld * kThreads) {
-        if (base != int(threadIdx.x)) load(base);
+    for (int unit = unit0; unit < a.units; unit += a.token_threads) {
+        constexpr int kTurns = W;        // pairs of a unit
+        float2 cs[kTurns];
+        const Unit turning = of_head(unit);
+        if (turning.turns) {
+            const float2* from = turns + mine * a.pairs + unit * kTurns;
 #pragma unroll
-        for (int s = 0; s < kHeld; ++s) {
-            const int i = base + s * kThreads;
-            if (i >= total) continue;
-            const Where u = locate(i);
-            if (u.turns) {
-                const float2* cs = turns + u.token * a.pairs;
-                if constexpr (W == 8 && NEIGHBOURS) {  // a word is a pair
-                    cs += u.first / 2;
+            for (int j = 0; j < kTurns; ++j) cs[j] = from[j];
+        }
+        for (int h0 = lane_head; h0 < heads; h0 += HELD * a.step) {
+            if (unit != unit0 || h0 != lane_head) load(unit, h0);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float2 x = turned(low<T>(one[s].w[j]), high<T>(one[s].w[j]), cs[j]);
-                        const float2 y = turned(low<T>(two[s].w[j]), high<T>(two[s].w[j]), cs[4 + j]);
-                        one[s].w[j] = Half16<T>::pack(x.x, x.y);
-                        two[s].w[j] = Half16<T>::pack(y.x, y.y);
+            for (int s = 0; s < HELD; ++s) {
+                const int h = h0 + s * a.step;
+                if (h >= heads) continue;
+                const int head = head0 + h, kind = kind_of(head);
+                const Unit u = kind < 2 ? turning : of_value(unit);
+                if (u.turns) {
+                    if constexpr (W == 8 && NEIGHBOURS) {  // a word is a pair
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float2 x = turned(low<T>(one[s].w[j]), high<T>(one[s].w[j]), cs[j]);
+                            const float2 y = turned(low<T>(two[s].w[j]), high<T>(two[s].w[j]), cs[4 + j]);
+                            one[s].w[j] = Half16<T>::pack(x.x, x.y);
+                            two[s].w[j] = Half16<T>::pack(y.x, y.y);
+                        }
+                    } else if constexpr (W == 8) {         // a word holds the first (or second) numbers of two pairs
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float2 x = turned(low<T>(one[s].w[j]), low<T>(two[s].w[j]), cs[2 * j]);
+                            const float2 y = turned(high<T>(one[s].w[j]), high<T>(two[s].w[j]), cs[2 * j + 1]);
+                            one[s].w[j] = Half16<T>::pack(x.x, y.x);
+                            two[s].w[j] = Half16<T>::pack(x.y, y.y);
+                        }
+                    } else {
+                        const float2 x = turned(low<T>(one[s].w[0]), low<T>(two[s].w[0]), cs[0]);
+                        one[s].w[0] = Half16<T>::from_float(x.x);
+                        two[s].w[0] = Half16<T>::from_float(x.y);
                     }
-                } else if constexpr (W == 8) {         // a word holds the first (or second) numbers of two pairs
-                    cs += u.first;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float2 x = turned(low<T>(one[s].w[j]), low<T>(two[s].w[j]), cs[2 * j]);
-                        const float2 y = turned(high<T>(one[s].w[j]), high<T>(two[s].w[j]), cs[2 * j + 1]);
-                        one[s].w[j] = Half16<T>::pack(x.x, y.x);
-                        two[s].w[j] = Half16<T>::pack(x.y, y.y);
-                    }
-                } else {
-                    const float2 x = turned(low<T>(one[s].w[0]), low<T>(two[s].w[0]), cs[NEIGHBOURS ? u.first / 2 : u.first]);
-                    one[s].w[0] = Half16<T>::from_float(x.x);
-                    two[s].w[0] = Half16<T>::from_float(x.y);
                 }
+                uint16_t* p = a.dst[kind] + (token0 + mine) * a.dst_token[kind] +
+                              (head - (kind > 0 ? a.nq : 0) - (kind > 1 ? a.nkv : 0)) * a.dst_head[kind];
+                if (kind > 0 && a.slots > 0) {
+                    if (at[mine] < 0) continue;
+                    p += at[mine] * a.head_dim;
+                }
+                if (u.first >= 0) one[s].store(p + u.first);
+                if (u.second >= 0) two[s].store(p + u.second);
             }
-            uint16_t* p = a.dst[u.kind] + (token0 + u.token) * a.dst_token[u.kind] + u.head * a.dst_head[u.kind];
-            if (u.kind > 0 && a.slots > 0) {
-                if (at[u.token] < 0) continue;
-                p += at[u.token] * a.head_dim;
-            }
-            if (u.first >= 0) one[s].store(p + u.first);
-            if (u.second >= 0) two[s].store(p + u.second);
         }
     }
 }
@@ -192,8 +205,10 @@ __global__ void rotary_table_kernel(float2* __restrict__ table, const double* fr
 
 template <typename T, bool NEIGHBOURS>
 cudaError_t launch_width(const RotaryArgs& a, bool wide, dim3 grid, size_t smem, cudaStream_t stream) {
-    return wide ? launch_overlapped(rotary_kernel<T, NEIGHBOURS, 8>, grid, dim3(kThreads), smem, stream, a)
-                : launch_overlapped(rotary_kernel<T, NEIGHBOURS, 1>, grid, dim3(kThreads), smem, stream, a);
+    const bool one = (a.block_heads + a.step - 1) / a.step == 1 && a.units <= a.token_threads;
+    auto* kernel = wide ? (one ? rotary_kernel<T, NEIGHBOURS, 8, 1> : rotary_kernel<T, NEIGHBOURS, 8, kHeld>)
+                        : (one ? rotary_kernel<T, NEIGHBOURS, 1, 1> : rotary_kernel<T, NEIGHBOURS, 1, kHeld>);
+    return launch_overlapped(kernel, grid, dim3(kThreads), smem, stream, a);
 }
 
 int32_t launch_rotary(const char* who, RotaryArgs a, int32_t layout, int32_t dtype, cudaStream_t stream) {
@@ -207,17 +222,19 @@ int32_t launch_rotary(const char* who, RotaryArgs a, int32_t layout, int32_t dty
     const int copied = (a.head_dim - 2 * a.pairs + 2 * w - 1) / (2 * w), whole = (a.head_dim + 2 * w - 1) / (2 * w);
     a.units = a.turning + copied;
     if (kinds == 3 && a.units < whole) a.units = whole;  // a head of v is copied whole
-    // About kHeld units a thread; with few tokens, fewer, so that every multiprocessor has a block.
+    // As many tokens a block as give a thread about kHeld heads; with few tokens, fewer, so that every
+    // multiprocessor has a block.
     const int sms = sm_count(), per_token = a.heads * a.units;
-    int tokens = (kHeld * kThreads + per_token - 1) / per_token;
-    const int spread = (a.tokens + 2 * sms - 1) / (2 * sms);
-    tokens = tokens < spread ? tokens : spread;
-    tokens = tokens > kMaxTokens ? kMaxTokens : tokens;
-    if (tokens * a.pairs > kMaxTurns) tokens = kMaxTurns / a.pairs;
+    int tokens = 1;
+    while (tokens < kMaxTokens && 2 * tokens * a.pairs <= kMaxTurns && kThreads / (2 * tokens) >= a.units &&
+           2 * tokens * per_token <= kHeld * kThreads && (a.tokens + 2 * tokens - 1) / (2 * tokens) >= 2 * sms)
+        tokens *= 2;
     a.block_tokens = tokens;
+    a.token_threads = kThreads / tokens;
+    a.step = a.token_threads / a.units > 1 ? a.token_threads / a.units : 1;
     const int blocks = (a.tokens + tokens - 1) / tokens;
     int parts = 2 * sms / blocks;                                    // blocks a token's heads are divided among
-    const int most = (per_token + kThreads / 2 - 1) / (kThreads / 2);  // at least half a unit a thread
+    const int most = (per_token + kThreads / 2 - 1) / (kThreads / 2);  // at least half the threads have a unit
     parts = parts > most ? most : parts;
     parts = parts > a.heads ? a.heads : parts < 1 ? 1 : parts;
     a.block_heads = (a.heads + parts - 1) / parts;
