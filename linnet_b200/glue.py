@@ -147,17 +147,19 @@ def silu_mul(gate_up: torch.Tensor) -> torch.Tensor:
 # ---- many answers to one prompt --------------------------------------------------------------
 
 _LAYOUTS = {"half": 0, "interleaved": 1}
+_Strides = ctypes.c_int64 * 12
 
 
 def _same(who: str, kinds: tuple[torch.dtype, ...], *tensors: torch.Tensor) -> torch.device:
     """One CUDA device, one of `kinds`, last dimension contiguous, no derivative asked for."""
     first = tensors[0]
+    index, kind = first.get_device(), first.dtype
     for t in tensors:
-        if not t.is_cuda or t.get_device() != first.get_device() or t.dtype != first.dtype or t.dtype not in kinds:
+        if t.get_device() != index or index < 0 or t.dtype is not kind or kind not in kinds:
             names = ", ".join(str(k).removeprefix("torch.") for k in kinds)
             raise RuntimeError(f"{who} takes CUDA tensors of one device and one of the types {names}; got "
                                f"{[f'{t.dtype} on {t.device}' for t in tensors]}")
-        if t.stride(-1) != 1 and t.numel() > 0 and t.shape[-1] > 1:
+        if not t.is_contiguous() and t.stride(-1) != 1 and t.numel() > 0 and t.shape[-1] > 1:
             raise RuntimeError(f"{who}: the last dimension has to be contiguous")
         if t.requires_grad and torch.is_grad_enabled():
             raise RuntimeError(f"{who} has no derivative: detach its inputs or call it under torch.no_grad()")
@@ -224,21 +226,23 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, fre
     pairs = _frequencies("rotary", frequencies, hd, device)
     code = _layout("rotary", layout)
     if out is None:
-        q_out, k_out = torch.empty(q.shape, dtype=q.dtype, device=device), None
+        q_out, k_out = torch.empty(tokens, nq, hd, dtype=q.dtype, device=device), None
         if k is not None:
-            k_out = torch.empty(k.shape, dtype=k.dtype, device=device)
+            k_out = torch.empty(tokens, k.shape[1], hd, dtype=k.dtype, device=device)
     else:
         q_out, k_out = out
         if q_out.shape != q.shape or (k is None) != (k_out is None) or (k is not None and k_out.shape != k.shape):
             raise ValueError("rotary: out has to have the shapes of q and k")
         _same("rotary", _HALF, q, q_out, *(() if k is None else (k_out,)))
-    given, made = (q, q if k is None else k), (q_out, q_out if k is None else k_out)
-    strides = [t.stride(d) for t in (*given, *made) for d in (0, 1)]
+    q_from, q_to = q.stride(), q_out.stride()
+    keys, k_from, k_to, nkv, at = None, q_from, q_to, 0, None
+    if k is not None:
+        keys, k_from, k_to, nkv, at = k.data_ptr(), k.stride(), k_out.stride(), k.shape[1], k_out.data_ptr()
     with _Device(device):
         _lib.check(_lib.load().b200q_rotary(
-            q.data_ptr(), None if k is None else k.data_ptr(), positions.data_ptr(), frequencies.data_ptr(),
-            q_out.data_ptr(), None if k is None else k_out.data_ptr(), tokens, nq, 0 if k is None else k.shape[1], hd,
-            pairs, *strides, factor, code, _CODES[q.dtype], _raw_stream(device.index)))
+            q.data_ptr(), keys, positions.data_ptr(), frequencies.data_ptr(), q_out.data_ptr(), at, tokens, nq, nkv, hd,
+            pairs, q_from[0], q_from[1], k_from[0], k_from[1], q_to[0], q_to[1], k_to[0], k_to[1], factor, code,
+            _CODES[q.dtype], _raw_stream(device.index)))
     return q_out, k_out
 
 
@@ -309,8 +313,9 @@ def prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Te
         at, _ = _word("prefix_attention", "prefix_length", prefix_length, device)
         if at is None:
             raise ValueError("prefix_attention: prefix_length is one int64 on the device (or cut the prefix to its length)")
-    strides = (*_steps(q, 0, 1), *_steps(prefix_k, 1, 0), *_steps(prefix_v, 1, 0), *_steps(cache_k, 2, 1, 0),
-               *_steps(cache_v, 2, 1, 0))
+    pk, pv, ck, cv = prefix_k.stride(), prefix_v.stride(), cache_k.stride(), cache_v.stride()
+    steps = q.stride()
+    strides = _Strides(steps[0], steps[1], pk[1], pk[0], pv[1], pv[0], ck[2], ck[1], ck[0], cv[2], cv[1], cv[0])
     lib = _lib.load()
     with _Device(device):
         size = lib.b200q_prefix_attention_scratch_bytes(batch, nq, nkv, hd, prefix, cache_k.shape[2])
@@ -321,14 +326,9 @@ def prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Te
         _lib.check(lib.b200q_prefix_attention(
             q.data_ptr(), prefix_k.data_ptr(), prefix_v.data_ptr(), cache_k.data_ptr(), cache_v.data_ptr(),
             positions.data_ptr(), at, out.data_ptr(), scratch.data_ptr(), batch, nq, nkv, hd, prefix, cache_k.shape[2],
-            (ctypes.c_int64 * 12)(*strides), hd ** -0.5 if scale is None else scale, _CODES[q.dtype],
+            strides, hd ** -0.5 if scale is None else scale, _CODES[q.dtype],
             _raw_stream(device.index)))
     return out
-
-
-def _steps(t: torch.Tensor, *dims: int) -> tuple[int, ...]:
-    """Strides of dims; that of a dimension of one means nothing."""
-    return tuple(t.stride(d) if t.shape[d] > 1 else 0 for d in dims)
 
 
 class TokenLogprobs(NamedTuple):
@@ -351,9 +351,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     if (tokens.device != device or tokens.dtype != torch.int64 or tokens.shape != (rows,) or not tokens.is_contiguous()):
         raise ValueError(f"token_logprobs: tokens must be a contiguous int64 tensor of {rows} entries on {device}, not "
                          f"{tokens.dtype}{list(tokens.shape)} on {tokens.device}")
-    numbers = torch.empty(rows * (2 + max(top, 0)), dtype=torch.float32, device=device)
-    index = torch.empty(rows, max(top, 0), dtype=torch.int64, device=device)
-    logprob, entropy, best = numbers[:rows], numbers[rows:2 * rows], numbers[2 * rows:].view(rows, max(top, 0))
+    kept = max(top, 0)
+    logprob, entropy = torch.empty(2, rows, dtype=torch.float32, device=device).unbind()
+    best = torch.empty(rows, kept, dtype=torch.float32, device=device)
+    index = torch.empty(rows, kept, dtype=torch.int64, device=device)
     with _Device(device):
         _lib.check(_lib.load().b200q_token_logprobs(
             logits.data_ptr(), tokens.data_ptr(), logprob.data_ptr(), entropy.data_ptr(), best.data_ptr(),
