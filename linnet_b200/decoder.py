@@ -20,7 +20,8 @@ CPU tests pass the oracle, so the sharding and the collectives are exercised on 
 ranks without a GPU.  Between the linears (RMSNorm, rotary embedding, cache write,
 attention, SwiGLU) `step` has two routes with the same arithmetic: plain PyTorch ops (any
 device; what the reference's generated source does, and what the CPU tests run) and, on a
-GPU, the fused kernels of `linnet_b200.glue` (eight launches a layer instead of about fifty).
+GPU, the fused kernels of `linnet_b200.glue` (eight launches a layer instead of about fifty).  Rows that
+answer the same prompt share its cache (`share_prefix`) on both routes.
 Either way a step is recorded into one CUDA graph per batch size, which is how the
 reference's serving engine replays a decode step
 (python/linnet/src/linnet/torch/compiled.py:430-503).
@@ -35,6 +36,8 @@ from typing import Callable
 import torch
 import torch.distributed as dist
 import torch.nn.functional as F
+
+from .rope import RopeScaling, frequencies
 
 Linear = Callable[[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor], torch.Tensor]
 
@@ -52,6 +55,7 @@ class DecoderConfig:
     eps: float = 1e-5
     max_seq: int = 2048
     group: int = 128
+    rope_scaling: RopeScaling | None = None
 
     @staticmethod
     def llama31_8b() -> "DecoderConfig":
@@ -128,9 +132,23 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, theta: float) -> torch.Tens
     return torch.cat([a * cos - b * sin, b * cos + a * sin], dim=-1).to(x.dtype)
 
 
+def rotary_by(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, factor: float) -> torch.Tensor:
+    """`rotary` of given frequencies f64 [D / 2], angles formed in f64: what `glue.rotary_cache` computes."""
+    half = x.shape[-1] // 2
+    angle = positions.to(torch.float64)[:, None] * freqs[None, :]
+    cos, sin = (factor * angle.cos()).float()[:, None, :], (factor * angle.sin()).float()[:, None, :]
+    a, b = x[..., :half].float(), x[..., half:].float()
+    return torch.cat([a * cos - b * sin, b * cos + a * sin], dim=-1).to(x.dtype)
+
+
 class Int4Decoder:
     """One tensor-parallel rank of the decoder.  `step` runs one decode step for
-    `tokens` [B] at `positions` [B] and returns the full `[B, vocab]` logits."""
+    `tokens` [B] at `positions` [B] and returns the full `[B, vocab]` logits; `score` runs one and
+    returns the log probabilities of given next tokens.
+
+    Many answers to one prompt: step the prompt into a cache of one row, then
+    `share_prefix(length, batch, max_new)`; from there on every row has a cache of its own of
+    `max_new` positions behind the prompt, which is stored and read once for all of them."""
 
     def __init__(self, cfg: DecoderConfig, layers: list[LayerWeights], embed: torch.Tensor,
                  final_norm: torch.Tensor, head: Int4, *, linear: Linear, rank: int = 0, tp: int = 1,
@@ -151,27 +169,81 @@ class Int4Decoder:
         self.cache_v: list[torch.Tensor] = []
         self.peer_reduce = None  # set by enable_peer_reduce()
         self.rope_table = None   # cos / sin of every position, made by allocate_cache()
+        self.frequencies: torch.Tensor | None = None  # of the rotary positions, where the table does not serve
+        self.rope_factor = 1.0
+        self.prompt: "tuple[list[torch.Tensor], list[torch.Tensor]] | None" = None  # the caches a prefix is shared from
+        self.answers: "tuple[list[torch.Tensor], list[torch.Tensor]] | None" = None  # the rows' own caches behind it
+        self.prefix: "list[tuple[torch.Tensor, torch.Tensor]] | None" = None  # keys and values of a layer's prefix
+        self.prefix_length: torch.Tensor | None = None  # one int64: how many of its positions there are
 
     # -- state ---------------------------------------------------------------------
     def allocate_cache(self, batch: int, fill: "torch.Generator | None" = None) -> None:
         """A `[batch, kv_heads / tp, max_seq, head_dim]` cache per layer for K and V,
         filled ~N(0, 1) when a generator is given (the benchmark's synthetic history)."""
+        self.prompt = self.answers = self.prefix = self.prefix_length = None
         cfg = self.cfg
-        shape = (batch, cfg.kv_heads // self.tp, cfg.max_seq, cfg.head_dim)
-        dev, dt = self.embed.device, self.embed.dtype
-        self.cache_k, self.cache_v = [], []
+        self.cache_k, self.cache_v = self._caches(batch, cfg.max_seq, fill)
+        dev = self.embed.device
+        if cfg.rope_scaling is not None:
+            self._make_frequencies()
+        if self.fused and dev.type == "cuda" and self.rope_table is None:
+            from . import glue
+
+            if cfg.rope_scaling is None:
+                self.rope_table = glue.rope_table(cfg.max_seq, cfg.head_dim, cfg.rope_theta, dev)
+            else:
+                self.rope_table = glue.rotary_table(cfg.max_seq, self.frequencies, self.rope_factor)
+
+    def _caches(self, batch: int, slots: int,
+                fill: "torch.Generator | None" = None) -> "tuple[list[torch.Tensor], list[torch.Tensor]]":
+        cfg = self.cfg
+        shape = (batch, cfg.kv_heads // self.tp, slots, cfg.head_dim)
+        keys: list[torch.Tensor] = []
+        values: list[torch.Tensor] = []
         for _ in range(cfg.layers):
-            for store in (self.cache_k, self.cache_v):
-                t = torch.empty(shape, device=dev, dtype=dt)
+            for store in (keys, values):
+                t = torch.empty(shape, device=self.embed.device, dtype=self.embed.dtype)
                 if fill is not None:
                     t.normal_(generator=fill)
                 else:
                     t.zero_()
                 store.append(t)
-        if self.fused and dev.type == "cuda" and self.rope_table is None:
-            from . import glue
+        return keys, values
 
-            self.rope_table = glue.rope_table(cfg.max_seq, cfg.head_dim, cfg.rope_theta, dev)
+    def _make_frequencies(self) -> None:
+        if self.frequencies is None:
+            numbers, self.rope_factor = frequencies(self.cfg.head_dim, self.cfg.rope_theta, self.cfg.rope_scaling)
+            self.frequencies = torch.tensor(numbers, dtype=torch.float64, device=self.embed.device)
+
+    def share_prefix(self, length: int, batch: int, max_new: int, row: int = 0) -> None:
+        """Positions 0 .. length - 1 of cache row `row` become the prefix of `batch` rows, each with an
+        empty cache of `max_new` positions of its own: from here on `step` takes, as positions, a row's
+        slot in its own cache, which lies at position length + slot of the model.  The caches the prefix
+        is read from stay as they are; `end_prefix` makes them the step's again, for the next prompt.
+        Sharing again with the same batch, max_new and row keeps every address (and the length is read
+        on the device), so that a captured step may be replayed."""
+        prompt = self.prompt or (self.cache_k, self.cache_v)
+        if not prompt[0]:
+            raise ValueError("share_prefix: there is no cache yet (allocate_cache)")
+        rows, _, slots, _ = prompt[0][0].shape
+        if not 0 <= row < rows or not 0 <= length <= slots or batch < 1 or max_new < 1:
+            raise ValueError(f"share_prefix: {length} positions of row {row} for {batch} rows of {max_new}; the cache "
+                             f"has {rows} rows of {slots} positions")
+        self._make_frequencies()
+        if self.answers is None or self.answers[0][0].shape[0] != batch or self.answers[0][0].shape[2] != max_new:
+            self.answers = self._caches(batch, max_new)
+        if self.prefix_length is None:
+            self.prefix_length = torch.empty(1, dtype=torch.int64, device=self.embed.device)
+        self.prefix_length.fill_(length)
+        self.prompt = prompt
+        self.prefix = [(k[row], v[row]) for k, v in zip(*prompt)]
+        self.cache_k, self.cache_v = self.answers
+
+    def end_prefix(self) -> None:
+        """Back to the caches that `share_prefix` read the prefix from."""
+        if self.prompt is not None:
+            self.cache_k, self.cache_v = self.prompt
+            self.prompt = self.prefix = None
 
     # -- collectives ---------------------------------------------------------------
     def _all_reduce(self, x: torch.Tensor) -> torch.Tensor:
@@ -192,6 +264,34 @@ class Int4Decoder:
         if self.fused:
             return self._step_fused(tokens, positions)
         return self._step_torch(tokens, positions)
+
+    def score(self, tokens: torch.Tensor, positions: torch.Tensor, given: torch.Tensor, top: int = 0):
+        """One step, and of its logits the log probabilities of the tokens `given` [B] to come next, the
+        entropy of every row and its `top` most probable tokens (`glue.TokenLogprobs`; a negative
+        token is none)."""
+        from . import glue
+
+        logits = self.step(tokens, positions)
+        if self.fused:
+            return glue.token_logprobs(logits, given, top)
+        logp = torch.log_softmax(logits.float(), dim=-1)
+        best = logp.topk(top, dim=-1)
+        # 0 * -inf of a forbidden token adds nothing to the entropy
+        entropy = -(logp.exp() * logp.clamp_min(torch.finfo(torch.float32).min)).sum(dim=-1)
+        logprob = logp.gather(1, given.clamp_min(0)[:, None])[:, 0].masked_fill(given < 0, 0.0)
+        return glue.TokenLogprobs(logprob, entropy, best.values, best.indices)
+
+    def _attend(self, layer: int, qkv: torch.Tensor, positions: torch.Tensor, nq: int, nkv: int) -> torch.Tensor:
+        """Rotary positions, cache write and attention of the fused routes: over a row's cache, or
+        over the shared prefix and then the row's own cache."""
+        from . import glue
+
+        keys, values = self.cache_k[layer], self.cache_v[layer]
+        if self.prefix is None:
+            return glue.rope_attention(qkv, positions, self.rope_table, keys, values, nq, nkv)
+        q = glue.rotary_cache(qkv, positions, self.frequencies, keys, values, nq, nkv, factor=self.rope_factor,
+                              offset=self.prefix_length)
+        return glue.prefix_attention(q, *self.prefix[layer], keys, values, positions, prefix_length=self.prefix_length)
 
     def enable_peer_reduce(self, max_rows: int, protocol: str | None = None) -> None:
         """Replaces each NCCL all-reduce + residual add + norm of the fused route by one
@@ -242,8 +342,7 @@ class Int4Decoder:
         delta = None
         for i, w in enumerate(self.layers):
             qkv = product(delta, w.norm1, w.qkv)
-            attn = glue.rope_attention(qkv, positions, self.rope_table, self.cache_k[i], self.cache_v[i],
-                                       cfg.heads, cfg.kv_heads)
+            attn = self._attend(i, qkv, positions, cfg.heads, cfg.kv_heads)
             gate_up = product(self.linear(attn, *w.o), w.norm2, w.gate_up)
             if self.fold_swiglu:
                 delta = self.linear(gate_up, *w.down, swiglu=True)
@@ -262,7 +361,7 @@ class Int4Decoder:
         h = glue.add_rmsnorm(x, None, self.layers[0].norm1, cfg.eps)
         for i, w in enumerate(self.layers):
             qkv = self._product(h, w.qkv)
-            attn = glue.rope_attention(qkv, positions, self.rope_table, self.cache_k[i], self.cache_v[i], nq, nkv)
+            attn = self._attend(i, qkv, positions, nq, nkv)
             h = self._reduce_norm(2 * i, x, attn, w.o, w.norm2)
             following = self.layers[i + 1].norm1 if i + 1 < len(self.layers) else self.final_norm
             if self.fold_swiglu:
@@ -277,18 +376,34 @@ class Int4Decoder:
         nq, nkv, hd = cfg.heads // tp, cfg.kv_heads // tp, cfg.head_dim
         batch = tokens.shape[0]
         rows = torch.arange(batch, device=tokens.device)
-        mask = (torch.arange(cfg.max_seq, device=tokens.device)[None, :] <= positions[:, None])[:, None, None, :]
+
+        def upto(slots: int, last: torch.Tensor) -> torch.Tensor:
+            return torch.arange(slots, device=tokens.device)[None, :] <= last[:, None]
+
+        mask, angles = upto(self.cache_k[0].shape[2], positions), positions
+        if self.prefix is not None:
+            shared = upto(self.prefix[0][0].shape[1], self.prefix_length - 1).expand(batch, -1)
+            mask, angles = torch.cat([shared, mask], dim=1), positions + self.prefix_length
+        mask = mask[:, None, None, :]
+
+        def turn(x: torch.Tensor) -> torch.Tensor:
+            if self.prefix is None and cfg.rope_scaling is None:
+                return rotary(x, positions, cfg.rope_theta)
+            return rotary_by(x, angles, self.frequencies, self.rope_factor)
+
         x = self.embed[tokens]
         for i, w in enumerate(self.layers):
             h = F.rms_norm(x, (cfg.hidden,), w.norm1, cfg.eps)
             qkv = self.linear(h, *w.qkv)
             q, k, v = qkv.split([nq * hd, nkv * hd, nkv * hd], dim=-1)
-            q = rotary(q.reshape(batch, nq, hd), positions, cfg.rope_theta)
-            k = rotary(k.reshape(batch, nkv, hd), positions, cfg.rope_theta)
+            q, k = turn(q.reshape(batch, nq, hd)), turn(k.reshape(batch, nkv, hd))
             self.cache_k[i][rows, :, positions] = k
             self.cache_v[i][rows, :, positions] = v.reshape(batch, nkv, hd)
-            attn = F.scaled_dot_product_attention(q[:, :, None, :], self.cache_k[i], self.cache_v[i],
-                                                  attn_mask=mask, enable_gqa=True)
+            keys, values = self.cache_k[i], self.cache_v[i]
+            if self.prefix is not None:
+                keys, values = (torch.cat([p.expand(batch, -1, -1, -1), own], dim=2)
+                                for p, own in zip(self.prefix[i], (keys, values)))
+            attn = F.scaled_dot_product_attention(q[:, :, None, :], keys, values, attn_mask=mask, enable_gqa=True)
             x = x + self._all_reduce(self.linear(attn.reshape(batch, nq * hd), *w.o))
             h = F.rms_norm(x, (cfg.hidden,), w.norm2, cfg.eps)
             gate_up = self.linear(h, *w.gate_up)
