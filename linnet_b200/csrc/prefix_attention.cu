@@ -42,6 +42,7 @@ constexpr int kProducerWarp = 8, kIssuerWarp = 10, kListWarp = 12;  // a produce
 constexpr int kThreads = 13 * 32;
 constexpr uint32_t kTmemColumns = 512;     // S of both groups, O of both groups
 constexpr float kStale = 8.0f;             // how far (log2) a tile's maximum may exceed the row's before it moves
+constexpr float kLowest = -3.0e38f;        // the maximum of scores that are all -inf: 2^(-inf - m) is 0, and any other exceeds it
 constexpr int kOwnStart = 1;               // what an item of own keys costs beside its tiles, in tiles
 
 template <int HD>
@@ -192,13 +193,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
         : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return r;
 }
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 r;
-    asm("{\n.reg .b64 x, y, z, w;\nmov.b64 x, {%2,%3};\nmov.b64 y, {%4,%5};\nmov.b64 z, {%6,%7};\n"
-        "fma.rn.f32x2 w, x, y, z;\nmov.b64 {%0,%1}, w;\n}"
-        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return r;
-}
 // V, MN-major with the 128-byte swizzle: rows (keys) of 128 bytes, 8-row atoms 1024 bytes apart along
 // the keys, columns 64..127 of D a half further.
 __device__ __forceinline__ uint64_t value_desc(uint32_t addr, uint32_t half) {
@@ -230,19 +224,29 @@ __device__ __forceinline__ void tmem_put_8(uint32_t taddr, const uint32_t (&v)[8
                  "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                  : "memory");
 }
+// Descriptors by halves: the address (in 16 bytes) is in the low one, all else stays.
+__device__ __forceinline__ uint64_t desc_of(uint32_t low, uint32_t high) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(low), "r"(high));
+    return d;
+}
+__device__ __forceinline__ void commit_at(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map)); }
 
-__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {  // does not suspend the thread
+__device__ __forceinline__ bool test_at(uint32_t bar, uint32_t parity) {  // does not suspend the thread
     uint32_t ok;
     asm volatile(
         "{\n.reg .pred p;\n"
         "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
         "selp.u32 %0, 1, 0, p;\n}"
         : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
+        : "r"(bar), "r"(parity)
         : "memory");
     return ok != 0;
 }
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) { return test_at(smem_u32(bar), parity); }
 
 // The bounded wait, once in the code for all roles: with its slow path written out at every use the
 // kernel was 80 KB, and its short turns went by the instruction cache.
@@ -252,6 +256,33 @@ __device__ __noinline__ bool mbar_wait_long(uint64_t* bar, uint32_t parity, int*
 __device__ __forceinline__ bool mbar_watch(uint64_t* bar, uint32_t parity, int* error, int code) {
     return mbar_try_wait(bar, parity) || mbar_wait_long(bar, parity, error, code);
 }
+
+// The same by the barrier's address in shared memory.
+__device__ __forceinline__ bool watch_at(uint32_t bar, uint32_t parity, int* error, int code) {
+    uint32_t ok;
+    asm volatile(
+        "{\n.reg .pred p;\n"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
+        "selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(kSuspendNs)
+        : "memory");
+    return ok != 0 || mbar_wait_long(static_cast<uint64_t*>(__cvta_shared_to_generic(bar)), parity, error, code);
+}
+
+// A way through a ring of slots: addresses of its barriers and its memory (that in 16 bytes), and where it stands.
+struct Walk {
+    uint32_t full, empty, memory, slots;
+    uint32_t slot, parity;
+    __device__ __forceinline__ void start(uint32_t load) {
+        const uint32_t lap = load / slots;
+        slot = load - lap * slots, parity = lap & 1;
+    }
+    __device__ __forceinline__ void step(uint32_t loads) {  // fewer than there are slots
+        slot += loads;
+        if (slot >= slots) slot -= slots, parity ^= 1;
+    }
+};
 
 struct Barriers {
     uint64_t full[20], empty[20];              // tiles of K and V that both groups take
@@ -482,9 +513,23 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
             constexpr uint32_t kValues = (1u << 4) | (kType << 7) | (kType << 10) | (1u << 16) | (uint32_t(HD >> 3) << 17) | (uint32_t(kRows >> 4) << 24);
             const int g = warp - kIssuerWarp;
             const uint32_t s_at = tmem + uint32_t(g) * 2 * kKeys, o_at = tmem + 4 * kKeys + uint32_t(g) * HD;
+            const uint32_t scores = smem_u32(&bars.scores[g][0]), weights = smem_u32(&bars.weights[g][0]), summed = smem_u32(&bars.summed[g]),
+                           result = smem_u32(&bars.result[g]), query_full = smem_u32(&bars.query_full[g][0]),
+                           query_empty = smem_u32(&bars.query_empty[g][0]), queries = (smem_u32(smem) + g * S::kQuery) >> 4;
+            const uint32_t k_high = uint32_t(smem_desc(0) >> 32), k_low = uint32_t(smem_desc(0));
+            const uint32_t v_high = uint32_t(value_desc(0, S::kHalf) >> 32), v_low = uint32_t(value_desc(0, S::kHalf));
+            auto walk = [&](const Piece& p, uint32_t load) {
+                const bool both = p.who == kBoth;
+                Walk w;
+                w.full = smem_u32(both ? bars.full : bars.own_full[g]), w.empty = smem_u32(both ? bars.empty : bars.own_empty[g]);
+                w.memory = (smem_u32(slots) + (both ? 0 : g * kOwnSlots) * S::kSlot) >> 4, w.slots = both ? S::kSlots : kOwnSlots;
+                w.start(p.base + load);
+                return w;
+            };
             // Two ways through the group's tiles: the sums', and the scores' up to two tiles ahead of it.
             Pieces pieces(&bars);
             Piece p, q;                           // the sums' and the scores' piece
+            Walk vs = {}, ks = {};                // their loads
             int tile = 0, q_tile = 0;
             uint32_t task = 0, q_task = 0, q_index = 0, changes = 0;
             bool found = false;                   // q is the scores' next piece, or the end
@@ -500,75 +545,75 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
                     }
                 } while (!p.of(g) || p.tiles == 0);
                 tile = 0;
+                vs = walk(p, load_of_v(0, p.tiles));
             };
-            // The slot of a load of a piece, and the barriers that go with it.
-            auto slot_of = [&](const Piece& p, uint32_t load, uint64_t** full, uint64_t** empty, uint32_t* parity) {
-                const uint32_t n = p.base + load, ring = p.who == kBoth ? S::kSlots : kOwnSlots, lap = n / ring, slot = n - lap * ring;
-                *full = (p.who == kBoth ? bars.full : bars.own_full[g]) + slot;
-                *empty = (p.who == kBoth ? bars.empty : bars.own_empty[g]) + slot;
-                *parity = lap & 1;
-                return smem_u32(slots) + ((p.who == kBoth ? 0 : g * kOwnSlots) + slot) * S::kSlot;
+            // The next scores' operands, where they are to be had: their keys and queries are there (and are waited for
+            // only if the sums have nothing to do without), and they lie neither beyond a change of kind that the sums
+            // have not come to nor two batches on.
+            uint32_t buffer = 0, query_parity = 0;
+            auto scores_ready = [&]() {
+                const bool wanted = q_task == task;
+                while (!found) {
+                    if (wanted) {
+                        q = p, q_index = pieces.i, found = true;
+                    } else {
+                        const uint32_t batch = q_index / kBatch;
+                        if (q_index % kBatch == 0 && (batch > (pieces.i - 1) / kBatch + 1 || !mbar_test(&bars.list_full[batch & 1], (batch >> 1) & 1))) return false;
+                        q = bars.list[q_index++ % (2 * kBatch)];
+                        found = q.who == kEnd || (q.of(g) && q.tiles > 0);
+                    }
+                    if (found && q.who != kEnd) {
+                        const Query query(q, g);
+                        q_tile = 0, buffer = query.buffer(), query_parity = query.parity();
+                        ks = walk(q, load_of_k(0));
+                    }
+                }
+                if (q.who == kEnd || q.epoch != p.epoch) return false;
+                if (!wanted) return (q_tile > 0 || test_at(query_full + 8 * buffer, query_parity)) && test_at(ks.full + 8 * ks.slot, ks.parity);
+                ok = (q_tile > 0 || watch_at(query_full + 8 * buffer, query_parity, a.error, 43)) &&
+                     watch_at(ks.full + 8 * ks.slot, ks.parity, a.error, 44);
+                return ok;
+            };
+            auto issue_scores = [&]() {
+                const uint32_t b = q_task & 1, at = s_at + b * kKeys;
+                const uint32_t qd = k_low + queries + buffer * (64 * 128 >> 4), kd = k_low + ks.memory + ks.slot * (S::kSlot >> 4);
+#pragma unroll
+                for (int k = 0; k < HD / 16; ++k)
+                    umma_f16_ss(at, desc_of(qd + uint32_t(k / 4) * ((kRows * 128) >> 4) + uint32_t(k % 4) * 2, k_high),
+                                desc_of(kd + uint32_t(k / 4) * (S::kHalf >> 4) + uint32_t(k % 4) * 2, k_high), kScores, k > 0);
+                commit_at(scores + 8 * b);
+                commit_at(ks.empty + 8 * ks.slot);
+                ++q_task;
+                ks.step(q_tile == 0 ? 1 : 2);
+                if (++q_tile == q.tiles) {
+                    commit_at(query_empty + 8 * buffer);
+                    found = false;
+                }
             };
             next_piece();
             while (ok && p.who != kEnd) {
-                // Scores: not beyond a change of kind that the sums have not come to, nor two batches on, and the sums
-                // do not wait for keys that are late.
-                while (ok && q_task < task + 2) {
-                    if (!found) {
-                        if (q_task == task) {
-                            q = p, q_index = pieces.i, found = true;
-                        } else {
-                            const uint32_t batch = q_index / kBatch;
-                            if (q_index % kBatch == 0 && (batch > (pieces.i - 1) / kBatch + 1 || !mbar_test(&bars.list_full[batch & 1], (batch >> 1) & 1))) break;
-                            q = bars.list[q_index++ % (2 * kBatch)];
-                            found = q.who == kEnd || (q.of(g) && q.tiles > 0);
-                            if (!found) continue;
-                        }
-                        q_tile = 0;
-                    }
-                    if (q.who == kEnd || q.epoch != p.epoch) break;
-                    const Query query(q, g);
-                    uint64_t* const query_full = &bars.query_full[g][query.buffer()];
-                    uint64_t *full, *empty;
-                    uint32_t parity;
-                    const uint32_t at = slot_of(q, load_of_k(q_tile), &full, &empty, &parity);
-                    if (q_task != task && !((q_tile > 0 || mbar_test(query_full, query.parity())) && mbar_test(full, parity))) break;
-                    if (q_tile == 0) ok = mbar_watch(query_full, query.parity(), a.error, 43);
-                    ok = ok && mbar_watch(full, parity, a.error, 44);
-                    if (!ok) break;
+                while (q_task < task + 2 && scores_ready()) {
                     tc_fence_after();
-                    const uint32_t b = q_task & 1;
-                    const uint64_t qd = smem_desc(smem_u32(smem) + g * S::kQuery + query.buffer() * (64 * 128)), kd = smem_desc(at);
-#pragma unroll
-                    for (int k = 0; k < HD / 16; ++k)
-                        umma_f16_ss(s_at + b * kKeys, qd + uint32_t(k / 4) * ((kRows * 128) >> 4) + uint32_t(k % 4) * 2,
-                                    kd + uint32_t(k / 4) * (S::kHalf >> 4) + uint32_t(k % 4) * 2, kScores, k > 0);
-                    umma_commit(&bars.scores[g][b]);
-                    umma_commit(empty);
-                    ++q_task;
-                    if (++q_tile == q.tiles) {
-                        umma_commit(&bars.query_empty[g][query.buffer()]);
-                        found = false;
-                    }
+                    issue_scores();
                 }
-                uint64_t *full, *empty;
-                uint32_t parity;
-                const uint32_t at = slot_of(p, load_of_v(tile, p.tiles), &full, &empty, &parity), b = task & 1;
-                ok = ok && mbar_watch(full, parity, a.error, 44) && mbar_watch(&bars.weights[g][b], (task >> 1) & 1, a.error, 45);
+                // The scores after those follow the sums at once, in the buffer that the sums read their weights from.
+                const bool follows = ok && q_task == task + 2 && scores_ready();
+                const uint32_t b = task & 1, from = s_at + b * kKeys, vd = v_low + vs.memory + vs.slot * (S::kSlot >> 4);
+                const int keys = p.keys - tile * kKeys;
+                const bool last = tile + 1 == p.tiles;
+                ok = ok && watch_at(vs.full + 8 * vs.slot, vs.parity, a.error, 44) && watch_at(weights + 8 * b, (task >> 1) & 1, a.error, 45);
                 if (!ok) break;
                 tc_fence_after();
-                const uint64_t vd = value_desc(at, S::kHalf);
-                const int keys = p.keys - tile * kKeys;
 #pragma unroll
                 for (int k = 0; k < kKeys / 16; ++k)
-                    if (k == 0 || k * 16 < keys) umma_f16_ts(o_at, s_at + b * kKeys + k * 8, vd + uint32_t(k) * (2048 >> 4), kValues, k > 0 || tile > 0);
-                umma_commit(empty);
-                umma_commit(&bars.summed[g]);
-                ++task;
-                if (++tile == p.tiles) {
-                    umma_commit(&bars.result[g]);
-                    next_piece();
-                }
+                    if (k == 0 || k * 16 < keys) umma_f16_ts(o_at, from + k * 8, desc_of(vd + uint32_t(k) * (2048 >> 4), v_high), kValues, k > 0 || tile > 0);
+                if (last) commit_at(result);
+                if (follows) issue_scores();
+                commit_at(vs.empty + 8 * vs.slot);
+                commit_at(summed);
+                ++task, ++tile;
+                if (last) next_piece();
+                else vs.step(tile + 1 == p.tiles ? 1 : 2);
             }
         }
         __syncwarp();
@@ -583,6 +628,8 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
         int kind = -1;
         uint32_t epoch = 0;
         for (uint32_t batch = 0; ok; ++batch) {
+            // (of the counts only "any" and the last two bits are asked for: long ones are kept from running into one another)
+            fills -= (fills & 0x80008000u) >> 1, own_fills -= (own_fills & 0x80008000u) >> 1;
             if (batch >= 2) ok = wait(&bars.list_empty[batch & 1], ((batch >> 1) - 1) & 1, 52);
             if (!ok) break;
             Piece* list = bars.list + (batch & 1) * kBatch;
@@ -684,7 +731,6 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
         const uint32_t s_at = lanes + uint32_t(g) * 2 * kKeys, o_at = lanes + 4 * kKeys + uint32_t(g) * HD;
         Pieces list(&bars);
         uint32_t task = 0, pieces = 0;            // that this group has had
-        const float2 scale = make_float2(a.scale_log2, a.scale_log2);
         for (;;) {
             const Piece p = list.next_of_warp(&ok, a.error);
             if (p.who == kEnd) break;
@@ -718,7 +764,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
                     const float here = a.scale_log2 * fmaxf(max3(max3(most[0], most[1], most[2]), most[3], most[4]),
                                                             max3(most[5], most[6], most[7]));
                     if (tile == 0) {
-                        m = here == -INFINITY ? 0.0f : here;
+                        m = here == -INFINITY ? kLowest : here;
                     } else if (__any_sync(0xFFFFFFFFu, row < live && here > m + kStale)) {
                         const float next = here > m + kStale ? here : m, by = exp2_approx(m - next);
                         m = next;
@@ -737,13 +783,15 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
                     }
                     // Scaled scores run kAhead pairs ahead of the exponentials and the sums as far behind, so that
                     // the exponential unit, which takes eight clocks an instruction, always has one to do.
-                    const float2 minus = make_float2(-m, -m);
                     constexpr int kPairs = kKeys / 2, kAhead = 4;
+                    uint32_t weights[kPairs];
                     float2 e[kPairs], sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-                    auto scaled = [&](int i) { e[i] = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), scale, minus); };
+                    auto scaled = [&](int i) {
+                        e[i].x = fmaf(__uint_as_float(v[2 * i]), a.scale_log2, -m), e[i].y = fmaf(__uint_as_float(v[2 * i + 1]), a.scale_log2, -m);
+                    };
                     auto added = [&](int i) {
                         sum[i & 1] = add2(sum[i & 1], e[i]);
-                        v[i] = H::pack(e[i].x, e[i].y);
+                        weights[i] = H::pack(e[i].x, e[i].y);
                     };
 #pragma unroll
                     for (int i = 0; i < kAhead; ++i) scaled(i);
@@ -755,7 +803,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
                     }
 #pragma unroll
                     for (int i = kPairs - kAhead; i < kPairs; ++i) added(i);
-                    tmem_put_32(at, v);
+                    tmem_put_32(at, weights);
                     const float2 pair = add2(sum[0], sum[1]);
                     l += pair.x + pair.y;
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
