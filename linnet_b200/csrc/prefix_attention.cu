@@ -4,30 +4,38 @@
 // cache.  Row by row the prefix would be read once a row; here all rows of a KV head that share it are
 // the 128 rows of a tcgen05 product, so its keys and values cross HBM once.
 //
-// Work is cut into TILES of 128 keys.  An ITEM is the prefix of one KV head for up to 256 query rows
+// Work is cut into tiles of 64 keys.  An ITEM is the prefix of one KV head for up to 256 query rows
 // (rep = heads / kv_heads rows a batch row), or one batch row's own keys of one KV head.  The items'
-// tiles stand in one sequence, prefix first, and block c of G takes the c-th G-th of it, so blocks
-// have equal work whatever the lengths; where a block's share begins and ends, an item is cut into
-// PIECES, each with its own softmax statistics, and a second kernel joins the pieces of a row.  An
-// item and a block have at most one piece in common, and (item + block) grows along the sequence:
-// that is a piece's place in the scratch memory.
+// tiles stand in one sequence, prefix first, and block c of G takes the c-th G-th of it, so blocks have
+// equal work whatever the lengths; where a block's share begins and ends, an item is cut into PIECES,
+// each with its own softmax statistics, and a second kernel joins the pieces of a row.  (An item of own
+// keys counts one tile more than it has, for its start: 64 rows of 16384 + 64 keys take 44.7 us so,
+// 62.5 without, 45.1 with two.)  An item and a block have at most one piece in common, and
+// (item + block) grows along the sequence: that is a piece's place in the scratch memory.
 //
-// A block: two softmax groups (4 warps, one query row a thread), a TMA producer, an issuer of the
-// products, a loader of queries.  Per task (a tile for one group):
-//   S [128 rows x 128 keys] = Q . K^T      Q and K in shared memory as TMA's 128-byte swizzle has them
+// A block has two groups, each a pipeline of its own: a TMA producer, an issuer of products and four
+// warps of softmax with one query row a thread.  Per task, a tile for one group:
+//   S [128 rows x 64 keys] = Q . K^T       Q and K in shared memory as TMA's 128-byte swizzle has them
 //   P = 2^(scale' S - m), l += sum P       one row a thread: no exchange between threads
 //   O [128 rows x D] += P . V              P in tensor memory over S's columns; V's rows are the keys, so
 //                                          it is the MN-major operand as it lies in memory
-// An item of more than 128 rows gives each group half of the rows and both every tile; one of fewer
-// gives both groups the same rows and alternate tiles.  Either way one group's products run while
-// the other has its exponentials.
+// S has two buffers a group, so that the next tile's scores are there while this one's weights are made.
+// A prefix item of more than 128 rows gives each group half of the rows and both every tile (each is
+// loaded once); one of fewer gives the groups the same rows and a half of the keys each; own keys are one
+// group's, the other is at the piece before or after.  A last warp, the lister, works out the pieces
+// ahead of all roles and writes them down: with that arithmetic in every role the kernel's code was 80 KB
+// and its short turns went by instruction fetches.
+//
 // m is a row's maximum of the first tile; a later tile whose own exceeds it by more than 2^8 moves it
 // and rescales O and l in tensor memory (rare: P stays below 2^8, and the sums are f32 anyway).
 // P is rounded to the tensors' type, as the product takes it; l sums P before that rounding.
 //
-// What bounds it: few rows, HBM (64 KB a tile of 128 keys at D = 128); many rows, the two products
-// (1024 clocks a task) and the 128 x 128 exponentials (1024 clocks of the special-function unit), which
-// overlap between the two groups.
+// What bounds it, measured on a B200 (nq 32, nkv 8, D 128, bf16; join included): few rows, HBM and the
+// start of the pipeline: 8 rows of 65536 keys 54 us, 5.0 TB/s; 64 rows of 8192 + up to 512 own keys
+// 40 us where the bytes take 15.6; 2 rows of 100 keys 9.3 us, two launches and their latencies.  Many
+// rows, the chain from scores to weights to the next scores: 256 rows of 65536 keys 283 us, 973 TFLOP/s
+// (59 % of measured).  A tile of both groups takes some 2200 clocks there; its products alone take 1300,
+// its 16384 exponentials 1024, its 32 KB from L2 some 1100.
 #include "mma.cuh"
 #include "umma.cuh"
 
@@ -731,6 +739,9 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
         const uint32_t s_at = lanes + uint32_t(g) * 2 * kKeys, o_at = lanes + 4 * kKeys + uint32_t(g) * HD;
         Pieces list(&bars);
         uint32_t task = 0, pieces = 0;            // that this group has had
+        // f16 has no weights below 2^-24: the largest is made 2^7 there (and 2^15 at most, before its maximum moves), so that
+        // those of 2^-21 of it still are normal numbers, and what is lost of any is 2^-32 of it at most.
+        constexpr float kLift = H::kDtype == B200Q_F16 ? 7.0f : 0.0f;
         for (;;) {
             const Piece p = list.next_of_warp(&ok, a.error);
             if (p.who == kEnd) break;
@@ -764,9 +775,9 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
                     const float here = a.scale_log2 * fmaxf(max3(max3(most[0], most[1], most[2]), most[3], most[4]),
                                                             max3(most[5], most[6], most[7]));
                     if (tile == 0) {
-                        m = here == -INFINITY ? kLowest : here;
-                    } else if (__any_sync(0xFFFFFFFFu, row < live && here > m + kStale)) {
-                        const float next = here > m + kStale ? here : m, by = exp2_approx(m - next);
+                        m = here == -INFINITY ? kLowest : here - kLift;
+                    } else if (__any_sync(0xFFFFFFFFu, row < live && here - kLift > m + kStale)) {
+                        const float next = here - kLift > m + kStale ? here - kLift : m, by = exp2_approx(m - next);
                         m = next;
                         l *= by;
                         // (these scores were asked for behind the sums before the last ones)
@@ -874,7 +885,9 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
 // columns of its rows, four columns of four numbers a warp.  Many (a long prefix for few rows and heads):
 // the parts are dealt among the warps too, and their sums meet in shared memory.
 constexpr int kJoinWarps = 8, kJoinHeld = 4;
-constexpr int kManyParts = 12;  // more than this many parts of a row are dealt among the warps
+// More than this many parts of a row are dealt among the warps: 33 rows of 5001 keys, 2 KV heads, 16.9 us so and 28.8
+// otherwise; 256 rows of 1024 + 128, 8 KV heads, 73.2 us so and 44.7 otherwise.
+constexpr int kManyParts = 12;
 
 template <typename T, int HD, bool MANY>
 __global__ void __launch_bounds__(32 * kJoinWarps)

@@ -16,6 +16,10 @@
 // element ahead of it.  So the first block finds a threshold that `top` groups reach and not many more
 // (by bisection over the floats' order where the first guess has too many), reads those groups once
 // more and ranks what reaches it.
+//
+// Measured on a B200, rows of 128256: 2048 of bf16 with 5 alternatives 107 us, 4.9 TB/s (92 without:
+// 5.7 TB/s); 64 of f32 15.8 us, 2.1 TB/s; one of bf16 with 20 alternatives 9.9 us, most of it the way
+// from the last logit over the cluster's barrier to the ranked list.
 #include <cooperative_groups.h>
 
 #include "mma.cuh"
@@ -520,13 +524,14 @@ extern "C" int32_t b200q_token_logprobs(const void* logits, const int64_t* token
     a.vocab = int(vocab), a.top = int(top);
     a.groups = int((vocab + elements - 1 + 32 * elements - 1) / (32 * elements));  // of a row wherever it starts
     a.status = decoder_error_word();
-    // As many blocks a row as four a multiprocessor take, while each has a round of its own.
+    // Blocks a row: twice as many while there are fewer than two a multiprocessor and each has a round of its own.
+    // 64 rows of 128256: 15.8 us with eight blocks each, 29.8 with one; 333 rows: 9.7 with one, 10.4 with two, 14.4 with four.
     const int64_t each = int64_t(kWarps) * kHeld;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t err = cudaSuccess;
     const int n = int(rows);
     int blocks = 1;
-    while (blocks < 8 && rows * blocks < 4 * sm_count() && a.groups > blocks * each) blocks *= 2;
+    while (blocks < 8 && rows * blocks < 2 * sm_count() && a.groups > blocks * each) blocks *= 2;
     if (dtype == B200Q_F32) err = top ? launch<float, true>(a, n, blocks, s) : launch<float, false>(a, n, blocks, s);
     else if (dtype == B200Q_BF16)
         err = top ? launch<__nv_bfloat16, true>(a, n, blocks, s) : launch<__nv_bfloat16, false>(a, n, blocks, s);

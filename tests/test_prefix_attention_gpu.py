@@ -233,3 +233,42 @@ def test_refusals():
     odd = torch.zeros(2 * 100 * 64 + 1, device="cuda", dtype=torch.bfloat16)[1:].view(2, 100, 64)
     with pytest.raises(ValueError, match="16-byte aligned"):
         glue.prefix_attention(q, odd, pv, ck, cv, positions)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("prefix,slots", [(200, 5), (1000, 0), (0, 300)])
+def test_scores_of_minus_infinity_have_no_weight(dtype, prefix, slots):
+    """Keys that score -inf for every row fill the first tiles; the others count as if those were not there."""
+    q, pk, pv, ck, cv, positions = _inputs(40, 8, 2, 64, prefix, slots, dtype)
+    q[..., 0] = 1.0
+    positions.fill_(slots - 1)
+    pk[:, :130, 0] = -math.inf
+    if prefix == 0:
+        ck[:, :, :130, 0] = -math.inf
+    got = glue.prefix_attention(q, pk, pv, ck, cv, positions)
+    if prefix:
+        want, allowed = _want(q, pk[:, 130:], pv[:, 130:], ck, cv, positions)
+    else:
+        want, allowed = _want(q, pk, pv, ck[:, :, 130:], cv[:, :, 130:], positions - 130)
+    assert ((got.double() - want).abs() / allowed).max().item() <= 1.0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_many_small_weights_beside_a_large_one(dtype):
+    """One key of weight 1 and value 0, 2^20 of 2^-26.5 and value 1: the result is what those come to,
+    2^-6.5.  The smallest step of an f16 weight is 2^-24 of 2^-7 of the largest, so each of them is off
+    by 2^-32 at most, and all by 2^-12; in bf16 by half a step, u of each.  The result's own rounding
+    is u of it again, the f32 sums' and the exponential's share 2^-18 as everywhere."""
+    small, count = 2.0 ** -26.5, 2 ** 20
+    pk = torch.zeros(1, count + 1, 64, device="cuda", dtype=dtype)
+    pv = torch.ones(1, count + 1, 64, device="cuda", dtype=dtype)
+    pk[0, 5, 0], pv[0, 5] = 1.0, 0.0
+    q = torch.zeros(3, 1, 64, device="cuda", dtype=dtype)
+    q[..., 0] = 8.0
+    empty = torch.zeros(3, 1, 0, 64, device="cuda", dtype=dtype)
+    # score 8 * scale of the large one: ln 2^26.5, whatever the product's rounding
+    got = glue.prefix_attention(q, pk, pv, empty, empty, torch.full((3,), -1, device="cuda"), scale=26.5 * math.log(2) / 8)
+    want = count * small / (1 + count * small)
+    u = torch.finfo(dtype).eps / 2
+    each = 2.0 ** -32 if dtype == torch.float16 else u * small
+    assert (got.double() - want).abs().max().item() <= count * each + u * want + (2.0 ** -18 + 2 * 18.4 * 2.0 ** -21) * want
