@@ -14,6 +14,9 @@ The package mirrors the pieces of the reference that this hot path consists of:
 * `install`    - makes a process that uses `linnet.torch.load` dispatch to the above
 * `decoder`    - a Llama-3.1-8B-shaped tensor-parallel int4 decoder used for the
                  decode benchmark
+* `glue`       - the kernels of a decode step between the products, and those for many
+                 answers to one prompt (rotary positions, shared-prefix attention, log
+                 probabilities); `rope` makes the rotary frequencies
 
 Every operator calls hand-written CUDA through the C ABI of `include/b200q.h`;
 nothing here falls back to PyTorch arithmetic or to a CPU.

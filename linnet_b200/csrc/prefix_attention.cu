@@ -1036,7 +1036,7 @@ int32_t check_prefix(int64_t batch, int64_t nq, int64_t nkv, int64_t hd, int64_t
     return B200Q_OK;
 }
 
-// A map of boxes of 64 numbers x `rows` x 1 x `last` (keys and values: 128 keys); strides in numbers.
+// A map of boxes of 64 numbers x `rows` x 1 x `last` (keys and values: the keys of a tile); strides in numbers.
 CUresult make_map(EncodeTiled encode, CUtensorMap* map, const void* base, int32_t dtype, int rank, const int64_t* extents,
                   const int64_t* strides, int rows, int last) {
     cuuint64_t dims[4], bytes[3];

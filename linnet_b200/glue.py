@@ -12,13 +12,14 @@ tensors that ask for one."""
 
 from __future__ import annotations
 
-import ctypes
+import functools
+import struct
 from typing import NamedTuple
 
 import torch
 
 from . import _lib, rope
-from .kernels import _CODES, _Device, _raw_stream
+from .kernels import _CODES, _current_device, _raw_stream
 
 
 def _stream(t: torch.Tensor) -> int:
@@ -147,11 +148,11 @@ def silu_mul(gate_up: torch.Tensor) -> torch.Tensor:
 # ---- many answers to one prompt --------------------------------------------------------------
 
 _LAYOUTS = {"half": 0, "interleaved": 1}
-_Strides = ctypes.c_int64 * 12
+_strides_of = struct.Struct("12q").pack
 
 
-def _same(who: str, kinds: tuple[torch.dtype, ...], *tensors: torch.Tensor) -> torch.device:
-    """One CUDA device, one of `kinds`, last dimension contiguous, no derivative asked for."""
+def _same(who: str, kinds: tuple[torch.dtype, ...], *tensors: torch.Tensor) -> int:
+    """One CUDA device (returned), one of `kinds`, last dimension contiguous, no derivative asked for."""
     first = tensors[0]
     index, kind = first.get_device(), first.dtype
     for t in tensors:
@@ -163,7 +164,27 @@ def _same(who: str, kinds: tuple[torch.dtype, ...], *tensors: torch.Tensor) -> t
             raise RuntimeError(f"{who}: the last dimension has to be contiguous")
         if t.requires_grad and torch.is_grad_enabled():
             raise RuntimeError(f"{who} has no derivative: detach its inputs or call it under torch.no_grad()")
-    return first.device
+    return index
+
+
+def _launch(index: int, entry, *args) -> None:
+    """Calls an entry of the library on the device's current stream.  A call of the smallest sizes is
+    bound by its host path: no context manager unless another device is current."""
+    if index == _current_device():
+        status = entry(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = entry(*args, _raw_stream(index))
+    if status:
+        _lib.check(status)
+
+
+def _words(who: str, name: str, words: torch.Tensor, count: int, index: int) -> None:
+    """Read on the device as int64: anything else would be misread."""
+    if (words.get_device() != index or words.dtype is not torch.int64 or words.numel() != count
+            or not words.is_contiguous()):
+        raise ValueError(f"{who}: {name} must be a contiguous int64 tensor of {count} entries on cuda:{index}, not "
+                         f"{words.dtype}{list(words.shape)} on {words.device}")
 
 
 _HALF = (torch.bfloat16, torch.float16)
@@ -176,13 +197,14 @@ def _contiguous(who: str, *tensors: torch.Tensor) -> None:
             raise RuntimeError(f"{who} takes contiguous caches and projections")
 
 
-def _frequencies(who: str, frequencies: torch.Tensor, head_dim: int, device: torch.device) -> int:
+def _frequencies(who: str, frequencies: torch.Tensor, head_dim: int, index: int) -> int:
     """Read on the device as f64: anything else would be misread."""
-    if (frequencies.device != device or frequencies.dtype != torch.float64 or not frequencies.is_contiguous()
-            or frequencies.dim() != 1 or not 1 <= frequencies.numel() <= head_dim // 2):
+    pairs = frequencies.numel()
+    if (frequencies.get_device() != index or frequencies.dtype is not torch.float64 or not frequencies.is_contiguous()
+            or frequencies.dim() != 1 or not 1 <= pairs <= head_dim // 2):
         raise ValueError(f"{who}: frequencies must be a contiguous float64 tensor of 1 to {head_dim // 2} entries on "
-                         f"{device}, not {frequencies.dtype}{list(frequencies.shape)} on {frequencies.device}")
-    return frequencies.numel()
+                         f"cuda:{index}, not {frequencies.dtype}{list(frequencies.shape)} on {frequencies.device}")
+    return pairs
 
 
 def _layout(who: str, layout: str) -> int:
@@ -191,13 +213,11 @@ def _layout(who: str, layout: str) -> int:
     return _LAYOUTS[layout]
 
 
-def _word(who: str, name: str, value: "int | torch.Tensor", device: torch.device) -> tuple[int | None, int]:
+def _word(who: str, name: str, value: "int | torch.Tensor", index: int) -> tuple[int | None, int]:
     """A number known on the host, or one int64 word on the device: (address or None, number)."""
     if not isinstance(value, torch.Tensor):
         return None, int(value)
-    if value.device != device or value.dtype != torch.int64 or value.numel() != 1:
-        raise ValueError(f"{who}: {name} must be a number or one int64 on {device}, not "
-                         f"{value.dtype}{list(value.shape)} on {value.device}")
+    _words(who, name, value, 1, index)
     return value.data_ptr(), 0
 
 
@@ -218,14 +238,15 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, fre
     positions[t] * frequencies[pair] and multiplied by `factor`; the others are copied.  `out`: where
     the results go, (q, k) themselves to turn in place; other overlaps are not allowed."""
     tensors = (q,) if k is None else (q, k)
-    device = _same("rotary", _HALF, *tensors)
+    index = _same("rotary", _HALF, *tensors)
     if q.dim() != 3 or (k is not None and (k.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2])):
         raise ValueError(f"rotary: q is [tokens, heads, D] and k the same, not {[list(t.shape) for t in tensors]}")
     tokens, nq, hd = q.shape
-    _positions(positions, tokens, device)
-    pairs = _frequencies("rotary", frequencies, hd, device)
+    _words("rotary", "positions", positions, tokens, index)
+    pairs = _frequencies("rotary", frequencies, hd, index)
     code = _layout("rotary", layout)
     if out is None:
+        device = q.device
         q_out, k_out = torch.empty(tokens, nq, hd, dtype=q.dtype, device=device), None
         if k is not None:
             k_out = torch.empty(tokens, k.shape[1], hd, dtype=k.dtype, device=device)
@@ -238,11 +259,10 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, fre
     keys, k_from, k_to, nkv, at = None, q_from, q_to, 0, None
     if k is not None:
         keys, k_from, k_to, nkv, at = k.data_ptr(), k.stride(), k_out.stride(), k.shape[1], k_out.data_ptr()
-    with _Device(device):
-        _lib.check(_lib.load().b200q_rotary(
+    _launch(index, _lib.load().b200q_rotary,
             q.data_ptr(), keys, positions.data_ptr(), frequencies.data_ptr(), q_out.data_ptr(), at, tokens, nq, nkv, hd,
             pairs, q_from[0], q_from[1], k_from[0], k_from[1], q_to[0], q_to[1], k_to[0], k_to[1], factor, code,
-            _CODES[q.dtype], _raw_stream(device.index)))
+            _CODES[q.dtype])
     return q_out, k_out
 
 
@@ -254,39 +274,44 @@ def rotary_cache(qkv: torch.Tensor, positions: torch.Tensor, frequencies: torch.
     [B, nkv, S, D] at slot positions[b] and returns q [B, nq, D].  `offset` (a number, or one int64 on
     the device) is where a row's own cache begins: the length of the prefix it shares.  A position
     outside the cache stores nothing and is reported by `decoder_status`."""
-    device = _same("rotary_cache", _HALF, qkv, cache_k, cache_v)
+    index = _same("rotary_cache", _HALF, qkv, cache_k, cache_v)
     _contiguous("rotary_cache", qkv, cache_k, cache_v)
-    batch = qkv.shape[0]
-    if (cache_k.dim() != 4 or cache_k.shape != cache_v.shape or cache_k.shape[:2] != (batch, nkv)
-            or qkv.shape != (batch, (nq + 2 * nkv) * cache_k.shape[3])):
+    shape = cache_k.shape
+    batch, _, max_seq, hd = shape if len(shape) == 4 else (-1, -1, -1, -1)
+    if shape != cache_v.shape or shape != (batch, nkv, max_seq, hd) or qkv.shape != (batch, (nq + 2 * nkv) * hd):
         raise ValueError(f"rotary_cache: qkv {list(qkv.shape)} of {nq} and {nkv} heads and caches "
                          f"{list(cache_k.shape)}, {list(cache_v.shape)} do not go together")
-    _positions(positions, batch, device)
-    _, _, max_seq, hd = cache_k.shape
-    pairs = _frequencies("rotary_cache", frequencies, hd, device)
+    _words("rotary_cache", "positions", positions, batch, index)
+    pairs = _frequencies("rotary_cache", frequencies, hd, index)
     code = _layout("rotary_cache", layout)
-    at, number = _word("rotary_cache", "offset", offset, device)
-    q = torch.empty(batch, nq, hd, device=device, dtype=qkv.dtype)
-    with _Device(device):
-        _lib.check(_lib.load().b200q_rotary_cache(
+    at, number = _word("rotary_cache", "offset", offset, index)
+    q = torch.empty(batch, nq, hd, device=qkv.device, dtype=qkv.dtype)
+    _launch(index, _lib.load().b200q_rotary_cache,
             qkv.data_ptr(), positions.data_ptr(), frequencies.data_ptr(), at, number, q.data_ptr(), cache_k.data_ptr(),
-            cache_v.data_ptr(), batch, nq, nkv, hd, pairs, max_seq, factor, code, _CODES[qkv.dtype],
-            _raw_stream(device.index)))
+            cache_v.data_ptr(), batch, nq, nkv, hd, pairs, max_seq, factor, code, _CODES[qkv.dtype])
     return q
 
 
 def rotary_table(max_seq: int, frequencies: torch.Tensor, factor: float = 1.0) -> torch.Tensor:
     """(cos, sin) * factor of positions 0 .. max_seq - 1, f32 [max_seq, len(frequencies), 2]: what
     `rope_attention` takes, for frequencies of any scaling (of whole heads, halves turned)."""
-    device = frequencies.device
-    if device.type != "cuda" or max_seq < 1:
-        raise ValueError(f"rotary_table: {max_seq} positions, frequencies on {device}")
-    pairs = _frequencies("rotary_table", frequencies, 1024, device)
-    table = torch.empty(max_seq, pairs, 2, dtype=torch.float32, device=device)
-    with _Device(device):
-        _lib.check(_lib.load().b200q_rotary_table(table.data_ptr(), frequencies.data_ptr(), max_seq, pairs, factor,
-                                                  _raw_stream(device.index)))
+    if not frequencies.is_cuda or max_seq < 1:
+        raise ValueError(f"rotary_table: {max_seq} positions, frequencies on {frequencies.device}")
+    index = frequencies.get_device()
+    pairs = _frequencies("rotary_table", frequencies, 1024, index)
+    table = torch.empty(max_seq, pairs, 2, dtype=torch.float32, device=frequencies.device)
+    _launch(index, _lib.load().b200q_rotary_table, table.data_ptr(), frequencies.data_ptr(), max_seq, pairs, factor)
     return table
+
+
+@functools.lru_cache(maxsize=256)
+def _prefix_scratch(index: int, batch: int, nq: int, nkv: int, head_dim: int, prefix: int, max_seq: int) -> int:
+    """Bytes of scratch memory; of the sizes alone (and the device's multiprocessors)."""
+    with torch.cuda.device(index):
+        size = _lib.load().b200q_prefix_attention_scratch_bytes(batch, nq, nkv, head_dim, prefix, max_seq)
+    if size < 0:
+        raise ValueError(_lib.last_error())
+    return size
 
 
 def prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor, cache_k: torch.Tensor,
@@ -299,35 +324,30 @@ def prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Te
     counts as that and is reported by `decoder_status`.  `prefix_length`: one int64 on the device, how
     many of the P positions there are (a captured step can be replayed on another prompt).  The last
     dimension is contiguous, other strides are multiples of 8 numbers (parts of longer caches)."""
-    device = _same("prefix_attention", _HALF, q, prefix_k, prefix_v, cache_k, cache_v)
-    if (q.dim() != 3 or prefix_k.dim() != 3 or cache_k.dim() != 4 or prefix_k.shape != prefix_v.shape
-            or cache_k.shape != cache_v.shape or cache_k.shape[:2] != (q.shape[0], prefix_k.shape[0])
-            or not q.shape[2] == prefix_k.shape[2] == cache_k.shape[3]):
-        raise ValueError(f"prefix_attention: q {list(q.shape)}, a prefix {list(prefix_k.shape)}, {list(prefix_v.shape)} and "
-                         f"caches {list(cache_k.shape)}, {list(cache_v.shape)} do not go together")
-    batch, nq, hd = q.shape
-    nkv, prefix = prefix_k.shape[:2]
-    _positions(positions, batch, device)
+    index = _same("prefix_attention", _HALF, q, prefix_k, prefix_v, cache_k, cache_v)
+    shape, shared, own = q.shape, prefix_k.shape, cache_k.shape
+    batch, nq, hd = shape if len(shape) == 3 else (-1, -1, -1)
+    nkv, prefix = shared[:2] if len(shared) == 3 else (-1, -1)
+    if (batch < 0 or shared != (nkv, prefix, hd) or shared != prefix_v.shape or len(own) != 4 or own != cache_v.shape
+            or own[0] != batch or own[1] != nkv or own[3] != hd):
+        raise ValueError(f"prefix_attention: q {list(shape)}, a prefix {list(shared)}, {list(prefix_v.shape)} and "
+                         f"caches {list(own)}, {list(cache_v.shape)} do not go together")
+    _words("prefix_attention", "positions", positions, batch, index)
     at = None
     if prefix_length is not None:
-        at, _ = _word("prefix_attention", "prefix_length", prefix_length, device)
-        if at is None:
+        if not isinstance(prefix_length, torch.Tensor):
             raise ValueError("prefix_attention: prefix_length is one int64 on the device (or cut the prefix to its length)")
+        at, _ = _word("prefix_attention", "prefix_length", prefix_length, index)
     pk, pv, ck, cv = prefix_k.stride(), prefix_v.stride(), cache_k.stride(), cache_v.stride()
     steps = q.stride()
-    strides = _Strides(steps[0], steps[1], pk[1], pk[0], pv[1], pv[0], ck[2], ck[1], ck[0], cv[2], cv[1], cv[0])
-    lib = _lib.load()
-    with _Device(device):
-        size = lib.b200q_prefix_attention_scratch_bytes(batch, nq, nkv, hd, prefix, cache_k.shape[2])
-        if size < 0:
-            raise ValueError(_lib.last_error())
-        scratch = torch.empty(size, dtype=torch.uint8, device=device)
-        out = torch.empty(batch, nq * hd, dtype=q.dtype, device=device)
-        _lib.check(lib.b200q_prefix_attention(
+    strides = _strides_of(steps[0], steps[1], pk[1], pk[0], pv[1], pv[0], ck[2], ck[1], ck[0], cv[2], cv[1], cv[0])
+    device, kind = q.device, q.dtype
+    scratch = torch.empty(_prefix_scratch(index, batch, nq, nkv, hd, prefix, own[2]), dtype=torch.uint8, device=device)
+    out = torch.empty(batch, nq * hd, dtype=kind, device=device)
+    _launch(index, _lib.load().b200q_prefix_attention,
             q.data_ptr(), prefix_k.data_ptr(), prefix_v.data_ptr(), cache_k.data_ptr(), cache_v.data_ptr(),
-            positions.data_ptr(), at, out.data_ptr(), scratch.data_ptr(), batch, nq, nkv, hd, prefix, cache_k.shape[2],
-            strides, hd ** -0.5 if scale is None else scale, _CODES[q.dtype],
-            _raw_stream(device.index)))
+            positions.data_ptr(), at, out.data_ptr(), scratch.data_ptr(), batch, nq, nkv, hd, prefix, own[2],
+            strides, hd ** -0.5 if scale is None else scale, _CODES[kind])
     return out
 
 
@@ -344,19 +364,19 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     Logits are f32, bf16 or f16, rows at any stride; -inf is a forbidden token.  A negative token
     stands for none (log probability 0: padded rows drop out of sums); one past the vocabulary gives
     NaN and is reported by `decoder_status`."""
-    device = _same("token_logprobs", _LOGITS, logits)
-    if logits.dim() != 2 or not 0 < logits.shape[1]:
-        raise ValueError(f"token_logprobs: logits are [rows, vocab], not {list(logits.shape)}")
-    rows, vocab = logits.shape
-    if (tokens.device != device or tokens.dtype != torch.int64 or tokens.shape != (rows,) or not tokens.is_contiguous()):
-        raise ValueError(f"token_logprobs: tokens must be a contiguous int64 tensor of {rows} entries on {device}, not "
-                         f"{tokens.dtype}{list(tokens.shape)} on {tokens.device}")
-    kept = max(top, 0)
+    index = _same("token_logprobs", _LOGITS, logits)
+    shape = logits.shape
+    if len(shape) != 2 or not 0 < shape[1]:
+        raise ValueError(f"token_logprobs: logits are [rows, vocab], not {list(shape)}")
+    rows, vocab = shape
+    if tokens.dim() != 1:
+        raise ValueError(f"token_logprobs: tokens must be an int64 tensor [rows], not {tokens.dtype}{list(tokens.shape)}")
+    _words("token_logprobs", "tokens", tokens, rows, index)
+    kept, device = max(top, 0), logits.device
     logprob, entropy = torch.empty(2, rows, dtype=torch.float32, device=device).unbind()
     best = torch.empty(rows, kept, dtype=torch.float32, device=device)
-    index = torch.empty(rows, kept, dtype=torch.int64, device=device)
-    with _Device(device):
-        _lib.check(_lib.load().b200q_token_logprobs(
+    best_tokens = torch.empty(rows, kept, dtype=torch.int64, device=device)
+    _launch(index, _lib.load().b200q_token_logprobs,
             logits.data_ptr(), tokens.data_ptr(), logprob.data_ptr(), entropy.data_ptr(), best.data_ptr(),
-            index.data_ptr(), rows, vocab, logits.stride(0), top, _CODES[logits.dtype], _raw_stream(device.index)))
-    return TokenLogprobs(logprob, entropy, best, index)
+            best_tokens.data_ptr(), rows, vocab, logits.stride(0), top, _CODES[logits.dtype])
+    return TokenLogprobs(logprob, entropy, best, best_tokens)
