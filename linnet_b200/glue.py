@@ -373,7 +373,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
         raise ValueError(f"token_logprobs: tokens must be an int64 tensor [rows], not {tokens.dtype}{list(tokens.shape)}")
     _words("token_logprobs", "tokens", tokens, rows, index)
     kept, device = max(top, 0), logits.device
-    logprob, entropy = torch.empty(2, rows, dtype=torch.float32, device=device).unbind()
+    logprob = torch.empty(rows, dtype=torch.float32, device=device)
+    entropy = torch.empty(rows, dtype=torch.float32, device=device)
     best = torch.empty(rows, kept, dtype=torch.float32, device=device)
     best_tokens = torch.empty(rows, kept, dtype=torch.int64, device=device)
     _launch(index, _lib.load().b200q_token_logprobs,
