@@ -337,7 +337,7 @@ int32_t b200q_rotary_table(void* table, const double* frequencies, int64_t max_s
  *   positions: -1 where a row has no keys of its own; a row without any key gives zeros.  A
  *     position outside -1 .. max_seq-1 counts as -1 and is recorded for b200q_decoder_status(); a
  *     prefix length outside 0 .. prefix counts as the nearer end and is recorded as row 0.
- *   strides: HOST array of 12, in numbers, multiples of 8: q's rows and heads; keys and heads of
+ *   strides: HOST array of 12, in numbers, positive multiples of 8: q's rows and heads; keys and heads of
  *     prefix_k, of prefix_v; keys, heads and rows of cache_k, of cache_v (of a dimension of one or
  *     none they are not read).
  *   scratch: device memory of b200q_prefix_attention_scratch_bytes(...) bytes (-1: a shape that is

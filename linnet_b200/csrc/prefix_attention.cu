@@ -1095,7 +1095,7 @@ extern "C" int32_t b200q_prefix_attention(const void* q, const void* prefix_k, c
                   "prefix_attention: tensors must be 16-byte aligned (positions and the prefix length: int64)");
     const int64_t extents[12] = {batch, nq, prefix, nkv, prefix, nkv, max_seq, nkv, batch, max_seq, nkv, batch};
     for (int i = 0; i < 12; ++i)
-        B200Q_REQUIRE(extents[i] <= 1 || (strides[i] % 8 == 0 && strides[i] >= 0),
+        B200Q_REQUIRE(extents[i] <= 1 || (strides[i] % 8 == 0 && strides[i] > 0),
                       "prefix_attention: strides must be whole 16-byte steps");
     EncodeTiled encode = encode_tiled();
     if (encode == nullptr) return unavailable("prefix_attention: the driver has no cuTensorMapEncodeTiled");

@@ -13,6 +13,7 @@ tensors that ask for one."""
 from __future__ import annotations
 
 import functools
+import operator
 import struct
 from typing import NamedTuple
 
@@ -216,7 +217,7 @@ def _layout(who: str, layout: str) -> int:
 def _word(who: str, name: str, value: "int | torch.Tensor", index: int) -> tuple[int | None, int]:
     """A number known on the host, or one int64 word on the device: (address or None, number)."""
     if not isinstance(value, torch.Tensor):
-        return None, int(value)
+        return None, operator.index(value)
     _words(who, name, value, 1, index)
     return value.data_ptr(), 0
 
@@ -323,7 +324,7 @@ def prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Te
     positive number, is D**-0.5 unless given.  A position of -1 is a row without keys of its own; one outside the cache
     counts as that and is reported by `decoder_status`.  `prefix_length`: one int64 on the device, how
     many of the P positions there are (a captured step can be replayed on another prompt).  The last
-    dimension is contiguous, other strides are multiples of 8 numbers (parts of longer caches)."""
+    dimension is contiguous, other strides are positive multiples of 8 numbers (parts of longer caches)."""
     index = _same("prefix_attention", _HALF, q, prefix_k, prefix_v, cache_k, cache_v)
     shape, shared, own = q.shape, prefix_k.shape, cache_k.shape
     batch, nq, hd = shape if len(shape) == 3 else (-1, -1, -1)

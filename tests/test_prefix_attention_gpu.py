@@ -272,3 +272,29 @@ def test_many_small_weights_beside_a_large_one(dtype):
     u = torch.finfo(dtype).eps / 2
     each = 2.0 ** -32 if dtype == torch.float16 else u * small
     assert (got.double() - want).abs().max().item() <= count * each + u * want + (2.0 ** -18 + 2 * 18.4 * 2.0 ** -21) * want
+
+
+def test_no_keys_at_all_and_repeated_memory():
+    q, pk, pv, ck, cv, positions = _inputs(5, 8, 2, 128, 0, 0, torch.bfloat16)
+    assert bool((glue.prefix_attention(q, pk, pv, ck, cv, positions) == 0).all())
+    q, pk, pv, ck, cv, positions = _inputs(5, 8, 2, 128, 100, 30, torch.bfloat16)
+    once = ck[:1].expand(5, -1, -1, -1)  # every row's cache the same memory: a stride of 0
+    with pytest.raises(ValueError, match="strides"):
+        glue.prefix_attention(q, pk, pv, once, cv, positions)
+    # of a dimension of one the stride is not read, whatever it is
+    got = glue.prefix_attention(q[:1], pk, pv, ck[:1].as_strided(ck[:1].shape, (3, *ck.stride()[1:])), cv[:1], positions[:1])
+    assert torch.equal(got, glue.prefix_attention(q[:1], pk, pv, ck[:1], cv[:1], positions[:1]))
+
+
+def test_more_pieces_than_16_bits_count():
+    """65536 rows of 300 KV heads, one key each: 66419 pieces a group of each of 148 blocks.  With one
+    key its weight is 1 and the result its value."""
+    batch, heads = 65536, 300
+    q = torch.zeros(batch, heads, 64, device="cuda", dtype=torch.bfloat16)
+    ck = torch.zeros(batch, heads, 1, 64, device="cuda", dtype=torch.bfloat16)
+    cv = torch.empty_like(ck).normal_()
+    none = torch.zeros(heads, 0, 64, device="cuda", dtype=torch.bfloat16)
+    got = glue.prefix_attention(q, none, none, ck, cv, torch.zeros(batch, dtype=torch.long, device="cuda"))
+    assert torch.equal(got, cv.view(batch, heads * 64))
+    del q, ck, cv, got
+    torch.cuda.empty_cache()

@@ -217,3 +217,23 @@ def test_rotary_refusals():
         glue.rotary_cache(x.view(2, 256), at, freq, cache[:, :, :4], cache[:, :, :4], 2, 1)
     with pytest.raises(ValueError, match="offset"):
         glue.rotary_cache(x.view(2, 256), at, freq, cache, cache, 2, 1, offset=torch.zeros(2, dtype=torch.int64, device="cuda"))
+
+
+def test_keys_of_no_heads_offsets_that_are_no_whole_numbers_and_views_in_place():
+    q = torch.randn(3, 4, 64, device="cuda").to(torch.bfloat16)
+    positions = torch.arange(3, device="cuda")
+    frequencies, _ = glue.rope_frequencies(64, 1e4)
+    alone, none = glue.rotary(q, None, positions, frequencies)
+    both, empty = glue.rotary(q, q[:, :0], positions, frequencies)
+    assert none is None and empty.shape == (3, 0, 64) and torch.equal(alone, both)
+    # q and k are views of one projection, turned where they are; v between them stays
+    fused = torch.randn(3, 4 + 2 + 2, 64, device="cuda").to(torch.bfloat16)
+    before = fused.clone()
+    want = glue.rotary(before[:, :4], before[:, 6:], positions, frequencies)
+    glue.rotary(fused[:, :4], fused[:, 6:], positions, frequencies, out=(fused[:, :4], fused[:, 6:]))
+    assert torch.equal(fused[:, :4], want[0]) and torch.equal(fused[:, 6:], want[1])
+    assert torch.equal(fused[:, 4:6], before[:, 4:6])
+    cache = torch.zeros(3, 1, 8, 64, device="cuda", dtype=torch.bfloat16)
+    qkv = torch.randn(3, 3 * 64, device="cuda").to(torch.bfloat16)
+    with pytest.raises(TypeError):
+        glue.rotary_cache(qkv, positions, frequencies, cache, cache.clone(), 1, 1, offset=1.5)
