@@ -17,7 +17,7 @@
 // (by bisection over the floats' order where the first guess has too many), reads those groups once
 // more and ranks what reaches it.
 //
-// Measured on a B200, rows of 128256: 2048 of bf16 with 5 alternatives 107 us, 4.9 TB/s (92 without:
+// Measured on a B200, rows of 128256: 2048 of bf16 with 5 alternatives 103 us, 5.1 TB/s (92 without:
 // 5.7 TB/s); 64 of f32 15.8 us, 2.1 TB/s; one of bf16 with 20 alternatives 9.9 us, most of it the way
 // from the last logit over the cluster's barrier to the ranked list.
 #include <cooperative_groups.h>
@@ -164,8 +164,11 @@ __device__ __forceinline__ void add(const float (&x)[E], float m, float2& l, flo
     }
 }
 
+// (16-bit logits with alternatives: told of four blocks a multiprocessor, the compiler takes 62 registers instead of 58,
+// which four blocks fit in as well: 107 -> 103 us for 2048 rows with five.  The other forms are left to it: told of
+// one, it takes 60 registers instead of 40 for f32, and 64 rows 21.6 us instead of 15.8.)
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, TOP && sizeof(T) == 2 ? 4 : 0)
 token_logprobs_kernel(const __grid_constant__ LogprobArgs a) {
     constexpr int E = Logit<T>::E;
     extern __shared__ float group_max[];  // this block's groups; in the first block, behind them, all of the row's
