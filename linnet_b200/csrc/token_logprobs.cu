@@ -13,13 +13,13 @@
 // The alternatives cost the pass one reduction a group: its largest logit, kept in shared memory.
 // The `top` first logits, larger ones first and the lower index first among equals, lie in the `top`
 // first groups by (largest logit, index), since each group ahead of an element's own holds an
-// element ahead of it.  So the first block finds a threshold that `top` groups reach and not many more
-// (by bisection over the floats' order where the first guess has too many), reads those groups once
-// more and ranks what reaches it.
+// element ahead of it.  So the first block, whose memory the others of the cluster store their groups'
+// to, finds a threshold that `top` groups reach and not many more (by bisection over the floats' order
+// where the first guess has too many), reads those groups once more and ranks what reaches it.
 //
-// Measured on a B200, rows of 128256: 2048 of bf16 with 5 alternatives 103 us, 5.1 TB/s (92 without:
-// 5.7 TB/s); 64 of f32 15.8 us, 2.1 TB/s; one of bf16 with 20 alternatives 9.9 us, most of it the way
-// from the last logit over the cluster's barrier to the ranked list.
+// Measured on a B200, rows of 128256: 2048 of bf16 with 5 alternatives 102 us, 5.1 TB/s (92 without:
+// 5.7 TB/s), of f32 162 us, 6.5 TB/s; 64 of f32 12.4 us; one of bf16 with 20 alternatives 8.9 us, half of
+// it the way from the last logit over the cluster's barrier to the ranked list.
 #include <cooperative_groups.h>
 
 #include "mma.cuh"
@@ -164,24 +164,27 @@ __device__ __forceinline__ void add(const float (&x)[E], float m, float2& l, flo
     }
 }
 
-// (16-bit logits with alternatives: told of four blocks a multiprocessor, the compiler takes 62 registers instead of 58,
-// which four blocks fit in as well: 107 -> 103 us for 2048 rows with five.  The other forms are left to it: told of
-// one, it takes 60 registers instead of 40 for f32, and 64 rows 21.6 us instead of 15.8.)
+// With alternatives, five blocks a multiprocessor: one's ranking goes by while the others read.  2048 rows with five:
+// 102 us so, 106 with four, 120 with three, 142 with six (of 40 registers, with spills); f32 162, 173, 184, 175.
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads, TOP && sizeof(T) == 2 ? 4 : 0)
+__global__ void __launch_bounds__(kThreads, TOP ? 5 : 0)
 token_logprobs_kernel(const __grid_constant__ LogprobArgs a) {
     constexpr int E = Logit<T>::E;
-    extern __shared__ float group_max[];  // this block's groups; in the first block, behind them, all of the row's
-    __shared__ Sums warp_sums[kWarps], block_sums;
+    extern __shared__ float group_max[];  // of the row's groups, in the first block
+    __shared__ Sums warp_sums[kWarps], block_sums[8];  // the cluster's, in its first block
     __shared__ double row_max, row_log;  // m and ln l: their sum would lose the second where logits are huge
     __shared__ int picked[kPicked];
     __shared__ uint64_t ranked[kRanked];
-    __shared__ uint32_t threshold;
-    __shared__ int picked_count, ranked_count, reached, in_order;  // in_order: the picked groups are, by index
-    pdl_launch_dependents();
-    pdl_wait();
+    __shared__ uint32_t threshold, class_max[32];
+    __shared__ int picked_count, ranked_count, reached;
     cg::cluster_group cluster = cg::this_cluster();
     const int blocks = int(cluster.num_blocks()), rank = int(cluster.block_rank()), row = int(blockIdx.x) / blocks;
+    // (the first block has started when the others store to its memory)
+    if (blocks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    pdl_launch_dependents();
+    pdl_wait();
+    if (blocks > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    float* const all_max = blocks > 1 ? cluster.map_shared_rank(group_max, 0) : group_max;
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     const Row<T> logits(a, row);
     // groups of this row (a row that starts past a boundary may have one more than others), divided evenly
@@ -210,7 +213,7 @@ token_logprobs_kernel(const __grid_constant__ LogprobArgs a) {
                 asm volatile("redux.sync.max.f32 %0, %1, 0xFFFFFFFF;" : "=f"(peak_all) : "f"(peak[u]));
                 if (lane == u) peak[0] = peak_all;
             }
-            if (lane < kept) group_max[g0 + lane - first] = peak[0];
+            if (lane < kept) all_max[g0 + lane] = peak[0];
         }
     };
     // Groups without an edge of the row, kHeld at a time; what is left of them, and the edges, after that.
@@ -252,6 +255,7 @@ token_logprobs_kernel(const __grid_constant__ LogprobArgs a) {
     }
     if (lane == 0) warp_sums[warp] = mine;
     if (threadIdx.x == 0) ranked_count = picked_count = 0;
+    if (threadIdx.x < 32) class_max[threadIdx.x] = 0;
     __syncthreads();
     auto join_lanes = [&](int count) {  // the sums of the first `count` lanes (a power of two), in lane 0
         for (int d = count / 2; d >= 1; d >>= 1) {
@@ -263,28 +267,16 @@ token_logprobs_kernel(const __grid_constant__ LogprobArgs a) {
     if (warp == kWarps - 1) {
         mine = warp_sums[lane % kWarps];
         join_lanes(kWarps);
-        if (lane == 0) block_sums = mine;
+        if (blocks > 1 && lane == 0) cluster.map_shared_rank(block_sums, 0)[rank] = mine;
     }
-    float* all_max = group_max;
-    if (blocks > 1) {
-        cluster.sync();  // every block's sums and groups are in its shared memory
-        if (rank == 0 && warp == kWarps - 1) {
-            mine = *cluster.map_shared_rank(&block_sums, lane % blocks);
-            join_lanes(blocks);
-        }
-        if (TOP && rank == 0) {
-            all_max = group_max + (groups + blocks - 1) / blocks;
-            for (int g = threadIdx.x; g < groups; g += kThreads) {
-                const int r = int(((int64_t(g) + 1) * blocks - 1) / groups), from = int(int64_t(groups) * r / blocks);
-                all_max[g] = cluster.map_shared_rank(group_max, r)[g - from];
-            }
-        }
-        cluster.sync();  // the others' shared memory is no longer read
-    } else {
-        __syncthreads();
-    }
+    if (blocks > 1) cluster.sync();  // every block's sums and groups are in the first one's memory
+    else __syncthreads();
     if (rank != 0) return;
-    if (threadIdx.x == (kWarps - 1) * 32) {  // (the first warp has the alternatives to look for)
+    if (blocks > 1 && warp == kWarps - 1) {
+        mine = block_sums[lane % blocks];
+        join_lanes(blocks);
+    }
+    if (threadIdx.x == (kWarps - 1) * 32) {
         const double most = double(mine.m), norm = log(double(mine.l));
         row_max = most, row_log = norm;
         const int64_t token = ld_mutable(a.tokens + row);
@@ -302,51 +294,59 @@ token_logprobs_kernel(const __grid_constant__ LogprobArgs a) {
 
     // ---- the groups that are read again: those above `low` ----
     const int top = a.top;
-    if (warp == 0) {
-        // Each lane's largest of every 32nd group: the top-th of the lanes' is reached by `top` groups at least,
-        // and seldom by many more.
-        uint32_t best = 0;
-        for (int g = lane; g < groups; g += 32) best = max(best, order_of(all_max[g]));
-        int ahead = 0;
+    // The largest of every 32nd group, 32 of them: the top-th of those is reached by `top` groups at least, and seldom by
+    // many more.
+    uint32_t best = 0, low;
+    for (int g = threadIdx.x; g < groups; g += kThreads) best = max(best, order_of(group_max[g]));
+    atomicMax(&class_max[lane], best);
+    __syncthreads();
+    best = class_max[lane];
+    int others = 0;
 #pragma unroll
-        for (int other = 0; other < 32; ++other) {
-            const uint32_t theirs = __shfl_sync(0xFFFFFFFFu, best, other);
-            ahead += theirs > best || (theirs == best && other < lane);
-        }
-        const uint32_t reached_by_top = __shfl_sync(0xFFFFFFFFu, best, __ffs(__ballot_sync(0xFFFFFFFFu, ahead == top - 1)) - 1);
-        int reach = 0;
-        for (int g = lane; g < groups; g += 32) reach += order_of(all_max[g]) >= reached_by_top;
-        reach = __reduce_add_sync(0xFFFFFFFFu, reach);
-        const bool few = groups >= 32 && reach <= kPicked;
-        if (few) {
-            if (lane == 0) threshold = reached_by_top - 1, in_order = 0;
-        } else {
+    for (int other = 0; other < 32; ++other) {
+        const uint32_t theirs = __shfl_sync(0xFFFFFFFFu, best, other);
+        others += theirs > best || (theirs == best && other < lane);
+    }
+    const uint32_t reached_by_top = __shfl_sync(0xFFFFFFFFu, best, __ffs(__ballot_sync(0xFFFFFFFFu, others == top - 1)) - 1);
+    low = reached_by_top - 1;
+    if (groups >= 32)
+        for (int g = threadIdx.x; g < groups; g += kThreads)
+            if (order_of(group_max[g]) > low) {
+                const int i = atomicAdd(&picked_count, 1);
+                if (i < kPicked) picked[i] = g;
+            }
+    __syncthreads();
+    const bool in_order = groups < 32 || picked_count > kPicked;  // the picked groups are, by index
+    if (in_order) {
+        __syncthreads();
+        if (warp == 0) {
             // low: at least min(top, groups) groups reach it; high: fewer do
             uint32_t least = 0xFFFFFFFFu, most = 0;
             for (int g = lane; g < groups; g += 32) {
-                const uint32_t k = order_of(all_max[g]);
+                const uint32_t k = order_of(group_max[g]);
                 least = min(least, k), most = max(most, k);
             }
             least = __reduce_min_sync(0xFFFFFFFFu, least), most = __reduce_max_sync(0xFFFFFFFFu, most);
-            uint32_t low = least, high = most + 1;
-            reach = groups;
+            low = least;
+            uint32_t high = most + 1;
+            int reach = groups;
             if (groups <= top) low = 0;
             while (groups > top && reach > kPicked && high - low > 1) {
                 const uint32_t mid = low + (high - low) / 2;
                 int c = 0;
-                for (int g = lane; g < groups; g += 32) c += order_of(all_max[g]) >= mid;
+                for (int g = lane; g < groups; g += 32) c += order_of(group_max[g]) >= mid;
                 c = __reduce_add_sync(0xFFFFFFFFu, c);
                 if (c >= top) low = mid, reach = c;
                 else high = mid;
             }
             // All groups above `low`; of those that just reach it as many as there is room for, the first ones.
             int above = 0;
-            for (int g = lane; g < groups; g += 32) above += order_of(all_max[g]) > low;
+            for (int g = lane; g < groups; g += 32) above += order_of(group_max[g]) > low;
             above = __reduce_add_sync(0xFFFFFFFFu, above);
             int room = kPicked - above, n = 0;
             for (int g0 = 0; g0 < groups; g0 += 32) {
                 const int g = g0 + lane;
-                const uint32_t k = g < groups ? order_of(all_max[g]) : 0;
+                const uint32_t k = g < groups ? order_of(group_max[g]) : 0;
                 const bool just = g < groups && k == low;
                 const uint32_t ties = __ballot_sync(0xFFFFFFFFu, just);
                 const bool take = (g < groups && k > low) || (just && __popc(ties & ((1u << lane) - 1)) < room);
@@ -355,15 +355,10 @@ token_logprobs_kernel(const __grid_constant__ LogprobArgs a) {
                 n += __popc(taken);
                 room -= min(room, __popc(ties));
             }
-            if (lane == 0) picked_count = n, threshold = low, in_order = 1;
+            if (lane == 0) picked_count = n, threshold = low;
         }
-    }
-    __syncthreads();
-    if (!in_order) {
-        const uint32_t above = threshold;
-        for (int g = threadIdx.x; g < groups; g += kThreads)
-            if (order_of(all_max[g]) > above) picked[atomicAdd(&picked_count, 1)] = g;
         __syncthreads();
+        low = threshold;
     }
 
     // Calls `f(order, element)` for every element of the picked groups; one warp a group.
@@ -393,7 +388,6 @@ token_logprobs_kernel(const __grid_constant__ LogprobArgs a) {
         });
         __syncthreads();
     };
-    uint32_t low = threshold;
     collect(low);
     if (ranked_count > kRanked) {  // many above a threshold made for groups: bisect over the elements
         if (!in_order) {           // (ties at the end of that go by index)
@@ -480,8 +474,7 @@ token_logprobs_kernel(const __grid_constant__ LogprobArgs a) {
 
 template <typename T, bool TOP>
 cudaError_t launch(const LogprobArgs& a, int rows, int blocks, cudaStream_t stream) {
-    // this block's groups, and in the first block of several all of the row's as well
-    const size_t smem = TOP ? sizeof(float) * size_t(blocks > 1 ? (a.groups + blocks - 1) / blocks + a.groups : a.groups) : 0;
+    const size_t smem = TOP ? sizeof(float) * size_t(a.groups) : 0;
     auto kernel = token_logprobs_kernel<T, TOP>;
     cudaError_t err = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
     if (err != cudaSuccess) return err;
@@ -528,7 +521,7 @@ extern "C" int32_t b200q_token_logprobs(const void* logits, const int64_t* token
     a.groups = int((vocab + elements - 1 + 32 * elements - 1) / (32 * elements));  // of a row wherever it starts
     a.status = decoder_error_word();
     // Blocks a row: twice as many while there are fewer than two a multiprocessor and each has a round of its own.
-    // 64 rows of 128256: 15.8 us with eight blocks each, 29.8 with one; 333 rows: 9.7 with one, 10.4 with two, 14.4 with four.
+    // 64 rows of 128256: 12.4 us with eight blocks each, twice that with one; 333 rows: 9.7 with one, 10.4 with two, 14.4 with four.
     const int64_t each = int64_t(kWarps) * kHeld;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t err = cudaSuccess;
