@@ -881,26 +881,28 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
 // ---- joining the pieces of a row ----------------------------------------------------------------
 // out = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i in f32 over a row's parts (a piece has one, or
 // one of each group); a row without any key is 0.  One query row a lane.  What the kernel waits for is
-// the way to the L2 cache, so a thread has several parts in flight.  Few parts a row: a block has all
-// columns of its rows, four columns of four numbers a warp.  Many (a long prefix for few rows and heads):
-// the parts are dealt among the warps too, and their sums meet in shared memory.
-constexpr int kJoinWarps = 8, kJoinHeld = 4;
+// the way to the L2 cache, so a thread has several parts in flight: 8 of two columns (of four numbers), or
+// where there are rows enough for a block on every multiprocessor, 4 of four.  (64 rows of 8192 + 512 keys
+// 38.1 us so and 40.1 with four columns; 256 of 16384 + 128, 107.4 with four and 110.1 with two.)  Few parts a
+// row: the warps share its columns.  Many (a long prefix for few rows and heads): the parts are dealt
+// among the warps, and their sums meet in shared memory.
+constexpr int kJoinWarps = 8;
 // More than this many parts of a row are dealt among the warps: 33 rows of 5001 keys, 2 KV heads, 16.9 us so and 28.8
 // otherwise; 256 rows of 1024 + 128, 8 KV heads, 73.2 us so and 44.7 otherwise.
 constexpr int kManyParts = 12;
 
-template <typename T, int HD, bool MANY>
+template <typename T, int HD, bool MANY, int COLUMNS>
 __global__ void __launch_bounds__(32 * kJoinWarps)
 prefix_join_kernel(const __grid_constant__ PrefixArgs a, int blocks) {
     using H = Half16<T>;
     constexpr int kSlices = MANY ? kJoinWarps : 1;     // warps that share a row's parts
-    constexpr int kColumns = MANY ? 2 : HD / 4 / kJoinWarps, kSums = 4 * kColumns;
+    constexpr int kSums = 4 * COLUMNS, kJoinHeld = 16 / COLUMNS;
     __shared__ float sums[MANY ? kJoinWarps : 1][kSums + 2][32];  // O, m and l
     pdl_launch_dependents();
     pdl_wait();
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int head = blockIdx.y, row = blockIdx.x * 32 + lane;  // row: batch row * rep + head of the group
-    const int slice = MANY ? warp : 0, column = (MANY ? int(blockIdx.z) : warp) * kColumns;
+    const int slice = MANY ? warp : 0, column = (MANY ? int(blockIdx.z) : int(blockIdx.z) * kJoinWarps + warp) * COLUMNS;
     const bool live = row < a.batch * a.rep;
     const int b = live ? row / a.rep : 0, r = row - b * a.rep;
     auto word = [&](int i) { return int(ld_mutable(reinterpret_cast<const uint32_t*>(a.cum) + i)); };
@@ -934,7 +936,7 @@ prefix_join_kernel(const __grid_constant__ PrefixArgs a, int blocks) {
     float m = -INFINITY, l = 0.0f, o[kSums] = {};
     for (int k0 = slice; k0 < parts; k0 += kSlices * kJoinHeld) {
         float ms[kJoinHeld], ls[kJoinHeld];
-        uint4 os[kJoinHeld][kColumns];
+        uint4 os[kJoinHeld][COLUMNS];
 #pragma unroll
         for (int u = 0; u < kJoinHeld; ++u) {
             const int k = k0 + u * kSlices;
@@ -945,7 +947,7 @@ prefix_join_kernel(const __grid_constant__ PrefixArgs a, int blocks) {
             ms[u] = ld_mutable(from + HD * it.span + it.at);
             ls[u] = ld_mutable(from + (HD + 1) * it.span + it.at);
 #pragma unroll
-            for (int c = 0; c < kColumns; ++c) os[u][c] = ld_mutable(reinterpret_cast<const uint4*>(from) + (column + c) * it.span + it.at);
+            for (int c = 0; c < COLUMNS; ++c) os[u][c] = ld_mutable(reinterpret_cast<const uint4*>(from) + (column + c) * it.span + it.at);
         }
         float most = m;
 #pragma unroll
@@ -961,7 +963,7 @@ prefix_join_kernel(const __grid_constant__ PrefixArgs a, int blocks) {
             const float weight = exp2_approx(ms[u] - m);
             l += weight * ls[u];
 #pragma unroll
-            for (int c = 0; c < kColumns; ++c) {
+            for (int c = 0; c < COLUMNS; ++c) {
                 o[4 * c] += weight * __uint_as_float(os[u][c].x), o[4 * c + 1] += weight * __uint_as_float(os[u][c].y);
                 o[4 * c + 2] += weight * __uint_as_float(os[u][c].z), o[4 * c + 3] += weight * __uint_as_float(os[u][c].w);
             }
@@ -1062,9 +1064,15 @@ cudaError_t launch_prefix(const CUtensorMap (&maps)[6], const PrefixArgs& a, int
     err = launch_overlapped(prefix_attention_kernel<T, HD>, dim3(unsigned(blocks)), dim3(kThreads), kSmem, stream, maps[0],
                             maps[1], maps[2], maps[3], maps[4], maps[5], a);
     if (err != cudaSuccess) return err;
-    const dim3 grid{unsigned((a.batch * a.rep + 31) / 32), unsigned(a.nkv), unsigned(many ? HD / 8 : 1)};
-    return many ? launch_overlapped(prefix_join_kernel<T, HD, true>, grid, dim3(32 * kJoinWarps), 0, stream, a, blocks)
-                : launch_overlapped(prefix_join_kernel<T, HD, false>, grid, dim3(32 * kJoinWarps), 0, stream, a, blocks);
+    const unsigned rows = unsigned((a.batch * a.rep + 31) / 32);
+    constexpr int warps = HD / 4 / (4 * kJoinWarps);  // of four columns: 1, or none where a warp has no more than two
+    auto join = [&](auto kernel, unsigned parts) {
+        return launch_overlapped(kernel, dim3(rows, unsigned(a.nkv), parts), dim3(32 * kJoinWarps), 0, stream, a, blocks);
+    };
+    if (many) return join(prefix_join_kernel<T, HD, true, 2>, HD / 8);
+    if constexpr (warps > 0)
+        if (int64_t(rows) * a.nkv >= sm_count()) return join(prefix_join_kernel<T, HD, false, 4>, warps);
+    return join(prefix_join_kernel<T, HD, false, 2>, HD / 8 / kJoinWarps);
 }
 
 }  // namespace

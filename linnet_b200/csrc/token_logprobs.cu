@@ -165,7 +165,7 @@ __device__ __forceinline__ void add(const float (&x)[E], float m, float2& l, flo
 }
 
 // With alternatives, five blocks a multiprocessor: one's ranking goes by while the others read.  2048 rows with five:
-// 102 us so, 106 with four, 120 with three, 142 with six (of 40 registers, with spills); f32 162, 173, 184, 175.
+// 102 us so, 106 with four, 120 with three, 142 with six (of 40 registers each); f32 162, 173, 184, 175.
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kThreads, TOP ? 5 : 0)
 token_logprobs_kernel(const __grid_constant__ LogprobArgs a) {
