@@ -92,20 +92,27 @@ __device__ __forceinline__ int prefix_length(const PrefixArgs& a) {
     const int64_t given = ld_mutable(a.prefix_at);
     return int(given < 0 ? 0 : given > a.prefix ? a.prefix : given);
 }
-// The first unit of block c, and the block that takes unit t, of `total` over `blocks`: no more of them
-// than half the units, so that every block between two of an item's has a tile of it.  (total * c / blocks
-// in 32 bits; its inverse from an estimate that is a block off at most.)
-__device__ __forceinline__ int used_blocks(int total, int blocks) { return max(1, min(total / 2, blocks)); }
-__device__ __forceinline__ int first_unit(int c, int total, int blocks) {
-    const int whole = total / blocks;
-    return c >= blocks ? total : whole * c + (total - whole * blocks) * c / blocks;
-}
-__device__ __forceinline__ int block_of(int t, int total, int blocks) {
-    int c = min(int(float(t) * (float(blocks) / float(total))), blocks - 1);
-    while (first_unit(c, total, blocks) > t) --c;
-    while (first_unit(c + 1, total, blocks) <= t) ++c;
-    return c;
-}
+// How `total` units are dealt to blocks: no more of them than half the units, so that every block between two of
+// an item's has a tile of it.  The first unit of block c is total * c / blocks, in 32 bits and without a division
+// a call: rest * c is less than blocks^2, so that with a half added its quotient is further from any whole number
+// than f32 is off.  block_of inverts it from an estimate that is a block off at most.
+struct Deal {
+    int total, blocks, whole, rest;
+    float inverse, share;
+    __device__ __forceinline__ Deal(int units, int most) : total(units), blocks(max(1, min(units / 2, most))) {
+        whole = total / blocks, rest = total - whole * blocks;
+        inverse = __fdividef(1.0f, float(blocks)), share = __fdividef(float(blocks), float(total));
+    }
+    __device__ __forceinline__ int first(int c) const {
+        return c >= blocks ? total : whole * c + int((float(rest * c) + 0.5f) * inverse);
+    }
+    __device__ __forceinline__ int block_of(int t) const {
+        int c = min(int(float(t) * share), blocks - 1);
+        while (first(c) > t) --c;
+        while (first(c + 1) <= t) ++c;
+        return c;
+    }
+};
 
 struct Share {  // of a block; in shared memory
     int first, last, own_first;          // units; of the rows' own keys
@@ -414,8 +421,8 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
             all += bars.warp_units[w];
         }
         const int own_first = a.items * tiles_of(keys) * a.weight, total = own_first + all * a.nkv;
-        const int blocks = used_blocks(total, gridDim.x);
-        const int first = first_unit(blockIdx.x, total, blocks), last = first_unit(blockIdx.x + 1, total, blocks);
+        const Deal deal(total, gridDim.x);
+        const int first = deal.first(blockIdx.x), last = deal.first(blockIdx.x + 1);
         const int look = max(first, own_first);  // the first own unit this block can have
         if (threadIdx.x == 0) share.first = first, share.last = last, share.own_first = own_first, share.prefix_keys = keys;
         const int begin = own_first + before * a.nkv, end = begin + mine * a.nkv;
@@ -908,7 +915,7 @@ prefix_join_kernel(const __grid_constant__ PrefixArgs a, int blocks) {
     auto word = [&](int i) { return int(ld_mutable(reinterpret_cast<const uint32_t*>(a.cum) + i)); };
     const int total = word(a.batch), prefix_tiles = word(a.batch + 1), before = word(b);
     const int keys = own_keys(a, ld_mutable(a.positions + b));
-    blocks = used_blocks(total, blocks);
+    const Deal deal(total, blocks);
 
     struct Item {              // the prefix, and the row's own keys
         const float* base;     // of the first group that has the row, in the first piece
@@ -919,7 +926,7 @@ prefix_join_kernel(const __grid_constant__ PrefixArgs a, int blocks) {
         const int pair = b / (2 * a.tile_rows), within = b - pair * 2 * a.tile_rows;
         const bool both = min(2 * a.tile_rows, a.batch - pair * 2 * a.tile_rows) > a.tile_rows;
         const int item = head * a.row_tiles + pair, first = item * prefix_tiles * a.weight;
-        const int from = block_of(first, total, blocks), to = block_of(first + (prefix_tiles - 1) * a.weight, total, blocks);
+        const int from = deal.block_of(first), to = deal.block_of(first + (prefix_tiles - 1) * a.weight);
         const int g = both && within >= a.tile_rows, groups = both ? 1 : 2;
         shared.base = a.scratch + (2 * int64_t(item + from) + g) * group_floats(kRows, HD);
         shared.parts = (to - from + 1) * groups, shared.skip = int(group_floats(kRows, HD)) * (2 / groups);
@@ -927,7 +934,7 @@ prefix_join_kernel(const __grid_constant__ PrefixArgs a, int blocks) {
     }
     if (live && keys > 0) {
         const int first = a.items * prefix_tiles * a.weight + before * a.nkv + head * own_units(keys) + kOwnStart;
-        const int from = block_of(first, total, blocks), to = block_of(first + tiles_of(keys) - 1, total, blocks);
+        const int from = deal.block_of(first), to = deal.block_of(first + tiles_of(keys) - 1);
         own.base = a.scratch + a.own_at + int64_t(b * a.nkv + head + from) * group_floats(a.rep, HD);
         own.parts = to - from + 1, own.skip = int(group_floats(a.rep, HD));
         own.span = a.rep, own.at = r;
