@@ -114,6 +114,16 @@ struct Deal {
     }
 };
 
+// t / d of numbers below 2^30, by an estimate and its correction: the compiler's integer division is some hundred
+// clocks of one thread, which the short turns of the roles are made of.
+__device__ __forceinline__ int quotient(int t, int d) {
+    const float inverse = __fdividef(1.0f, float(d));
+    int q = int(float(t) * inverse);          // off by 2^-21 of it at most, and one
+    q += int(float(t - q * d) * inverse);     // off by one at most
+    const int left = t - q * d;
+    return left < 0 ? q - 1 : left >= d ? q + 1 : q;
+}
+
 struct Share {  // of a block; in shared memory
     int first, last, own_first;          // units; of the rows' own keys
     int prefix_keys;
@@ -289,10 +299,7 @@ __device__ __forceinline__ bool watch_at(uint32_t bar, uint32_t parity, int* err
 struct Walk {
     uint32_t full, empty, memory, slots;
     uint32_t slot, parity;
-    __device__ __forceinline__ void start(uint32_t load) {
-        const uint32_t lap = load / slots;
-        slot = load - lap * slots, parity = lap & 1;
-    }
+    __device__ __forceinline__ void start(uint32_t load, uint32_t lap) { slot = load - lap * slots, parity = lap & 1; }
     __device__ __forceinline__ void step(uint32_t loads) {  // fewer than there are slots
         slot += loads;
         if (slot >= slots) slot -= slots, parity ^= 1;
@@ -492,7 +499,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
                 uint64_t* const full = both ? bars.full : bars.own_full[g];
                 uint64_t* const empty = both ? bars.empty : bars.own_empty[g];
                 const uint32_t memory = smem_u32(slots) + (both ? 0 : g * kOwnSlots * S::kSlot), ring = both ? S::kSlots : kOwnSlots;
-                uint32_t slot = p.base % ring, lap = p.base / ring;
+                uint32_t lap = both ? p.base / S::kSlots : p.base / kOwnSlots, slot = p.base - lap * ring;
                 const int loads = 2 * p.tiles;
 #pragma unroll 1
                 for (int i = 0; i < loads; ++i) {
@@ -538,7 +545,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
                 Walk w;
                 w.full = smem_u32(both ? bars.full : bars.own_full[g]), w.empty = smem_u32(both ? bars.empty : bars.own_empty[g]);
                 w.memory = (smem_u32(slots) + (both ? 0 : g * kOwnSlots) * S::kSlot) >> 4, w.slots = both ? S::kSlots : kOwnSlots;
-                w.start(p.base + load);
+                w.start(p.base + load, both ? (p.base + load) / S::kSlots : (p.base + load) / kOwnSlots);
                 return w;
             };
             // Two ways through the group's tiles: the sums', and the scores' up to two tiles ahead of it.
@@ -653,10 +660,10 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
                 Piece p;
                 int first_tile, end_tile, count;  // this lane's tiles of its item; lanes that write
                 if (t < prefix_end) {             // two lanes an item: both groups' piece, or a group's half of the keys each
-                    const int item0 = t / item_units, item = item0 + lane / 2, head = item / a.row_tiles, tile = item - head * a.row_tiles;
+                    const int item0 = quotient(t, item_units), item = item0 + lane / 2, head = quotient(item, a.row_tiles), tile = item - head * a.row_tiles;
                     const int first = item * item_units;
-                    first_tile = (max(t, first) - first + a.weight - 1) / a.weight;
-                    end_tile = (min(first + item_units, prefix_end) - first + a.weight - 1) / a.weight;
+                    first_tile = (max(t, first) - first + a.weight - 1) >> (a.weight - 1);  // (a weight is 1 or 2)
+                    end_tile = (min(first + item_units, prefix_end) - first + a.weight - 1) >> (a.weight - 1);
                     p.head = static_cast<unsigned short>(head), p.row = tile * 2 * a.tile_rows;
                     p.rows = static_cast<unsigned short>(max(0, min(2 * a.tile_rows, a.batch - p.row)));
                     p.place = item + int(blockIdx.x);
@@ -670,7 +677,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
                         p.who = kNobody;
                     }
                     p.key = first_tile * kKeys, p.keys = share.prefix_keys - p.key;
-                    const int items = (prefix_end - item0 * item_units + item_units - 1) / item_units;
+                    const int items = quotient(prefix_end - item0 * item_units + item_units - 1, item_units);
                     count = min(kBatch - n, 2 * items);
                     t = min(prefix_end, (item0 + count / 2) * item_units);
                 } else {                          // a head of the row a lane; one group's: the other is at the piece before or after
@@ -686,13 +693,13 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
                         if (t < at + each * a.nkv) break;
                         at += each * a.nkv;
                     }
-                    const int head0 = (t - at) / each, head = head0 + lane, first = at + head * each;
+                    const int head0 = quotient(t - at, each), head = head0 + lane, first = at + head * each;
                     first_tile = max(0, t - first - kOwnStart), end_tile = min(tiles_of(keys), share.last - first - kOwnStart);
                     p.head = static_cast<unsigned short>(head), p.row = row, p.rows = 1, p.kind = kOwn;
                     p.who = end_tile <= first_tile ? kNobody : (n + lane) & 1 ? kGroup1 : kGroup0;
                     p.key = first_tile * kKeys, p.keys = keys - p.key;
                     p.place = row * a.nkv + head + int(blockIdx.x);
-                    const int left = min(a.nkv - head0, (share.last - (at + head0 * each) + each - 1) / each);
+                    const int left = min(a.nkv - head0, quotient(share.last - (at + head0 * each) + each - 1, each));
                     count = min(kBatch - n, left);
                     t = min(share.last, at + (head0 + count) * each);
                 }
@@ -830,8 +837,9 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
                     // Rows of V past the last key may hold anything, and 0 * NaN is no 0: those that the last
                     // step of 16 keys takes in are cleared (by either group where both use the tile).
                     const bool both = p.who == kBoth;
-                    const uint32_t load = p.base + load_of_v(tile, p.tiles), ring = both ? S::kSlots : kOwnSlots, slot = load % ring;
-                    ok = ok && wait((both ? bars.full : bars.own_full[g]) + slot, (load / ring) & 1, 49);
+                    const uint32_t load = p.base + load_of_v(tile, p.tiles), lap = both ? load / S::kSlots : load / kOwnSlots,
+                                   slot = load - lap * (both ? S::kSlots : kOwnSlots);
+                    ok = ok && wait((both ? bars.full : bars.own_full[g]) + slot, lap & 1, 49);
                     if (!ok) break;
                     uint8_t* tail = slots + ((both ? 0 : g * kOwnSlots) + slot) * S::kSlot;
                     const int rows = (16 - keys % 16) % 16;
@@ -911,7 +919,7 @@ prefix_join_kernel(const __grid_constant__ PrefixArgs a, int blocks) {
     const int head = blockIdx.y, row = blockIdx.x * 32 + lane;  // row: batch row * rep + head of the group
     const int slice = MANY ? warp : 0, column = (MANY ? int(blockIdx.z) : int(blockIdx.z) * kJoinWarps + warp) * COLUMNS;
     const bool live = row < a.batch * a.rep;
-    const int b = live ? row / a.rep : 0, r = row - b * a.rep;
+    const int b = live ? quotient(row, a.rep) : 0, r = row - b * a.rep;
     auto word = [&](int i) { return int(ld_mutable(reinterpret_cast<const uint32_t*>(a.cum) + i)); };
     const int total = word(a.batch), prefix_tiles = word(a.batch + 1), before = word(b);
     const int keys = own_keys(a, ld_mutable(a.positions + b));
@@ -923,7 +931,7 @@ prefix_join_kernel(const __grid_constant__ PrefixArgs a, int blocks) {
         int span, at;          // rows of a group in the scratch memory, and which one this is
     } shared = {}, own = {};
     if (live && prefix_tiles > 0) {
-        const int pair = b / (2 * a.tile_rows), within = b - pair * 2 * a.tile_rows;
+        const int pair = quotient(b, 2 * a.tile_rows), within = b - pair * 2 * a.tile_rows;
         const bool both = min(2 * a.tile_rows, a.batch - pair * 2 * a.tile_rows) > a.tile_rows;
         const int item = head * a.row_tiles + pair, first = item * prefix_tiles * a.weight;
         const int from = deal.block_of(first), to = deal.block_of(first + (prefix_tiles - 1) * a.weight);
