@@ -9,8 +9,8 @@
 // tiles stand in one sequence, prefix first, and block c of G takes the c-th G-th of it, so blocks have
 // equal work whatever the lengths; where a block's share begins and ends, an item is cut into PIECES,
 // each with its own softmax statistics, and a second kernel joins the pieces of a row.  (An item of own
-// keys counts one tile more than it has, for its start: 64 rows of 16384 + 64 keys take 44.7 us so,
-// 62.5 without, 45.1 with two.)  An item and a block have at most one piece in common, and
+// keys counts one tile more than it has, for its start: 256 rows of 1024 + 128 keys take 43.9 us so,
+// 46.2 without, 50.7 with two; of 16384 + 128 keys 104, 151 and 105.)  An item and a block have at most one piece in common, and
 // (item + block) grows along the sequence: that is a piece's place in the scratch memory.
 //
 // A block has two groups, each a pipeline of its own: a TMA producer, an issuer of products and four
@@ -31,11 +31,11 @@
 // P is rounded to the tensors' type, as the product takes it; l sums P before that rounding.
 //
 // What bounds it, measured on a B200 (nq 32, nkv 8, D 128, bf16; join included): few rows, HBM and the
-// start of the pipeline: 8 rows of 65536 keys 54 us, 5.0 TB/s; 64 rows of 8192 + up to 512 own keys
-// 40 us where the bytes take 15.6; 2 rows of 100 keys 9.3 us, two launches and their latencies.  Many
-// rows, the chain from scores to weights to the next scores: 256 rows of 65536 keys 283 us, 973 TFLOP/s
-// (59 % of measured).  A tile of both groups takes some 2200 clocks there; its products alone take 1300,
-// its 16384 exponentials 1024, its 32 KB from L2 some 1100.
+// start of the pipeline: 8 rows of 65536 keys 53 us, 5.1 TB/s; 64 rows of 8192 + up to 512 own keys
+// 37 us where the bytes take 15.6; 2 rows of 100 keys 8.4 us, two launches and their latencies.  Many
+// rows, the chain from scores to weights to the next scores, at the clock that the power limit leaves (1.4 to
+// 1.7 GHz): 256 rows of 65536 keys 284 us, 960 TFLOP/s (58 % of measured).  A tile of both groups takes
+// some 2000 clocks there; its products alone take 1300, its 16384 exponentials 1024, its 32 KB 700.
 #include "mma.cuh"
 #include "umma.cuh"
 
@@ -898,13 +898,14 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
 // one of each group); a row without any key is 0.  One query row a lane.  What the kernel waits for is
 // the way to the L2 cache, so a thread has several parts in flight: 8 of two columns (of four numbers), or
 // where there are rows enough for a block on every multiprocessor, 4 of four.  (64 rows of 8192 + 512 keys
-// 38.1 us so and 40.1 with four columns; 256 of 16384 + 128, 107.4 with four and 110.1 with two.)  Few parts a
+// 37.1 us so and 39.3 with four columns; 256 of 16384 + 128, 103.9 with four and 107.2 with two.)  Few parts a
 // row: the warps share its columns.  Many (a long prefix for few rows and heads): the parts are dealt
 // among the warps, and their sums meet in shared memory.
 constexpr int kJoinWarps = 8;
-// More than this many parts of a row are dealt among the warps: 33 rows of 5001 keys, 2 KV heads, 16.9 us so and 28.8
-// otherwise; 256 rows of 1024 + 128, 8 KV heads, 73.2 us so and 44.7 otherwise.
-constexpr int kManyParts = 12;
+// More than so many parts of a row are dealt among the warps, where there are fewer than so many blocks of rows
+// and heads: 33 rows of 5001 keys, 2 KV heads (16 blocks), 14.2 us so and 22.5 otherwise; 64 of 16384 + 64, 8 KV heads
+// (64 blocks), 43.5 so and 39.8 otherwise; 256 of 1024 + 128, few parts, 73.8 so and 43.8 otherwise.
+constexpr int kManyParts = 12, kFewBlocks = 32;
 
 template <typename T, int HD, bool MANY, int COLUMNS>
 __global__ void __launch_bounds__(32 * kJoinWarps)
@@ -1032,7 +1033,8 @@ PrefixPlan plan_of(int64_t batch, int64_t nkv, int64_t rep, int64_t hd, int64_t 
     if (units / 2 < p.blocks) p.blocks = units < 2 ? 1 : int(units / 2);
     // Parts of a row, were all rows' caches full: blocks an item's tiles are spread over, and a block at either end.
     const int64_t share = units < 1 ? 1 : (units + p.blocks - 1) / p.blocks;
-    p.many = (p.items > 0 ? ((of_prefix * p.weight + share - 1) / share + 1) * (batch > p.tile_rows ? 1 : 2) : 0) + (of_own + share - 1) / share + 1 > kManyParts;
+    const int64_t parts = (p.items > 0 ? ((of_prefix * p.weight + share - 1) / share + 1) * (batch > p.tile_rows ? 1 : 2) : 0) + (of_own + share - 1) / share + 1;
+    p.many = parts > kManyParts && (batch * rep + 31) / 32 * nkv < kFewBlocks;
     p.own_at = (p.items > 0 ? p.items + p.blocks : 0) * 2 * group_floats(kRows, int(hd));
     p.cum_at = p.own_at + (batch * nkv + p.blocks) * group_floats(int(rep), int(hd));
     p.floats = p.cum_at + (batch + 2 + 3) / 4 * 4;

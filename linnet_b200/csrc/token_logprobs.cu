@@ -18,7 +18,7 @@
 // where the first guess has too many), reads those groups once more and ranks what reaches it.
 //
 // Measured on a B200, rows of 128256: 2048 of bf16 with 5 alternatives 102 us, 5.1 TB/s (92 without:
-// 5.7 TB/s), of f32 162 us, 6.5 TB/s; 64 of f32 12.4 us; one of bf16 with 20 alternatives 8.9 us, half of
+// 5.7 TB/s), of f32 162 us, 6.5 TB/s; 64 of f32 12.5 us; one of bf16 with 20 alternatives 8.9 us, half of
 // it the way from the last logit over the cluster's barrier to the ranked list.
 #include <cooperative_groups.h>
 
@@ -520,14 +520,15 @@ extern "C" int32_t b200q_token_logprobs(const void* logits, const int64_t* token
     a.vocab = int(vocab), a.top = int(top);
     a.groups = int((vocab + elements - 1 + 32 * elements - 1) / (32 * elements));  // of a row wherever it starts
     a.status = decoder_error_word();
-    // Blocks a row: twice as many while there are fewer than two a multiprocessor and each has a round of its own.
-    // 64 rows of 128256: 12.4 us with eight blocks each, twice that with one; 333 rows: 9.7 with one, 10.4 with two, 14.4 with four.
+    // Blocks a row: twice as many while there are fewer than four a multiprocessor and each has a round of its own.
+    // 64 f32 rows of 128256: 12.5 us with eight blocks each, 29.6 with one; 148: 20.6 with four, 25.3 with two, 24.6 with
+    // eight; 333 f16 rows of 32003: 9.8 with one, 10.0 with two, 13.9 with four.
     const int64_t each = int64_t(kWarps) * kHeld;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t err = cudaSuccess;
     const int n = int(rows);
     int blocks = 1;
-    while (blocks < 8 && rows * blocks < 2 * sm_count() && a.groups > blocks * each) blocks *= 2;
+    while (blocks < 8 && rows * blocks < 4 * sm_count() && a.groups > blocks * each) blocks *= 2;
     if (dtype == B200Q_F32) err = top ? launch<float, true>(a, n, blocks, s) : launch<float, false>(a, n, blocks, s);
     else if (dtype == B200Q_BF16)
         err = top ? launch<__nv_bfloat16, true>(a, n, blocks, s) : launch<__nv_bfloat16, false>(a, n, blocks, s);
