@@ -10,7 +10,9 @@
 // equal work whatever the lengths; where a block's share begins and ends, an item is cut into PIECES,
 // each with its own softmax statistics, and a second kernel joins the pieces of a row.  (An item of own
 // keys counts one tile more than it has, for its start: 256 rows of 1024 + 128 keys take 43.9 us so,
-// 46.2 without, 50.7 with two; of 16384 + 128 keys 104, 151 and 105.)  An item and a block have at most one piece in common, and
+// 46.2 without, 50.7 with two; of 16384 + 128 keys 104, 151 and 105.  One of the prefix counts two more: 256 rows
+// of 64 + 128 keys 38.2 us so, 50.8 with one, 84.1 without, 37.9 with three; 33 rows of 5001, 2 KV heads, 13.0,
+// 13.6, 14.2 and 13.6.)  An item and a block have at most one piece in common, and
 // (item + block) grows along the sequence: that is a piece's place in the scratch memory.
 //
 // A block has two groups, each a pipeline of its own: a TMA producer, an issuer of products and four
@@ -32,7 +34,7 @@
 //
 // What bounds it, measured on a B200 (nq 32, nkv 8, D 128, bf16; join included): few rows, HBM and the
 // start of the pipeline: 8 rows of 65536 keys 53 us, 5.1 TB/s; 64 rows of 8192 + up to 512 own keys
-// 37 us where the bytes take 15.6; 2 rows of 100 keys 8.4 us, two launches and their latencies.  Many
+// 36 us where the bytes take 15.6; 2 rows of 100 keys 8.4 us, two launches and their latencies.  Many
 // rows, the chain from scores to weights to the next scores, at the clock that the power limit leaves (1.4 to
 // 1.7 GHz): 256 rows of 65536 keys 284 us, 960 TFLOP/s (58 % of measured).  A tile of both groups takes
 // some 2000 clocks there; its products alone take 1300, its 16384 exponentials 1024, its 32 KB 700.
@@ -52,6 +54,7 @@ constexpr uint32_t kTmemColumns = 512;     // S of both groups, O of both groups
 constexpr float kStale = 8.0f;             // how far (log2) a tile's maximum may exceed the row's before it moves
 constexpr float kLowest = -3.0e38f;        // the maximum of scores that are all -inf: 2^(-inf - m) is 0, and any other exceeds it
 constexpr int kOwnStart = 1;               // what an item of own keys costs beside its tiles, in tiles
+constexpr int kPrefixStart = 2;            // and what one of the prefix does
 
 template <int HD>
 struct Shape {
@@ -85,6 +88,8 @@ __device__ __forceinline__ int own_keys(const PrefixArgs& a, int64_t position) {
     return position < -1 || position >= a.slots ? 0 : int(position) + 1;  // outside the cache: none
 }
 __device__ __forceinline__ int tiles_of(int keys) { return (keys + kKeys - 1) / kKeys; }
+// Units of an item of the prefix.
+__device__ __forceinline__ int prefix_units(const PrefixArgs& a, int tiles) { return tiles > 0 ? (tiles + kPrefixStart) * a.weight : 0; }
 // Units of one head of a row.
 __device__ __forceinline__ int own_units(int keys) { return keys > 0 ? tiles_of(keys) + kOwnStart : 0; }
 __device__ __forceinline__ int prefix_length(const PrefixArgs& a) {
@@ -427,7 +432,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
             if (w < warp) before += bars.warp_units[w];
             all += bars.warp_units[w];
         }
-        const int own_first = a.items * tiles_of(keys) * a.weight, total = own_first + all * a.nkv;
+        const int own_first = a.items * prefix_units(a, tiles_of(keys)), total = own_first + all * a.nkv;
         const Deal deal(total, gridDim.x);
         const int first = deal.first(blockIdx.x), last = deal.first(blockIdx.x + 1);
         const int look = max(first, own_first);  // the first own unit this block can have
@@ -644,7 +649,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
         int t = share.first, row = share.own_row, at = share.own_row_unit;
         int keys_of = 0, held = -1;            // own keys of rows 32 * held + lane
         const int prefix_end = min(share.own_first, share.last), prefix_tiles = tiles_of(share.prefix_keys);
-        const int item_units = prefix_tiles * a.weight;
+        const int item_units = prefix_units(a, prefix_tiles);
         uint32_t loads_both = 0, loads_0 = 0, loads_1 = 0;     // before the batch's next piece: loads of the rings,
         uint32_t fills = 0, own_fills = 0;                     // pieces of the groups (16 bits each): of a prefix, of own keys
         int kind = -1;
@@ -662,8 +667,8 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
                 if (t < prefix_end) {             // two lanes an item: both groups' piece, or a group's half of the keys each
                     const int item0 = quotient(t, item_units), item = item0 + lane / 2, head = quotient(item, a.row_tiles), tile = item - head * a.row_tiles;
                     const int first = item * item_units;
-                    first_tile = (max(t, first) - first + a.weight - 1) >> (a.weight - 1);  // (a weight is 1 or 2)
-                    end_tile = (min(first + item_units, prefix_end) - first + a.weight - 1) >> (a.weight - 1);
+                    first_tile = max(0, ((max(t, first) - first + a.weight - 1) >> (a.weight - 1)) - kPrefixStart);  // (a weight is 1 or 2)
+                    end_tile = max(first_tile, ((min(first + item_units, prefix_end) - first + a.weight - 1) >> (a.weight - 1)) - kPrefixStart);
                     p.head = static_cast<unsigned short>(head), p.row = tile * 2 * a.tile_rows;
                     p.rows = static_cast<unsigned short>(max(0, min(2 * a.tile_rows, a.batch - p.row)));
                     p.place = item + int(blockIdx.x);
@@ -903,8 +908,8 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
 // among the warps, and their sums meet in shared memory.
 constexpr int kJoinWarps = 8;
 // More than so many parts of a row are dealt among the warps, where there are fewer than so many blocks of rows
-// and heads: 33 rows of 5001 keys, 2 KV heads (16 blocks), 14.2 us so and 22.5 otherwise; 64 of 16384 + 64, 8 KV heads
-// (64 blocks), 43.5 so and 39.8 otherwise; 256 of 1024 + 128, few parts, 73.8 so and 43.8 otherwise.
+// and heads: 33 rows of 5001 keys, 2 KV heads (16 blocks), 13.0 us so and 21.3 otherwise; 64 of 16384 + 64, 8 KV heads
+// (64 blocks), 43.5 so and 39.7 otherwise; 256 of 1024 + 128, few parts, 72.1 so and 42.2 otherwise.
 constexpr int kManyParts = 12, kFewBlocks = 32;
 
 template <typename T, int HD, bool MANY, int COLUMNS>
@@ -934,7 +939,7 @@ prefix_join_kernel(const __grid_constant__ PrefixArgs a, int blocks) {
     if (live && prefix_tiles > 0) {
         const int pair = quotient(b, 2 * a.tile_rows), within = b - pair * 2 * a.tile_rows;
         const bool both = min(2 * a.tile_rows, a.batch - pair * 2 * a.tile_rows) > a.tile_rows;
-        const int item = head * a.row_tiles + pair, first = item * prefix_tiles * a.weight;
+        const int item = head * a.row_tiles + pair, first = item * prefix_units(a, prefix_tiles) + kPrefixStart * a.weight;
         const int from = deal.block_of(first), to = deal.block_of(first + (prefix_tiles - 1) * a.weight);
         const int g = both && within >= a.tile_rows, groups = both ? 1 : 2;
         shared.base = a.scratch + (2 * int64_t(item + from) + g) * group_floats(kRows, HD);
@@ -942,7 +947,7 @@ prefix_join_kernel(const __grid_constant__ PrefixArgs a, int blocks) {
         shared.span = kRows, shared.at = (within - g * a.tile_rows) * a.rep + r;
     }
     if (live && keys > 0) {
-        const int first = a.items * prefix_tiles * a.weight + before * a.nkv + head * own_units(keys) + kOwnStart;
+        const int first = a.items * prefix_units(a, prefix_tiles) + before * a.nkv + head * own_units(keys) + kOwnStart;
         const int from = deal.block_of(first), to = deal.block_of(first + tiles_of(keys) - 1);
         own.base = a.scratch + a.own_at + int64_t(b * a.nkv + head + from) * group_floats(a.rep, HD);
         own.parts = to - from + 1, own.skip = int(group_floats(a.rep, HD));
@@ -1029,7 +1034,7 @@ PrefixPlan plan_of(int64_t batch, int64_t nkv, int64_t rep, int64_t hd, int64_t 
     p.weight = batch > p.tile_rows ? 2 : 1;
     p.blocks = sm_count();
     const int64_t of_prefix = (prefix + kKeys - 1) / kKeys, of_own = (slots + kKeys - 1) / kKeys;
-    const int64_t units = p.items * of_prefix * p.weight + batch * nkv * (of_own + kOwnStart);
+    const int64_t units = p.items * (of_prefix + kPrefixStart) * p.weight + batch * nkv * (of_own + kOwnStart);
     if (units / 2 < p.blocks) p.blocks = units < 2 ? 1 : int(units / 2);
     // Parts of a row, were all rows' caches full: blocks an item's tiles are spread over, and a block at either end.
     const int64_t share = units < 1 ? 1 : (units + p.blocks - 1) / p.blocks;
@@ -1049,7 +1054,7 @@ int32_t check_prefix(int64_t batch, int64_t nq, int64_t nkv, int64_t hd, int64_t
     B200Q_REQUIRE(prefix >= 0 && prefix < (int64_t(1) << 30) && slots >= 0 && slots < (int64_t(1) << 30),
                   "prefix_attention: bad length of the prefix or the cache");
     const int64_t row_tiles = batch / (2 * (kRows / (nq / nkv))) + 1;
-    B200Q_REQUIRE(2 * nkv * row_tiles * (prefix / kKeys + 1) + batch * nkv * (slots / kKeys + 2) < (int64_t(1) << 30) &&
+    B200Q_REQUIRE(2 * nkv * row_tiles * (prefix / kKeys + 1 + kPrefixStart) + batch * nkv * (slots / kKeys + 2) < (int64_t(1) << 30) &&
                       batch * nq < (int64_t(1) << 30),
                   "prefix_attention: more than 2^30 tiles of 64 keys, or rows times heads");
     return B200Q_OK;
