@@ -9,8 +9,8 @@
 // tiles stand in one sequence, prefix first, and block c of G takes the c-th G-th of it, so blocks have
 // equal work whatever the lengths; where a block's share begins and ends, an item is cut into PIECES,
 // each with its own softmax statistics, and a second kernel joins the pieces of a row.  (An item of own
-// keys counts one tile more than it has, for its start: 256 rows of 1024 + 128 keys take 43.9 us so,
-// 46.2 without, 50.7 with two; of 16384 + 128 keys 104, 151 and 105.  One of the prefix counts two more: 256 rows
+// keys counts one tile more than it has, for its start: 256 rows of 1024 + 128 keys take 41.8 us so,
+// 46.7 without, 46.8 with two; of 16384 + 128 keys 104, 152 and 103.  One of the prefix counts two more: 256 rows
 // of 64 + 128 keys 38.2 us so, 50.8 with one, 84.1 without, 37.9 with three; 33 rows of 5001, 2 KV heads, 13.0,
 // 13.6, 14.2 and 13.6.)  An item and a block have at most one piece in common, and
 // (item + block) grows along the sequence: that is a piece's place in the scratch memory.
@@ -903,13 +903,13 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
 // one of each group); a row without any key is 0.  One query row a lane.  What the kernel waits for is
 // the way to the L2 cache, so a thread has several parts in flight: 8 of two columns (of four numbers), or
 // where there are rows enough for a block on every multiprocessor, 4 of four.  (64 rows of 8192 + 512 keys
-// 37.1 us so and 39.3 with four columns; 256 of 16384 + 128, 103.9 with four and 107.2 with two.)  Few parts a
+// 35.7 us so and 38.0 with four columns; 256 of 16384 + 128, 104.3 with four and 106.6 with two.)  Few parts a
 // row: the warps share its columns.  Many (a long prefix for few rows and heads): the parts are dealt
 // among the warps, and their sums meet in shared memory.
 constexpr int kJoinWarps = 8;
 // More than so many parts of a row are dealt among the warps, where there are fewer than so many blocks of rows
-// and heads: 33 rows of 5001 keys, 2 KV heads (16 blocks), 13.0 us so and 21.3 otherwise; 64 of 16384 + 64, 8 KV heads
-// (64 blocks), 43.5 so and 39.7 otherwise; 256 of 1024 + 128, few parts, 72.1 so and 42.2 otherwise.
+// and heads: 33 rows of 5001 keys, 2 KV heads (16 blocks), 12.8 us so and 21.1 otherwise; 64 of 16384 + 64, 8 KV heads
+// (64 blocks), 43.5 so and 39.6 otherwise; 256 of 1024 + 128, few parts, 71.6 so and 41.8 otherwise.
 constexpr int kManyParts = 12, kFewBlocks = 32;
 
 template <typename T, int HD, bool MANY, int COLUMNS>
