@@ -13,14 +13,13 @@
 // head a thread, reading the cosines took 60 % of the shared memory's time.)  With few tokens the heads
 // of one are divided among blocks too.
 //
-// Measured on a B200: 8192 tokens of 32 + 8 heads of 128, bf16, 34.3 us, 4.9 TB/s (neighbours 38.2);
-// one token 2.5 us, its latency.
+// Measured on a B200: 8192 tokens of 32 + 8 heads of 128, bf16, 33.2 us, 5.05 TB/s; one token 2.5 us, its latency.
 #include "mma.cuh"
 
 namespace b200q {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;      // 8192 tokens 33.2 us, of neighbours 33.3; with 256 threads 34.4 and 38.2
 constexpr int kHeld = 5;           // heads a thread has in flight, of large calls; of small ones 1
 constexpr int kMaxTokens = 16;     // of a block
 constexpr int kMaxTurns = 4096;    // (cos, sin) pairs of a block: 32 KB
@@ -224,9 +223,9 @@ int32_t launch_rotary(const char* who, RotaryArgs a, int32_t layout, int32_t dty
     const int copied = (a.head_dim - 2 * a.pairs + 2 * w - 1) / (2 * w), whole = (a.head_dim + 2 * w - 1) / (2 * w);
     a.units = a.turning + copied;
     if (kinds == 3 && a.units < whole) a.units = whole;  // a head of v is copied whole
-    // Few units (eight blocks of one a thread on every multiprocessor have them all): one head at a time, which takes
-    // half the registers, so that all blocks are there at once.  512 tokens, 32 + 8 heads of 128: 4.3 us so and
-    // 6.5 with five heads in flight; 8192 tokens 50.9 so and 34.4 (38.1 with eight, 39.6 with four).
+    // Few units (eight blocks of one a thread on every multiprocessor have them all): one head at a time, the shorter
+    // kernel.  16 tokens, 32 + 8 heads of 128: 2.5 us so and 2.8 with five heads in flight; 512 tokens 5.4 so and 4.5; 8192
+    // tokens 34.1 so and 33.2 (36.7 with four, 36.0 with eight).
     const int sms = sm_count(), per_token = a.heads * a.units;
     const bool few = int64_t(a.tokens) * per_token <= int64_t(8) * sms * kThreads;
     const int held = few ? 1 : kHeld;
