@@ -344,7 +344,8 @@ int32_t b200q_rotary_table(void* table, const double* frequencies, int64_t max_s
  *     not taken), 16-byte aligned, of this call until it is done; nothing in it needs clearing.
  *   scale: positive.
  *   What lies behind the last key of a prefix or cache may hold anything, NaN too.
- *   batch up to 65536, kv heads up to 65535, fewer than 2^30 tiles of 64 keys over all of them.
+ *   batch up to 65536, kv heads up to 65535, fewer than 2^26 tiles of 64 keys over all of them (those
+ *     of the prefix counted once for every 128 query rows of a KV head).
  * Two launches.  A bounded wait that expires is reported by b200q_int4_gemm_status(). */
 int64_t b200q_prefix_attention_scratch_bytes(int64_t batch, int64_t nq, int64_t nkv,
                                              int64_t head_dim, int64_t prefix, int64_t max_seq);

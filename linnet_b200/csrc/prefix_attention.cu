@@ -1054,9 +1054,10 @@ int32_t check_prefix(int64_t batch, int64_t nq, int64_t nkv, int64_t hd, int64_t
     B200Q_REQUIRE(prefix >= 0 && prefix < (int64_t(1) << 30) && slots >= 0 && slots < (int64_t(1) << 30),
                   "prefix_attention: bad length of the prefix or the cache");
     const int64_t row_tiles = batch / (2 * (kRows / (nq / nkv))) + 1;
-    B200Q_REQUIRE(2 * nkv * row_tiles * (prefix / kKeys + 1 + kPrefixStart) + batch * nkv * (slots / kKeys + 2) < (int64_t(1) << 30) &&
+    // (a multiprocessor's share of these takes a third of a second, so that no role waits for the second that ends a wait)
+    B200Q_REQUIRE(2 * nkv * row_tiles * (prefix / kKeys + 1 + kPrefixStart) + batch * nkv * (slots / kKeys + 2) < (int64_t(1) << 26) &&
                       batch * nq < (int64_t(1) << 30),
-                  "prefix_attention: more than 2^30 tiles of 64 keys, or rows times heads");
+                  "prefix_attention: 2^26 tiles of 64 keys or more (those of the prefix counted for every 128 rows), or 2^30 rows times heads");
     return B200Q_OK;
 }
 

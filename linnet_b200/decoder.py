@@ -376,6 +376,8 @@ class Int4Decoder:
         nq, nkv, hd = cfg.heads // tp, cfg.kv_heads // tp, cfg.head_dim
         batch = tokens.shape[0]
         rows = torch.arange(batch, device=tokens.device)
+        if cfg.rope_scaling is not None:
+            self._make_frequencies()
 
         def upto(slots: int, last: torch.Tensor) -> torch.Tensor:
             return torch.arange(slots, device=tokens.device)[None, :] <= last[:, None]
