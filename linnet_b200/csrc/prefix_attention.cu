@@ -315,8 +315,8 @@ struct Barriers {
     uint64_t full[20], empty[20];              // tiles of K and V that both groups take
     uint64_t own_full[2][10], own_empty[2][10];    // ... that one takes: half of the slots each
     uint64_t query_full[2][2], query_empty[2][2];  // of the groups: two buffers
-    uint64_t scores[2][2], weights[2][2];      // of the groups' two buffers: S is there, P is there
-    uint64_t summed[2], result[2];             // of the groups: P . V of a tile is done; O of a piece is complete
+    uint64_t scores[2][2], weights[2][2], summed[2][2];  // of the groups' two buffers: S is there, P is there, P . V is done
+    uint64_t result[2];                        // of the groups: O of a piece is complete
     uint64_t changed;                          // the pieces of one kind are done, those of another begin
     uint64_t list_full[2], list_empty[2];      // batches of pieces
     Piece list[2 * kBatch];
@@ -389,9 +389,9 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
             for (int s = 0; s < kOwnSlots; ++s) mbar_init(&bars.own_full[g][s], 1), mbar_init(&bars.own_empty[g][s], 1);
             for (int b = 0; b < 2; ++b) {
                 mbar_init(&bars.query_full[g][b], 1), mbar_init(&bars.query_empty[g][b], 1);
-                mbar_init(&bars.scores[g][b], 1), mbar_init(&bars.weights[g][b], 4);
+                mbar_init(&bars.scores[g][b], 1), mbar_init(&bars.weights[g][b], 4), mbar_init(&bars.summed[g][b], 1);
             }
-            mbar_init(&bars.summed[g], 1), mbar_init(&bars.result[g], 1);
+            mbar_init(&bars.result[g], 1);
             mbar_init(&bars.list_full[g], 1), mbar_init(&bars.list_empty[g], kListReaders);
         }
         mbar_init(&bars.changed, 4);  // producers and issuers
@@ -540,7 +540,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
             constexpr uint32_t kValues = (1u << 4) | (kType << 7) | (kType << 10) | (1u << 16) | (uint32_t(HD >> 3) << 17) | (uint32_t(kRows >> 4) << 24);
             const int g = warp - kIssuerWarp;
             const uint32_t s_at = tmem + uint32_t(g) * 2 * kKeys, o_at = tmem + 4 * kKeys + uint32_t(g) * HD;
-            const uint32_t scores = smem_u32(&bars.scores[g][0]), weights = smem_u32(&bars.weights[g][0]), summed = smem_u32(&bars.summed[g]),
+            const uint32_t scores = smem_u32(&bars.scores[g][0]), weights = smem_u32(&bars.weights[g][0]), summed = smem_u32(&bars.summed[g][0]),
                            result = smem_u32(&bars.result[g]), query_full = smem_u32(&bars.query_full[g][0]),
                            query_empty = smem_u32(&bars.query_empty[g][0]), queries = (smem_u32(smem) + g * S::kQuery) >> 4;
             const uint32_t k_high = uint32_t(smem_desc(0) >> 32), k_low = uint32_t(smem_desc(0));
@@ -635,9 +635,9 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
                 for (int k = 0; k < kKeys / 16; ++k)
                     if (k == 0 || k * 16 < keys) umma_f16_ts(o_at, from + k * 8, desc_of(vd + uint32_t(k) * (2048 >> 4), v_high), kValues, k > 0 || tile > 0);
                 if (last) commit_at(result);
+                commit_at(summed + 8 * b);
                 if (follows) issue_scores();
                 commit_at(vs.empty + 8 * vs.slot);
-                commit_at(summed);
                 ++task, ++tile;
                 if (last) next_piece();
                 else vs.step(tile + 1 == p.tiles ? 1 : 2);
@@ -772,6 +772,10 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
                 const int keys = p.keys - tile * kKeys;   // of the tile, and more
                 const uint32_t b = task & 1, at = s_at + b * kKeys;
                 ok = wait(&bars.scores[g][b], (task >> 1) & 1, 48);
+                // The sums of two tiles ago, which these scores stood behind, but by a commit of their own: every phase of
+                // `summed` is waited for in order (no later one of this barrier can be over, its weights are not made yet),
+                // or the wait for the sums of the last tile, below, could take the phase before theirs for it.
+                if (ok && task >= 2) ok = wait(&bars.summed[g][b], ((task - 2) >> 1) & 1, 53);
                 if (!ok) break;
                 tc_fence_after();
                 if (any) {
@@ -799,8 +803,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
                         const float next = here - kLift > m + kStale ? here - kLift : m, by = exp2_approx(m - next);
                         m = next;
                         l *= by;
-                        // (these scores were asked for behind the sums before the last ones)
-                        ok = wait(&bars.summed[g], (task - 1) & 1, 53);
+                        ok = wait(&bars.summed[g][b ^ 1], ((task - 1) >> 1) & 1, 53);
                         tc_fence_after();
 #pragma unroll 1
                         for (int c = 0; c < HD; c += 8) {
