@@ -52,7 +52,7 @@ constexpr int kProducerWarp = 8, kIssuerWarp = 10, kListWarp = 12;  // a produce
 constexpr int kThreads = 13 * 32;
 constexpr uint32_t kTmemColumns = 512;     // S of both groups, O of both groups
 constexpr float kStale = 8.0f;             // how far (log2) a tile's maximum may exceed the row's before it moves
-constexpr float kLowest = -3.0e38f;        // the maximum of scores that are all -inf: 2^(-inf - m) is 0, and any other exceeds it
+constexpr float kLowest = -3.0e38f;        // the maximum of scores that are all -inf (2^(-inf - m) is 0, and any other exceeds it) or NaN
 constexpr int kOwnStart = 1;               // what an item of own keys costs beside its tiles, in tiles
 constexpr int kPrefixStart = 2;            // and what one of the prefix does
 
@@ -798,7 +798,7 @@ prefix_attention_kernel(const __grid_constant__ CUtensorMap prefix_k, const __gr
                     const float here = a.scale_log2 * fmaxf(max3(max3(most[0], most[1], most[2]), most[3], most[4]),
                                                             max3(most[5], most[6], most[7]));
                     if (tile == 0) {
-                        m = here == -INFINITY ? kLowest : here - kLift;
+                        m = here > -INFINITY ? here - kLift : kLowest;  // (NaN too: l is NaN then, and m says that it was stored)
                     } else if (__any_sync(0xFFFFFFFFu, row < live && here - kLift > m + kStale)) {
                         const float next = here - kLift > m + kStale ? here - kLift : m, by = exp2_approx(m - next);
                         m = next;
