@@ -268,17 +268,21 @@ class Int4Decoder:
     def score(self, tokens: torch.Tensor, positions: torch.Tensor, given: torch.Tensor, top: int = 0):
         """One step, and of its logits the log probabilities of the tokens `given` [B] to come next, the
         entropy of every row and its `top` most probable tokens (`glue.TokenLogprobs`; a negative
-        token is none)."""
+        token is none, one past the vocabulary gives NaN, which the kernel reports by `decoder_status`)."""
         from . import glue
 
+        if given.dim() != 1 or given.shape != tokens.shape or given.dtype is not torch.int64:
+            raise ValueError(f"score: `given` is an int64 tensor of {tokens.numel()} tokens, not {given.dtype}{list(given.shape)}")
         logits = self.step(tokens, positions)
         if self.fused:
             return glue.token_logprobs(logits, given, top)
+        vocab = logits.shape[1]
         logp = torch.log_softmax(logits.float(), dim=-1)
         best = logp.topk(top, dim=-1)
         # 0 * -inf of a forbidden token adds nothing to the entropy
         entropy = -(logp.exp() * logp.clamp_min(torch.finfo(torch.float32).min)).sum(dim=-1)
-        logprob = logp.gather(1, given.clamp_min(0)[:, None])[:, 0].masked_fill(given < 0, 0.0)
+        logprob = logp.gather(1, given.clamp(0, vocab - 1)[:, None])[:, 0]
+        logprob = logprob.masked_fill(given >= vocab, float("nan")).masked_fill(given < 0, 0.0)
         return glue.TokenLogprobs(logprob, entropy, best.values, best.indices)
 
     def _attend(self, layer: int, qkv: torch.Tensor, positions: torch.Tensor, nq: int, nkv: int) -> torch.Tensor:

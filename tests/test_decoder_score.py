@@ -1,0 +1,91 @@
+"""`Int4Decoder.score` at its edges, on the plain route and on the fused one: tokens past the vocabulary,
+none given, equal logits, forbidden tokens, and what is refused.  `step` is replaced by one that
+returns given logits, so that both routes have the same."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from linnet_b200 import decoder as dec
+from linnet_b200 import glue
+from tests import decoder_util as du
+
+VOCAB = dec.DecoderConfig.tiny().vocab
+
+
+def scorer(logits: torch.Tensor, fused: bool) -> dec.Int4Decoder:
+    cfg = dec.DecoderConfig.tiny()
+    model = du.rank_model(cfg, du.whole_model(cfg), 0, 1, du.oracle_linear)
+    model.fused = fused
+    model.step = lambda tokens, positions: logits
+    return model
+
+
+def rows() -> torch.Tensor:
+    """Logits of few different values (so that most have equals), one row of one value, one row with
+    most tokens forbidden, one with all of them, one that holds NaN."""
+    gen = torch.Generator().manual_seed(5)
+    logits = torch.randint(-4, 5, (7, VOCAB), generator=gen).to(torch.bfloat16)
+    logits[1] = 0.5
+    logits[2, torch.rand(VOCAB, generator=gen) < 0.97] = -math.inf
+    logits[3] = -math.inf
+    logits[4, 100] = math.nan
+    logits[5, ::2] = -0.0
+    logits[5, 1::2] = 0.0
+    return logits
+
+
+GIVEN = [3, VOCAB, 7, 1, -1, VOCAB - 1, 1 << 40]
+
+
+def check(got: glue.TokenLogprobs, logits: torch.Tensor, top: int) -> None:
+    """f32 sums of VOCAB terms: VOCAB * 2^-24 relative at the worst, and as much of numbers below 16."""
+    logits = logits.double().cpu()
+    want = logits - torch.logsumexp(logits, dim=-1, keepdim=True)
+    given = torch.tensor(GIVEN)
+    logprob = want.gather(1, given.clamp(0, VOCAB - 1)[:, None])[:, 0]
+    logprob[given >= VOCAB], logprob[given < 0] = math.nan, 0.0
+    near = dict(rtol=VOCAB * 2.0 ** -24, atol=16 * VOCAB * 2.0 ** -24, equal_nan=True)
+    torch.testing.assert_close(got.logprob.double().cpu(), logprob, **near)
+    entropy = -torch.special.xlogy(want.exp(), want.exp()).sum(dim=-1)
+    torch.testing.assert_close(got.entropy.double().cpu(), entropy, **near)
+    order = torch.tensor([sorted(range(VOCAB), key=lambda i: (-row[i], i))[:top] for row in logits.nan_to_num(nan=-math.inf).tolist()]).long()
+    plain = [r for r in range(len(GIVEN)) if r != 4]  # where NaN stands in the order is not said
+    assert torch.equal(got.top_tokens.cpu()[plain], order[plain])
+    torch.testing.assert_close(got.top_logprobs.double().cpu()[plain], want.gather(1, order)[plain], **near)
+    assert bool(got.top_logprobs[4].isnan().all())
+
+
+def run(fused: bool, device: str, top: int) -> None:
+    logits = rows().to(device)
+    at = torch.zeros(len(GIVEN), dtype=torch.long, device=device)
+    check(scorer(logits, fused).score(at, at, torch.tensor(GIVEN, device=device), top=top), logits, top)
+
+
+@pytest.mark.parametrize("top", [0])
+def test_edges_of_the_plain_route(top):
+    run(False, "cpu", top)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fused", [False, True])
+def test_edges_on_a_gpu(fused):
+    for top in (0,):
+        run(fused, "cuda", top)
+    if fused:
+        with pytest.raises(ValueError, match="batch row"):
+            glue.decoder_status()
+    glue.decoder_status()
+
+
+@pytest.mark.parametrize("fused", [False, True])
+@pytest.mark.parametrize("given", [torch.tensor([1]), torch.tensor([[1, 2]]), torch.tensor([1, 2], dtype=torch.int32)])
+def test_tokens_that_are_refused(given, fused):
+    """Before the step: the caches are not written for a call that fails."""
+    model = scorer(torch.zeros(2, VOCAB), fused)
+    model.step = None
+    with pytest.raises(ValueError, match="given"):
+        model.score(torch.zeros(2, dtype=torch.long), torch.zeros(2, dtype=torch.long), given)
