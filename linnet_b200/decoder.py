@@ -277,13 +277,17 @@ class Int4Decoder:
         if self.fused:
             return glue.token_logprobs(logits, given, top)
         vocab = logits.shape[1]
-        logp = torch.log_softmax(logits.float(), dim=-1)
-        best = logp.topk(top, dim=-1)
+        if not 0 <= top <= vocab:
+            raise ValueError(f"score: 0 to {vocab} alternatives of a row, not {top}")
+        logits = logits.float()
+        logp = torch.log_softmax(logits, dim=-1)
+        # (stable: the lower index first among equals; by the logits, which may differ where their logarithms do not)
+        best = (torch.sort(logits, dim=-1, descending=True, stable=True).indices if top else given.new_empty(len(logits), 0))[:, :top]
         # 0 * -inf of a forbidden token adds nothing to the entropy
         entropy = -(logp.exp() * logp.clamp_min(torch.finfo(torch.float32).min)).sum(dim=-1)
         logprob = logp.gather(1, given.clamp(0, vocab - 1)[:, None])[:, 0]
         logprob = logprob.masked_fill(given >= vocab, float("nan")).masked_fill(given < 0, 0.0)
-        return glue.TokenLogprobs(logprob, entropy, best.values, best.indices)
+        return glue.TokenLogprobs(logprob, entropy, logp.gather(1, best), best)
 
     def _attend(self, layer: int, qkv: torch.Tensor, positions: torch.Tensor, nq: int, nkv: int) -> torch.Tensor:
         """Rotary positions, cache write and attention of the fused routes: over a row's cache, or

@@ -65,7 +65,7 @@ def run(fused: bool, device: str, top: int) -> None:
     check(scorer(logits, fused).score(at, at, torch.tensor(GIVEN, device=device), top=top), logits, top)
 
 
-@pytest.mark.parametrize("top", [0])
+@pytest.mark.parametrize("top", [0, 1, 5, 32, VOCAB])
 def test_edges_of_the_plain_route(top):
     run(False, "cpu", top)
 
@@ -73,7 +73,7 @@ def test_edges_of_the_plain_route(top):
 @pytest.mark.gpu
 @pytest.mark.parametrize("fused", [False, True])
 def test_edges_on_a_gpu(fused):
-    for top in (0,):
+    for top in (0, 1, 5, 32):
         run(fused, "cuda", top)
     if fused:
         with pytest.raises(ValueError, match="batch row"):
@@ -89,3 +89,10 @@ def test_tokens_that_are_refused(given, fused):
     model.step = None
     with pytest.raises(ValueError, match="given"):
         model.score(torch.zeros(2, dtype=torch.long), torch.zeros(2, dtype=torch.long), given)
+
+
+@pytest.mark.parametrize("top", [-1, VOCAB + 1])
+def test_alternatives_that_are_refused(top):
+    at = torch.zeros(2, dtype=torch.long)
+    with pytest.raises(ValueError, match="alternatives"):
+        scorer(torch.zeros(2, VOCAB), False).score(at, at, at, top=top)
