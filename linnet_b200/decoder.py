@@ -122,10 +122,15 @@ def check_tp(cfg: DecoderConfig, tp: int) -> None:
         raise ValueError(f"{tp} shards do not divide the vocabulary or the MLP width")
 
 
+def plain_frequencies(half: int, theta: float, device: torch.device) -> torch.Tensor:
+    """Frequencies f32 [half] of unscaled positions, as `rotary` and (on a GPU) `glue.rope_table` have them."""
+    return theta ** (-torch.arange(half, device=device, dtype=torch.float32) / half)
+
+
 def rotary(x: torch.Tensor, positions: torch.Tensor, theta: float) -> torch.Tensor:
     """Rotary embedding of `x` [B, heads, D] at `positions` [B] (halves rotated)."""
     half = x.shape[-1] // 2
-    freqs = theta ** (-torch.arange(half, device=x.device, dtype=torch.float32) / half)
+    freqs = plain_frequencies(half, theta, x.device)
     angle = positions.to(torch.float32)[:, None] * freqs[None, :]
     cos, sin = angle.cos()[:, None, :], angle.sin()[:, None, :]
     a, b = x[..., :half].float(), x[..., half:].float()
@@ -211,7 +216,14 @@ class Int4Decoder:
         return keys, values
 
     def _make_frequencies(self) -> None:
-        if self.frequencies is None:
+        if self.frequencies is not None:
+            return
+        if self.cfg.rope_scaling is None:
+            # A prompt's keys stand in its cache as turned by these f32 numbers: answers turned by exact ones would be
+            # off against them by as much as the numbers are, times the prompt's length.
+            plain = plain_frequencies(self.cfg.head_dim // 2, self.cfg.rope_theta, self.embed.device)
+            self.frequencies, self.rope_factor = plain.double(), 1.0
+        else:
             numbers, self.rope_factor = frequencies(self.cfg.head_dim, self.cfg.rope_theta, self.cfg.rope_scaling)
             self.frequencies = torch.tensor(numbers, dtype=torch.float64, device=self.embed.device)
 
