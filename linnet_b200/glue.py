@@ -373,11 +373,13 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     if tokens.dim() != 1:
         raise ValueError(f"token_logprobs: tokens must be an int64 tensor [rows], not {tokens.dtype}{list(tokens.shape)}")
     _words("token_logprobs", "tokens", tokens, rows, index)
-    kept, device = max(top, 0), logits.device
+    if not 0 <= top <= min(32, vocab):
+        raise ValueError(f"token_logprobs: 0 to {min(32, vocab)} alternatives of a row, not {top}")
+    device = logits.device
     logprob = torch.empty(rows, dtype=torch.float32, device=device)
     entropy = torch.empty(rows, dtype=torch.float32, device=device)
-    best = torch.empty(rows, kept, dtype=torch.float32, device=device)
-    best_tokens = torch.empty(rows, kept, dtype=torch.int64, device=device)
+    best = torch.empty(rows, top, dtype=torch.float32, device=device)
+    best_tokens = torch.empty(rows, top, dtype=torch.int64, device=device)
     _launch(index, _lib.load().b200q_token_logprobs,
             logits.data_ptr(), tokens.data_ptr(), logprob.data_ptr(), entropy.data_ptr(), best.data_ptr(),
             best_tokens.data_ptr(), rows, vocab, logits.stride(0), top, _CODES[logits.dtype])
