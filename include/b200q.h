@@ -306,7 +306,8 @@ int32_t b200q_decoder_status(void);
  * numbers i and i + pairs) or of neighbours (layout 1: 2i and 2i + 1), are turned by
  * positions[token] * frequencies[pair] (radians, f64) and multiplied by `factor`; the others
  * are copied.  Angles are formed in f64.  Strides of tokens and heads are in numbers; an
- * output may be its input, and otherwise must not overlap any tensor of the call.  head_dim
+ * output may be its input, and otherwise must not overlap any tensor of the call (one that overlaps
+ * itself is refused).  head_dim
  * up to 1024. */
 int32_t b200q_rotary(const void* q, const void* k, const int64_t* positions,
                      const double* frequencies, void* q_out, void* k_out, int64_t tokens,

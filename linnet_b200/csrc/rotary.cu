@@ -268,6 +268,22 @@ int32_t check_rotary(const char* who, int64_t tokens, int64_t nq, int64_t nkv, i
     return B200Q_OK;
 }
 
+// Whether heads of an output share memory.  (A sufficient rule for those that do not: the farther apart of its two
+// dimensions steps over all that the nearer one spans.)
+bool overlaps_itself(int64_t tokens, int64_t token_stride, int64_t heads, int64_t head_stride, int64_t head_dim) {
+    __int128 inner = head_stride, outer = token_stride;
+    int64_t inner_count = heads, outer_count = tokens;
+    if (inner < 0) inner = -inner;
+    if (outer < 0) outer = -outer;
+    if (outer_count <= 1 || (inner_count > 1 && outer < inner)) {
+        const __int128 stride = inner;
+        const int64_t count = inner_count;
+        inner = outer, inner_count = outer_count, outer = stride, outer_count = count;
+    }
+    if (inner_count <= 1) return outer_count > 1 && outer < head_dim;
+    return inner < head_dim || (outer_count > 1 && outer < inner * (inner_count - 1) + head_dim);
+}
+
 }  // namespace
 }  // namespace b200q
 
@@ -283,6 +299,9 @@ extern "C" int32_t b200q_rotary(const void* q, const void* k, const int64_t* pos
     B200Q_REQUIRE(q && q_out && positions && frequencies && (nkv == 0 || (k && k_out)) && aligned(q, 2) && aligned(q_out, 2) &&
                       aligned(k, 2) && aligned(k_out, 2) && aligned(positions, 8) && aligned(frequencies, 8),
                   "rotary: null or misaligned tensor");
+    B200Q_REQUIRE(!overlaps_itself(tokens, q_out_token, nq, q_out_head, head_dim) &&
+                      (nkv == 0 || !overlaps_itself(tokens, k_out_token, nkv, k_out_head, head_dim)),
+                  "rotary: an output overlaps itself");
     RotaryArgs a = {};
     a.src[0] = static_cast<const uint16_t*>(q), a.dst[0] = static_cast<uint16_t*>(q_out);
     a.src[1] = static_cast<const uint16_t*>(k), a.dst[1] = static_cast<uint16_t*>(k_out);

@@ -6,7 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from linnet_b200 import glue
+from linnet_b200 import _lib, glue
 
 
 @pytest.mark.gpu
@@ -19,3 +19,51 @@ def test_alternatives_that_there_are_none_of(top):
     with pytest.raises(ValueError, match="alternatives of a row"):
         glue.token_logprobs(logits, tokens, top)
     assert torch.cuda.memory_stats()["allocation.all.allocated"] == before
+
+
+def _rotary_status(tokens, nq, nkv, head_dim, q_out, k_out) -> str:
+    """What `b200q_rotary` says of outputs of these strides (of tokens and heads)."""
+    lib, memory = _lib.load(), torch.zeros(64, dtype=torch.float64)
+    at = memory.data_ptr()
+    dense = (nq * head_dim, head_dim, nkv * head_dim, head_dim)
+    status = lib.b200q_rotary(at, at, at, at, at, at, tokens, nq, nkv, head_dim, 1, *dense, *q_out, *k_out, 1.0, 0, 1, None)
+    return _lib.last_error() if status else ""
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="host memory: only where no kernel can be launched")
+@pytest.mark.parametrize("tokens,nq,nkv,head_dim,q_out,k_out,wrong", [
+    (3, 2, 1, 64, (0, 64), (64, 64), True),           # the same memory for every token
+    (3, 2, 1, 64, (128, 0), (64, 64), True),          # for every head
+    (3, 2, 1, 64, (64, 64), (64, 64), True),          # a token's second head is the next one's first
+    (3, 2, 1, 64, (127, 64), (64, 64), True),
+    (3, 2, 1, 64, (64, 191), (64, 64), True),         # [heads, tokens, D], a number short
+    (3, 2, 2, 64, (128, 64), (128, 32), True),        # keys
+    (3, 2, 1, 64, (128, 64), (63, 64), True),
+    (3, 1, 1, 64, (-32, 0), (64, 64), True),
+    (3, 2, 1, 64, (64, 192), (64, 64), False),        # [heads, tokens, D]
+    (3, 2, 1, 64, (-128, 64), (-64, 64), False),
+    (1, 2, 1, 64, (0, 64), (0, 0), False),            # of one token or head the stride is not read
+    (3, 1, 1, 64, (64, 0), (64, 0), False),
+    (1, 1, 1, 64, (0, 0), (0, 0), False),
+    (3, 2, 1, 64, (1 << 62, 64), (64, 1 << 62), False)])
+def test_rotary_outputs_that_overlap_themselves(tokens, nq, nkv, head_dim, q_out, k_out, wrong):
+    """What is taken goes on to the launch, which fails here for want of a GPU."""
+    said = _rotary_status(tokens, nq, nkv, head_dim, q_out, k_out)
+    assert said and ("overlaps itself" in said) == wrong, said
+
+
+@pytest.mark.gpu
+def test_rotary_refuses_an_expanded_output():
+    q = torch.randn(4, 6, 64, device="cuda", dtype=torch.bfloat16)
+    positions, freq = torch.arange(4, device="cuda"), torch.ones(32, device="cuda", dtype=torch.float64)
+    want, _ = glue.rotary(q, None, positions, freq)
+    for out in (torch.empty_like(q[:1]).expand(4, 6, 64), torch.empty_like(q[:, :1]).expand(4, 6, 64)):
+        with pytest.raises(ValueError, match="overlaps itself"):
+            glue.rotary(q, None, positions, freq, out=(out, None))
+        with pytest.raises(ValueError, match="overlaps itself"):
+            glue.rotary(q, q, positions, freq, out=(torch.empty_like(q), out))
+    by_head = torch.empty(6, 4, 64, device="cuda", dtype=torch.bfloat16).transpose(0, 1)
+    wide = torch.empty(4, 20, 72, device="cuda", dtype=torch.bfloat16)[:, 3:9, :64]
+    for out in (by_head, wide, q):
+        got, _ = glue.rotary(q.clone() if out is not q else q, None, positions, freq, out=(out, None))
+        assert got is out and torch.equal(out, want)
