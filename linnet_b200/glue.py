@@ -8,7 +8,7 @@ of a head (`csrc/rotary.cu`: `rotary`, `rotary_cache`, `rotary_table`; `rope_fre
 frequencies), attention over one shared prefix and each row's own cache
 (`csrc/prefix_attention.cu`: `prefix_attention`), and log probabilities of given tokens with entropy
 and alternatives (`csrc/token_logprobs.cu`: `token_logprobs`).  These have no derivative and refuse
-tensors that ask for one."""
+tensors that ask for one, in reverse or in forward mode."""
 
 from __future__ import annotations
 
@@ -18,6 +18,7 @@ import struct
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, rope
 from .kernels import _CODES, _current_device, _raw_stream
@@ -163,9 +164,16 @@ def _same(who: str, kinds: tuple[torch.dtype, ...], *tensors: torch.Tensor) -> i
                                f"{[f'{t.dtype} on {t.device}' for t in tensors]}")
         if not t.is_contiguous() and t.stride(-1) != 1 and t.numel() > 0 and t.shape[-1] > 1:
             raise RuntimeError(f"{who}: the last dimension has to be contiguous")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError(f"{who} has no derivative: detach its inputs or call it under torch.no_grad()")
+        if t.requires_grad or forward_ad._current_level >= 0:
+            _no_derivative(who, t)
     return index
+
+
+def _no_derivative(who: str, t: torch.Tensor) -> None:
+    """Of a tensor that may ask for one.  (A forward-mode tangent counts under torch.no_grad() too, which leaves that
+    mode on.)"""
+    if (t.requires_grad and torch.is_grad_enabled()) or forward_ad.unpack_dual(t).tangent is not None:
+        raise RuntimeError(f"{who} has no derivative: detach its inputs or call it under torch.no_grad()")
 
 
 def _launch(index: int, entry, *args) -> None:
@@ -205,6 +213,8 @@ def _frequencies(who: str, frequencies: torch.Tensor, head_dim: int, index: int)
             or frequencies.dim() != 1 or not 1 <= pairs <= head_dim // 2):
         raise ValueError(f"{who}: frequencies must be a contiguous float64 tensor of 1 to {head_dim // 2} entries on "
                          f"cuda:{index}, not {frequencies.dtype}{list(frequencies.shape)} on {frequencies.device}")
+    if frequencies.requires_grad or forward_ad._current_level >= 0:
+        _no_derivative(who, frequencies)
     return pairs
 
 

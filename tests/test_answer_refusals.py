@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from linnet_b200 import _lib, glue
 
@@ -67,3 +68,52 @@ def test_rotary_refuses_an_expanded_output():
     for out in (by_head, wide, q):
         got, _ = glue.rotary(q.clone() if out is not q else q, None, positions, freq, out=(out, None))
         assert got is out and torch.equal(out, want)
+
+
+def _dual(t: torch.Tensor) -> torch.Tensor:
+    return forward_ad.make_dual(t, torch.ones_like(t))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["rotary", "rotary_cache", "prefix_attention", "token_logprobs"])
+def test_tangents_are_refused(which):
+    """In forward mode too there is no derivative, and none is dropped: an input with a tangent is refused,
+    under torch.no_grad as well (which leaves forward mode on); one without passes."""
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    make = lambda *shape: torch.randn(*shape, device="cuda", generator=gen).bfloat16()  # noqa: E731
+    freq, at = torch.ones(32, device="cuda", dtype=torch.float64), torch.zeros(3, device="cuda", dtype=torch.long)
+    calls = {
+        "rotary": (lambda q, k: glue.rotary(q, k, at, freq), [make(3, 4, 64), make(3, 2, 64)]),
+        "rotary_cache": (lambda x, k, v: glue.rotary_cache(x, at, freq, k, v, 4, 2), [make(3, 8 * 64), make(3, 2, 5, 64), make(3, 2, 5, 64)]),
+        "prefix_attention": (lambda q, a, b, c, d: glue.prefix_attention(q, a, b, c, d, at),
+                             [make(3, 4, 64), make(2, 9, 64), make(2, 9, 64), make(3, 2, 5, 64), make(3, 2, 5, 64)]),
+        "token_logprobs": (lambda x: glue.token_logprobs(x, at), [make(3, 100)])}
+    call, inputs = calls[which]
+    with forward_ad.dual_level():
+        call(*inputs)
+        for i in range(len(inputs)):
+            with pytest.raises(RuntimeError, match="no derivative"):
+                call(*[_dual(t) if j == i else t for j, t in enumerate(inputs)])
+            with torch.no_grad(), pytest.raises(RuntimeError, match="no derivative"):
+                call(*[_dual(t) if j == i else t for j, t in enumerate(inputs)])
+    with pytest.raises(RuntimeError, match="no derivative"):
+        torch.func.jvp(call, tuple(inputs), tuple(torch.ones_like(t) for t in inputs))
+    call(*inputs)
+
+
+@pytest.mark.gpu
+def test_frequencies_that_ask_for_a_derivative_are_refused():
+    q, at = torch.randn(3, 4, 64, device="cuda").bfloat16(), torch.zeros(3, device="cuda", dtype=torch.long)
+    qkv, cache = torch.randn(3, 8 * 64, device="cuda").bfloat16(), torch.zeros(2, 3, 2, 5, 64, device="cuda", dtype=torch.bfloat16)
+    freq = torch.ones(32, device="cuda", dtype=torch.float64)
+    calls = (lambda f: glue.rotary(q, None, at, f), lambda f: glue.rotary_cache(qkv, at, f, cache[0], cache[1], 4, 2),
+             lambda f: glue.rotary_table(9, f))
+    for call in calls:
+        with pytest.raises(RuntimeError, match="no derivative"):
+            call(freq.clone().requires_grad_())
+        with torch.no_grad():
+            call(freq.clone().requires_grad_())
+        with forward_ad.dual_level():
+            call(freq)
+            with pytest.raises(RuntimeError, match="no derivative"):
+                call(_dual(freq))
