@@ -96,3 +96,72 @@ def test_alternatives_that_are_refused(top):
     at = torch.zeros(2, dtype=torch.long)
     with pytest.raises(ValueError, match="alternatives"):
         scorer(torch.zeros(2, VOCAB), False).score(at, at, at, top=top)
+
+
+# ---- every step of sampled answers, by itself ----------------------------------------------------
+
+STEPS, BATCH = 6, 6
+
+
+def _model(fused: bool) -> dec.Int4Decoder:
+    device, linear = "cpu", du.oracle_linear
+    if fused:
+        from linnet_b200 import kernels
+
+        device, linear = "cuda", kernels.int4_linear
+    cfg = dec.DecoderConfig.tiny()
+    model = du.rank_model(cfg, du.whole_model(cfg), 0, 1, linear, device=device)
+    model.fused = fused
+    return model
+
+
+def _furthest(model: dec.Int4Decoder, prompt: list[int], planted: int | None = None) -> list[float]:
+    """How far each step's log probabilities of answers that share the prompt (of the token given and of
+    eight alternatives, the worst of all rows) are from those of rows that step through prompt and answer
+    by themselves on the plain route, as a share of what is allowed.  Two routes' logits differ by 3 % of
+    the largest (`tests/test_decoder_shared.py`), a logit less the logarithm of a sum by twice that.
+    `planted`: at this step the prompt is taken for one position shorter."""
+    device = model.embed.device
+    gen = torch.Generator().manual_seed(23)
+    chosen = torch.randint(0, VOCAB, (STEPS + 1, BATCH), generator=gen)
+    plain = _model(False)
+    plain.allocate_cache(BATCH)
+    sequence = [torch.full((BATCH,), token) for token in prompt] + list(chosen)
+    want = []
+    for at, token in enumerate(sequence[:-1]):
+        logits = plain.step(token, torch.full((BATCH,), at)).double()
+        if at >= len(prompt):
+            want.append((torch.log_softmax(logits, dim=-1), 2 * 3e-2 * logits.abs().max().item()))
+    model.allocate_cache(1)
+    for at, token in enumerate(prompt):
+        model.step(torch.tensor([token], device=device), torch.tensor([at], device=device))
+    model.share_prefix(len(prompt), BATCH, STEPS)
+    out = []
+    for t, (exact, allowed) in enumerate(want):
+        model.prefix_length.fill_(len(prompt) - (t == planted))
+        got = model.score(chosen[t].to(device), torch.full((BATCH,), t, device=device), chosen[t + 1].to(device), top=8)
+        tokens = torch.cat([chosen[t + 1][:, None], got.top_tokens.cpu()], dim=1)
+        mine = torch.cat([got.logprob[:, None], got.top_logprobs], dim=1).double().cpu()
+        out.append((mine - exact.gather(1, tokens)).abs().max().item() / allowed)
+    return out
+
+
+PROMPTS = [[7, 301, 12, 44, 44, 9, 250], [(i * 97) % VOCAB for i in range(25)]]
+
+
+@pytest.mark.parametrize("prompt", PROMPTS, ids=["short", "longer"])
+def test_every_step_of_the_plain_route(prompt):
+    assert max(_furthest(_model(False), prompt)) <= 1.0
+
+
+def test_a_step_at_the_wrong_position_shows():
+    """A test of the tests around it."""
+    share = _furthest(_model(False), PROMPTS[0], planted=3)
+    assert max(share[:3]) <= 1.0 < share[3]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("prompt", PROMPTS, ids=["short", "longer"])
+def test_every_step_of_the_fused_route(prompt):
+    assert max(_furthest(_model(True), prompt)) <= 1.0
+    glue.decoder_status()
