@@ -32,12 +32,15 @@
 // and rescales O and l in tensor memory (rare: P stays below 2^8, and the sums are f32 anyway).
 // P is rounded to the tensors' type, as the product takes it; l sums P before that rounding.
 //
+// Registers are handed out to four warps at a time, so that 13 warps leave a thread 128: some 40 bytes of it are spilled.
+//
 // What bounds it, measured on a B200 (nq 32, nkv 8, D 128, bf16; join included): few rows, HBM and the
-// start of the pipeline: 8 rows of 65536 keys 53 us, 5.1 TB/s; 64 rows of 8192 + up to 512 own keys
-// 36 us where the bytes take 15.6; 2 rows of 100 keys 8.4 us, two launches and their latencies.  Many
-// rows, the chain from scores to weights to the next scores, at the clock that the power limit leaves (1.4 to
-// 1.7 GHz): 256 rows of 65536 keys 284 us, 960 TFLOP/s (58 % of measured).  A tile of both groups takes
-// some 2000 clocks there; its products alone take 1300, its 16384 exponentials 1024, its 32 KB 700.
+// start of the pipeline: 8 rows of 65536 keys 56 us, 4.8 TB/s; 64 rows of 8192 + up to 512 own keys
+// 37 us where the bytes take 15.6; 2 rows of 100 keys 8.5 us, two launches and their latencies.  Many
+// rows, the chain from scores to weights to the next scores: 256 rows of 16384 + up to 128 own keys 108 us, 640 TFLOP/s,
+// and 117 in a run of a second, which the power limit takes to 1.8 GHz; of 65536 keys 313 us, 880 TFLOP/s (53 % of
+// measured).  A tile of both groups takes some 2000 clocks there; its products alone take 1300, its 16384
+// exponentials 1024, its 32 KB 700.
 #include "mma.cuh"
 #include "umma.cuh"
 

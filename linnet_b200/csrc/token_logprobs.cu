@@ -19,7 +19,12 @@
 //
 // Measured on a B200, rows of 128256: 2048 of bf16 with 5 alternatives 102 us, 5.1 TB/s (92 without:
 // 5.7 TB/s), of f32 162 us, 6.5 TB/s; 64 of f32 12.5 us; one of bf16 with 20 alternatives 8.9 us, half of
-// it the way from the last logit over the cluster's barrier to the ranked list.
+// it the way from the last logit over the cluster's barrier to the ranked list.  (2048 of bf16 in a run of a second, at
+// the clock that the power limit leaves, 1.84 GHz: 107 us.)
+//
+// Slow is a row of no more groups than alternatives: no group can be left out, and a block bisects over all of its
+// elements.  1000 bf16 rows of 1000 logits 27 us with 20 alternatives, 70 with 99 % of them forbidden, 7 without
+// alternatives; of 2890, 63, 83 and 8; of 8200 logits 18, 18 and 9.
 #include <cooperative_groups.h>
 
 #include "mma.cuh"
@@ -165,7 +170,8 @@ __device__ __forceinline__ void add(const float (&x)[E], float m, float2& l, flo
 }
 
 // With alternatives, five blocks a multiprocessor: one's ranking goes by while the others read.  2048 rows with five:
-// 102 us so, 106 with four, 120 with three, 142 with six (of 40 registers each); f32 162, 173, 184, 175.
+// 102 us so (of 48 registers, with 44 bytes spilled), 106 with four, 120 with three, 142 with six (of 40 registers each);
+// f32 162 (of 46, nothing spilled), 173, 184, 175.
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kThreads, TOP ? 5 : 0)
 token_logprobs_kernel(const __grid_constant__ LogprobArgs a) {
@@ -521,8 +527,10 @@ extern "C" int32_t b200q_token_logprobs(const void* logits, const int64_t* token
     a.groups = int((vocab + elements - 1 + 32 * elements - 1) / (32 * elements));  // of a row wherever it starts
     a.status = decoder_error_word();
     // Blocks a row: twice as many while there are fewer than four a multiprocessor and each has a round of its own.
-    // 64 f32 rows of 128256: 12.5 us with eight blocks each, 29.6 with one; 148: 20.6 with four, 25.3 with two, 24.6 with
-    // eight; 333 f16 rows of 32003: 9.8 with one, 10.0 with two, 13.9 with four.
+    // With five alternatives, 64 f32 rows of 128256: 12.7 us with eight blocks each, 30.1 with one; 148: 19.8 with four, 25.0
+    // with two, 23.0 with eight; 333: 33.2 with two, 41.7 with one.  The rule knows neither the type nor how many blocks are
+    // resident (four to six a multiprocessor), and costs some rows a second round of them: 333 16-bit rows of 32003 without
+    // alternatives take 10.4 with its two and 10.0 with one, 222 of them 10.3 with its four and 7.6 with two.
     const int64_t each = int64_t(kWarps) * kHeld;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t err = cudaSuccess;
